@@ -52,6 +52,9 @@ enum {
     TRC_CUDA_TYPE_Q8_0 = 8
 };
 
+/* ggml type ids of the half-precision element types that a low-rank adapter may be held in. */
+enum { TRC_CUDA_TYPE_F16 = 1, TRC_CUDA_TYPE_BF16 = 30 };
+
 /* One ggml tensor view in device memory (the fields of Tensor that the kernels need:
  * include/traincpp/trc_tensor.h:37-70; data = buffer base + Tensor::data_offset). */
 typedef struct trc_cuda_view {
@@ -334,6 +337,117 @@ int    trc_cuda_sum_sqr_acc(float* acc, const float* a, int64_t n, void* workspa
  * Replaces compute_clip_scale_inplace (src/backends/cpu/trc_cpu_ops.cpp:1594-1611),
  * OP_CLIP_SCALE_INPLACE. */
 int trc_cuda_clip_scale_inplace(float* a, int64_t n, const float* norm, float max_norm, float eps, void* stream);
+
+/* ------------------------------------------------------------------ low-rank adapters
+ * y = base + scale * B (A x) beside a shared projection: `base` is what trc_cuda_mul_mat or
+ * trc_cuda_mul_mat_q made of the frozen weight, and every row (token) has the adapter of its own
+ * request. No reference counterpart. F32 activations, F32 accuracy (3xTF32 products, sums in fp32). */
+
+#define TRC_CUDA_LORA_MAX_ADAPTERS 256 /* adapters of one call */
+#define TRC_CUDA_LORA_MAX_RANK     256
+
+/* One adapter, its factors in device memory as GGUF adapter files hold them, without padding.
+ * da and db (F32, the factors' shapes) receive the gradients in trc_cuda_lora_back; a null one is not
+ * computed. trc_cuda_lora does not look at them. */
+typedef struct trc_cuda_lora_adapter {
+    const void* a;     /* lora_a: ne = {K, rank} */
+    const void* b;     /* lora_b: ne = {rank, N} */
+    float*      da;
+    float*      db;
+    float       scale; /* alpha / rank, or what the caller takes for it */
+    int32_t     rank;  /* 1 .. TRC_CUDA_LORA_MAX_RANK; adapters of one call may differ */
+} trc_cuda_lora_adapter;
+
+/* Floats of one row of the buffer `h` for these adapters (the largest rank rounded up to 16); a
+ * negative status if one of them is not valid. */
+int64_t trc_cuda_lora_h_ld(const trc_cuda_lora_adapter* adapters, int n_adapters);
+
+/* d[:, t] = base[:, t] + scale * B (A x[:, t]) with the adapter ids[t] of row t.
+ * x has ne = {K, n1, n2, n3}, base and d have ne = {N, n1, n2, n3}, any byte strides; t counts the
+ * n1*n2*n3 rows in ggml order. `type` is the element type of every A and B: TRC_CUDA_TYPE_F32,
+ * _F16 or _BF16. `adapters` is a HOST array, passed to the kernels by value.
+ *   - ids: device array of one int32 per row. A row whose id is outside 0 .. n_adapters-1 (say -1) has
+ *     no adapter: d = base, and its x is not read. Null ids give every row adapter 0. Any order is
+ *     right; rows of one adapter side by side are fastest.
+ *   - base may be null (d = the adapter's part alone) and may be d itself; d may not overlap x or
+ *     base in another way.
+ *   - h: device buffer of rows * trc_cuda_lora_h_ld() floats, 16-byte aligned. It receives
+ *     scale * A x (zeros behind a row's rank, and for a row without an adapter), which
+ *     trc_cuda_lora_back takes.
+ * Each output is the same whatever the other rows hold. A row with an infinity or a NaN in x
+ * gives infinities or NaN in that row alone. */
+int trc_cuda_lora(int type, const trc_cuda_lora_adapter* adapters, int n_adapters, const int32_t* ids,
+                  const trc_cuda_view* x, const trc_cuda_view* base, const trc_cuda_view* d, float* h,
+                  void* stream);
+
+/* Bytes of device workspace trc_cuda_lora_back needs for that many rows (0 if an adapter is not valid). */
+size_t trc_cuda_lora_back_workspace_bytes(const trc_cuda_lora_adapter* adapters, int n_adapters, int64_t rows);
+
+/* The gradients of trc_cuda_lora for the upstream gradient dy (ne = {N, n1, n2, n3}), with
+ * g[t] = scale * B^T dy[:, t]:
+ *     dx[:, t] = base[:, t] + A^T g[t]                       (base null: the adapter's part alone)
+ *     da (+)= sum over the adapter's rows of g[t] x[:, t]^T,  db (+)= sum of dy[:, t] h[t]^T
+ * h is what trc_cuda_lora wrote for the same x, ids and adapters. dx may be null (no gradient of x
+ * wanted) and base may be dx itself (the gradient that the shared projection's backward left there).
+ * flags: TRC_CUDA_MM_ACCUMULATE adds to da and db, 0 overwrites them (with zeros for an adapter
+ * without rows). Sums over rows are taken in a fixed order: equal calls give equal bits. dx overlaps
+ * nothing but base, and the gradients of two adapters do not overlap. workspace: device memory, 16-byte
+ * aligned; calls that may run at the same time need one each. */
+int trc_cuda_lora_back(int type, const trc_cuda_lora_adapter* adapters, int n_adapters, const int32_t* ids,
+                       const trc_cuda_view* x, const trc_cuda_view* dy, const float* h, const trc_cuda_view* base,
+                       const trc_cuda_view* dx, void* workspace, size_t workspace_bytes, uint32_t flags,
+                       void* stream);
+
+/* ------------------------------------------------------------------ the optimizer over many tensors
+ * One launch (per 256 tensors) for a step that trc_cuda_opt_step_adamw takes tensor by tensor, with
+ * the states in 32 bits, or in 8 bits with one float scale for each TRC_CUDA_STATE8_BLOCK
+ * elements of a tensor (its last block may be shorter). The 8-bit forms:
+ *     first moment   m = c |c| scale,        c an int8 in -127 .. 127   (scale = max|m| / 127^2)
+ *     second moment  sqrt(v) = c c scale,    c a uint8                  (scale = max sqrt(v) / 255^2)
+ * The square law spends the codes on small values: neighbouring codes at the top are 1.6 % (m) and
+ * 0.8 % (sqrt(v)) apart, and the smallest nonzero value is 1/16129 (m) and 1/65025 (sqrt(v)) of the block's
+ * largest. Codes are rounded to nearest in the code; a v > 0 never takes the code 0, so no step is
+ * divided by a vanished second moment. A block whose largest |m| is below 2^-100 is stored as zero. A
+ * block that holds an infinity or a NaN gets the scale NaN: all of it reads back as NaN. Zero codes with
+ * zero scales are the initial state. */
+#define TRC_CUDA_STATE8_BLOCK 256
+
+typedef struct trc_cuda_adamw_job {
+    float*       param;
+    const float* grad;
+    void*        m;       /* float, or int8 codes */
+    void*        v;       /* float, or uint8 codes */
+    float*       m_scale; /* 8-bit states: one float per block; not used with 32 bits */
+    float*       v_scale;
+    int64_t      n;       /* >= 0 */
+} trc_cuda_adamw_job;
+
+/* AdamW over n_jobs tensors (HOST array). params6 as for trc_cuda_opt_step_adamw; state_bits is 32
+ * (each element bit for bit what trc_cuda_opt_step_adamw gives) or 8 (the same step from the decoded
+ * states, in fp32; the new states are rounded to their codes after the parameter took its step).
+ * norm (one float, device; may be null): the gradients are first multiplied by
+ * min(1, max_norm / (sqrt(norm[0]) + clip_eps)) as trc_cuda_clip_scale_inplace does; grad itself is left as it
+ * is. Two jobs may not share memory, except that gradients may be shared. */
+int trc_cuda_opt_step_adamw_many(const trc_cuda_adamw_job* jobs, int n_jobs, int state_bits, const float* params6,
+                                 const float* norm, float max_norm, float clip_eps, void* stream);
+
+/* Codes and scales to values and back, for states written to and read from a checkpoint.
+ * which: 0 = first moment (int8), 1 = second moment (uint8; a negative v is taken as NaN). */
+int trc_cuda_state8_to_f32(int which, const void* codes, const float* scales, float* values, int64_t n, void* stream);
+int trc_cuda_state8_from_f32(int which, const float* values, void* codes, float* scales, int64_t n, void* stream);
+
+/* One contiguous run of floats. */
+typedef struct trc_cuda_span {
+    const float* data;
+    int64_t      n; /* >= 0 */
+} trc_cuda_span;
+
+/* *out (one float, device) = (float) sum over all spans of (double) a[i]^2, in a fixed order: what
+ * trc_cuda_sum_sqr_acc over each of them accumulates, rounded once. spans is a HOST array. workspace:
+ * device memory, 8-byte aligned, of at least the stated bytes; it needs no initial value. */
+size_t trc_cuda_sum_sqr_many_workspace_bytes(const trc_cuda_span* spans, int n_spans);
+int    trc_cuda_sum_sqr_many(const trc_cuda_span* spans, int n_spans, float* out, void* workspace,
+                             size_t workspace_bytes, void* stream);
 
 /* ------------------------------------------------------------------ measurement support
  * The dequant kernel's memory traffic without its arithmetic, to measure what HBM delivers for that

@@ -1,0 +1,498 @@
+// optim_many.cu -- the optimizer over many tensors at once: AdamW with 32-bit or 8-bit states, and the
+// squared norm of all gradients that clips it.
+//
+// A low-rank adapter gives two small tensors for every projection, hundreds for a model, so one launch
+// per tensor costs more than its work. Here the tensors of a call are a table in the kernel's parameters,
+// cut into runs of 2048 elements; one CTA takes one run.
+//
+// Every fp32 operation is rounded by itself, in the order of train_ops.cu's adamw_kernel, so the 32-bit
+// form is bit-exact with the one-tensor step and the 8-bit form is the same on every machine.
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <cstdint>
+
+#include "trc_internal.h"
+
+namespace trc {
+
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kRun     = 2048;  // elements of one CTA: 8 per thread, 8 blocks of an 8-bit state
+constexpr int kBlock   = TRC_CUDA_STATE8_BLOCK;
+constexpr int kMaxJobs = 480;   // tensors of one launch (31 KB of kernel parameters)
+static_assert(kRun == kThreads * 8 && kBlock == 256, "a warp takes one block of 256, 8 elements per lane");
+
+// 1 / 127^2 and 1 / 255^2: the units of the two square laws.
+constexpr float kUnitM = 1.0f / 16129.0f, kUnitV = 1.0f / 65025.0f;
+constexpr float kTinyM = 7.888609052210118e-31f;  // 2^-100: below it 16129 / max|m| could overflow
+
+struct AdamwParams {
+    float step_sz, bc2_sqrt, decay, beta1, beta2, eps, max_norm, clip_eps;
+};
+
+struct StepJob {
+    float*       p;
+    const float* g;
+    void*        m;
+    void*        v;
+    float*       m_scale;
+    float*       v_scale;
+    int64_t      n;
+    int32_t      run_begin;  // first run of this tensor
+    int32_t      aligned;    // its vectors may be loaded whole
+};
+
+struct StepBatch {
+    StepJob      job[kMaxJobs];
+    const float* norm;
+    AdamwParams  a;
+    int32_t      n_jobs;
+};
+static_assert(sizeof(StepBatch) <= 32764, "kernel parameter limit");
+
+// The tensor that run `run` belongs to (run_begin ascends).
+template <class JOB>
+__device__ __forceinline__ int job_of(const JOB* job, int n_jobs, int run) {
+    int lo = 0, hi = n_jobs - 1;
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (job[mid].run_begin <= run) lo = mid;
+        else hi = mid - 1;
+    }
+    return lo;
+}
+
+// Four consecutive floats at i, those beyond n as zero.
+__device__ __forceinline__ void load4(const float* q, int64_t i, int64_t n, bool whole, float (&x)[4]) {
+    if (whole && i + 4 <= n) {
+        const float4 t = *reinterpret_cast<const float4*>(q + i);
+        x[0] = t.x; x[1] = t.y; x[2] = t.z; x[3] = t.w;
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[e] = i + e < n ? q[i + e] : 0.0f;
+    }
+}
+
+__device__ __forceinline__ void store4(float* q, int64_t i, int64_t n, bool whole, const float (&x)[4]) {
+    if (whole && i + 4 <= n) {
+        *reinterpret_cast<float4*>(q + i) = make_float4(x[0], x[1], x[2], x[3]);
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (i + e < n) q[i + e] = x[e];
+    }
+}
+
+// The same for one-byte codes (four in a word, byte e = element e).
+__device__ __forceinline__ uint32_t load4c(const uint8_t* q, int64_t i, int64_t n, bool whole) {
+    if (whole && i + 4 <= n) return *reinterpret_cast<const uint32_t*>(q + i);
+    uint32_t w = 0;
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+        if (i + e < n) w |= static_cast<uint32_t>(q[i + e]) << (8 * e);
+    return w;
+}
+
+__device__ __forceinline__ void store4c(uint8_t* q, int64_t i, int64_t n, bool whole, uint32_t w) {
+    if (whole && i + 4 <= n) {
+        *reinterpret_cast<uint32_t*>(q + i) = w;
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (i + e < n) q[i + e] = static_cast<uint8_t>(w >> (8 * e));
+    }
+}
+
+__device__ __forceinline__ float decode_m(uint32_t w, int e, float scale) {
+    const int c = static_cast<int8_t>(w >> (8 * e));
+    return __fmul_rn(static_cast<float>(c * abs(c)), scale);
+}
+
+__device__ __forceinline__ float decode_v(uint32_t w, int e, float scale) {
+    const int c = static_cast<int>((w >> (8 * e)) & 0xFFu);
+    const float u = __fmul_rn(static_cast<float>(c * c), scale);
+    return __fmul_rn(u, u);
+}
+
+// The largest of the warp's values, NaN if one of them is infinite or NaN (values are not negative).
+__device__ __forceinline__ float block_max(const float (&x)[8]) {
+    float top = 0.0f;
+    bool  fine = true;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        top  = fmaxf(top, x[e]);
+        fine = fine && x[e] <= 3.402823466e+38f;
+    }
+    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
+    return __all_sync(0xFFFFFFFFu, fine) ? top : __int_as_float(0x7FC00000);
+}
+
+// One block's new codes from the warp's 8 values per lane (a lane's values 0-3 in w[0], 4-7 in
+// w[1]); returns the scale.
+__device__ __forceinline__ float encode_m(const float (&m)[8], uint32_t (&w)[2]) {
+    float x[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = fabsf(m[e]);
+    float top = block_max(x);
+    if (top < kTinyM) top = 0.0f;
+    const float per = top > 0.0f ? __fdiv_rn(16129.0f, top) : 0.0f;  // 0 for NaN too
+    w[0] = w[1] = 0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        const int c = per > 0.0f ? __float2int_rn(__fsqrt_rn(__fmul_rn(x[e], per))) : 0;
+        w[e >> 2] |= static_cast<uint32_t>((m[e] < 0.0f ? -c : c) & 0xFF) << (8 * (e & 3));
+    }
+    return __fmul_rn(top, kUnitM);
+}
+
+__device__ __forceinline__ float encode_v(const float (&v)[8], uint32_t (&w)[2]) {
+    float u[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) u[e] = __fsqrt_rn(v[e]);  // NaN for a negative v
+    const float top = block_max(u);
+    const float per = top > 0.0f ? __fdiv_rn(65025.0f, top) : 0.0f;
+    w[0] = w[1] = 0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        int c = per > 0.0f ? __float2int_rn(__fsqrt_rn(__fmul_rn(u[e], per))) : 0;
+        if (per > 0.0f && u[e] > 0.0f) c = max(c, 1);
+        w[e >> 2] |= static_cast<uint32_t>(c) << (8 * (e & 3));
+    }
+    return __fmul_rn(top, kUnitV);
+}
+
+// One element's step: train_ops.cu's adamw_kernel.
+__device__ __forceinline__ void adamw_one(float& p, float g, float& m, float& v, const AdamwParams& a, float one_b1,
+                                          float one_b2) {
+    m = __fadd_rn(m, __fmul_rn(__fsub_rn(g, m), one_b1));
+    v = __fadd_rn(__fmul_rn(v, a.beta2), __fmul_rn(__fmul_rn(g, g), one_b2));
+    const float denom = __fadd_rn(__fdiv_rn(__fsqrt_rn(v), a.bc2_sqrt), a.eps);
+    p = __fsub_rn(__fmul_rn(p, a.decay), __fmul_rn(a.step_sz, __fdiv_rn(m, denom)));
+}
+
+template <int BITS>
+__global__ void __launch_bounds__(kThreads) adamw_many_kernel(const __grid_constant__ StepBatch batch) {
+    // From the last run to the first: the norm's pass read the gradients from the first to the last, so
+    // those that are still in L2 come first.
+    const int      run = static_cast<int>(gridDim.x - 1 - blockIdx.x);
+    const StepJob& J   = batch.job[job_of(batch.job, batch.n_jobs, run)];
+    const AdamwParams& a = batch.a;
+    const int     warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int64_t b0 = static_cast<int64_t>(run - J.run_begin) * (kRun / kBlock) + warp;  // this warp's block
+    const int64_t i0 = b0 * kBlock + lane * 4, n = J.n;
+    if (b0 * kBlock >= n) return;
+    const bool  whole = J.aligned != 0;
+    const float one_b1 = __fsub_rn(1.0f, a.beta1), one_b2 = __fsub_rn(1.0f, a.beta2);
+    float clip = 1.0f;
+    if (batch.norm != nullptr) {  // clip_scale_kernel's factor
+        clip = __fdiv_rn(a.max_norm, __fadd_rn(__fsqrt_rn(batch.norm[0]), a.clip_eps));
+        if (clip > 1.0f) clip = 1.0f;
+    }
+    float p[2][4], g[2][4], m[8], v[8];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        load4(J.p, i0 + 128 * h, n, whole, p[h]);
+        load4(J.g, i0 + 128 * h, n, whole, g[h]);
+    }
+    if constexpr (BITS == 32) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            load4(static_cast<const float*>(J.m), i0 + 128 * h, n, whole, reinterpret_cast<float (&)[4]>(m[4 * h]));
+            load4(static_cast<const float*>(J.v), i0 + 128 * h, n, whole, reinterpret_cast<float (&)[4]>(v[4 * h]));
+        }
+    } else {
+        const float sm = J.m_scale[b0], sv = J.v_scale[b0];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const uint32_t wm = load4c(static_cast<const uint8_t*>(J.m), i0 + 128 * h, n, whole);
+            const uint32_t wv = load4c(static_cast<const uint8_t*>(J.v), i0 + 128 * h, n, whole);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                m[4 * h + e] = decode_m(wm, e, sm);
+                v[4 * h + e] = decode_v(wv, e, sv);
+            }
+        }
+    }
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const float ge = batch.norm != nullptr ? __fmul_rn(g[h][e], clip) : g[h][e];
+            adamw_one(p[h][e], ge, m[4 * h + e], v[4 * h + e], a, one_b1, one_b2);
+        }
+#pragma unroll
+    for (int h = 0; h < 2; ++h) store4(J.p, i0 + 128 * h, n, whole, p[h]);
+    if constexpr (BITS == 32) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            store4(static_cast<float*>(J.m), i0 + 128 * h, n, whole, reinterpret_cast<float (&)[4]>(m[4 * h]));
+            store4(static_cast<float*>(J.v), i0 + 128 * h, n, whole, reinterpret_cast<float (&)[4]>(v[4 * h]));
+        }
+    } else {
+        // what lies behind the tensor's end is not part of its last block
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+            if (i0 + 128 * (e >> 2) + (e & 3) >= n) m[e] = v[e] = 0.0f;
+        uint32_t wm[2], wv[2];
+        const float sm = encode_m(m, wm), sv = encode_v(v, wv);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            store4c(static_cast<uint8_t*>(J.m), i0 + 128 * h, n, whole, wm[h]);
+            store4c(static_cast<uint8_t*>(J.v), i0 + 128 * h, n, whole, wv[h]);
+        }
+        if (lane == 0) {
+            J.m_scale[b0] = sm;
+            J.v_scale[b0] = sv;
+        }
+    }
+}
+
+// ------------------------------------------------------------------ 8-bit states <-> values
+// One warp per block of 256.
+template <int WHICH>
+__global__ void __launch_bounds__(kThreads) state8_to_f32_kernel(const uint8_t* codes, const float* scales, float* values,
+                                                                 int64_t n, bool whole) {
+    const int64_t b = static_cast<int64_t>(blockIdx.x) * (kThreads / 32) + (threadIdx.x >> 5);
+    const int64_t i0 = b * kBlock + (threadIdx.x & 31) * 4;
+    if (b * kBlock >= n) return;
+    const float s = scales[b];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const uint32_t w = load4c(codes, i0 + 128 * h, n, whole);
+        float x[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[e] = WHICH == 0 ? decode_m(w, e, s) : decode_v(w, e, s);
+        store4(values, i0 + 128 * h, n, whole, x);
+    }
+}
+
+template <int WHICH>
+__global__ void __launch_bounds__(kThreads) state8_from_f32_kernel(const float* values, uint8_t* codes, float* scales,
+                                                                   int64_t n, bool whole) {
+    const int64_t b = static_cast<int64_t>(blockIdx.x) * (kThreads / 32) + (threadIdx.x >> 5);
+    const int64_t i0 = b * kBlock + (threadIdx.x & 31) * 4;
+    if (b * kBlock >= n) return;
+    float x[8];
+    load4(values, i0, n, whole, reinterpret_cast<float (&)[4]>(x[0]));
+    load4(values, i0 + 128, n, whole, reinterpret_cast<float (&)[4]>(x[4]));
+    uint32_t w[2];
+    const float s = WHICH == 0 ? encode_m(x, w) : encode_v(x, w);
+    store4c(codes, i0, n, whole, w[0]);
+    store4c(codes, i0 + 128, n, whole, w[1]);
+    if ((threadIdx.x & 31) == 0) scales[b] = s;
+}
+
+// ------------------------------------------------------------------ squared norm of many tensors
+// Pass 1: one double for each chunk of a span (each square is exact in double). Pass 2 adds them in a
+// fixed order.
+constexpr int64_t kChunk    = 16384;
+constexpr int     kMaxSpans = 1000;
+
+struct Span {
+    const float* a;
+    int64_t      n;
+    int32_t      run_begin;
+    int32_t      aligned;
+};
+
+struct SpanBatch {
+    Span    job[kMaxSpans];
+    double* partials;
+    int32_t n_jobs;
+};
+static_assert(sizeof(SpanBatch) <= 32764, "kernel parameter limit");
+
+__device__ __forceinline__ double block_sum(double s) {
+    __shared__ double sh[kThreads / 32];
+    for (int o = 16; o > 0; o >>= 1) s += __shfl_down_sync(0xFFFFFFFFu, s, o);
+    if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = s;
+    __syncthreads();
+    s = 0.0;
+    if (threadIdx.x == 0)
+        for (int w = 0; w < kThreads / 32; ++w) s = __dadd_rn(s, sh[w]);
+    return s;
+}
+
+__global__ void __launch_bounds__(kThreads) sum_sqr_many_kernel(const __grid_constant__ SpanBatch batch) {
+    const int     run = static_cast<int>(blockIdx.x);
+    const Span&   J   = batch.job[job_of(batch.job, batch.n_jobs, run)];
+    const int64_t lo = static_cast<int64_t>(run - J.run_begin) * kChunk, hi = min(J.n, lo + kChunk);
+    double s = 0.0;
+#pragma unroll 4
+    for (int64_t i = lo + threadIdx.x * 4; i < hi; i += kThreads * 4) {
+        float x[4];
+        load4(J.a, i, hi, J.aligned != 0, x);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const double d = static_cast<double>(x[e]);
+            s = fma(d, d, s);
+        }
+    }
+    s = block_sum(s);
+    if (threadIdx.x == 0) batch.partials[run] = s;
+}
+
+__global__ void __launch_bounds__(kThreads) sum_sqr_many_final_kernel(const double* partials, int64_t n, float* out) {
+    double s = 0.0;
+    for (int64_t i = threadIdx.x; i < n; i += kThreads) s = __dadd_rn(s, partials[i]);
+    s = block_sum(s);
+    if (threadIdx.x == 0) out[0] = __double2float_rn(s);
+}
+
+bool aligned_to(const void* p, uint64_t bytes) { return (reinterpret_cast<uint64_t>(p) & (bytes - 1)) == 0; }
+
+int64_t chunks_of(const trc_cuda_span* spans, int n_spans) {
+    int64_t c = 0;
+    for (int i = 0; i < n_spans; ++i) c += spans[i].n > 0 ? (spans[i].n + kChunk - 1) / kChunk : 0;
+    return c;
+}
+
+constexpr int64_t kMaxElems = int64_t(1) << 40;  // of one tensor: its runs and chunks fit a grid
+
+}  // namespace
+
+}  // namespace trc
+
+using namespace trc;
+
+extern "C" {
+
+int trc_cuda_opt_step_adamw_many(const trc_cuda_adamw_job* jobs, int n_jobs, int state_bits, const float* params6,
+                                 const float* norm, float max_norm, float clip_eps, void* stream) {
+    if (n_jobs < 0 || (n_jobs > 0 && jobs == nullptr) || params6 == nullptr) return TRC_CUDA_EINVAL;
+    if (state_bits != 32 && state_bits != 8) return TRC_CUDA_EUNSUPPORTED;
+    if (!aligned_to(norm, 4)) return TRC_CUDA_EINVAL;
+    const uint64_t state_bytes = state_bits == 32 ? 4 : 1;
+    for (int i = 0; i < n_jobs; ++i) {  // every tensor before the first launch
+        const trc_cuda_adamw_job& in = jobs[i];
+        if (in.n < 0 || in.n > kMaxElems) return TRC_CUDA_EINVAL;
+        if (in.n == 0) continue;
+        if (in.param == nullptr || in.grad == nullptr || in.m == nullptr || in.v == nullptr) return TRC_CUDA_EINVAL;
+        if (!aligned_to(in.param, 4) || !aligned_to(in.grad, 4) || !aligned_to(in.m, state_bytes) ||
+            !aligned_to(in.v, state_bytes))
+            return TRC_CUDA_EINVAL;
+        if (state_bits == 8 && (in.m_scale == nullptr || in.v_scale == nullptr || !aligned_to(in.m_scale, 4) ||
+                                !aligned_to(in.v_scale, 4)))
+            return TRC_CUDA_EINVAL;
+    }
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    StepBatch batch;
+    batch.norm = norm;
+    batch.a = AdamwParams{params6[0], params6[1], params6[2], params6[3], params6[4], params6[5], max_norm, clip_eps};
+    // Batches from the last tensor to the first, as the runs inside a launch.
+    for (int last = n_jobs; last > 0;) {
+        int64_t runs = 0;
+        int first = last;
+        batch.n_jobs = 0;
+        while (first > 0 && last - first < kMaxJobs) {
+            const int64_t r = (jobs[first - 1].n + kRun - 1) / kRun;
+            if (runs + r > INT32_MAX) break;
+            runs += r;
+            --first;
+        }
+        runs = 0;
+        for (int i = first; i < last; ++i) {
+            const trc_cuda_adamw_job& in = jobs[i];
+            if (in.n == 0) continue;
+            StepJob& J  = batch.job[batch.n_jobs++];
+            J.p         = in.param;
+            J.g         = in.grad;
+            J.m         = in.m;
+            J.v         = in.v;
+            J.m_scale   = in.m_scale;
+            J.v_scale   = in.v_scale;
+            J.n         = in.n;
+            J.run_begin = static_cast<int32_t>(runs);
+            J.aligned   = aligned_to(in.param, 16) && aligned_to(in.grad, 16) && aligned_to(in.m, 4 * state_bytes) &&
+                        aligned_to(in.v, 4 * state_bytes);
+            runs += (in.n + kRun - 1) / kRun;
+        }
+        last = first;
+        if (runs == 0) continue;
+        if (state_bits == 32) adamw_many_kernel<32><<<static_cast<unsigned>(runs), kThreads, 0, s>>>(batch);
+        else adamw_many_kernel<8><<<static_cast<unsigned>(runs), kThreads, 0, s>>>(batch);
+        note_launch();
+        const int st = check_launch();
+        if (st != TRC_CUDA_OK) return st;
+    }
+    return TRC_CUDA_OK;
+}
+
+int trc_cuda_state8_to_f32(int which, const void* codes, const float* scales, float* values, int64_t n, void* stream) {
+    if (which != 0 && which != 1) return TRC_CUDA_EUNSUPPORTED;
+    if (n < 0 || n > kMaxElems) return TRC_CUDA_EINVAL;
+    if (n == 0) return TRC_CUDA_OK;
+    if (codes == nullptr || scales == nullptr || values == nullptr || !aligned_to(scales, 4) || !aligned_to(values, 4))
+        return TRC_CUDA_EINVAL;
+    const unsigned grid = static_cast<unsigned>((n + kRun - 1) / kRun);
+    const bool whole = aligned_to(codes, 4) && aligned_to(values, 16);
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    const uint8_t* c = static_cast<const uint8_t*>(codes);
+    if (which == 0) state8_to_f32_kernel<0><<<grid, kThreads, 0, s>>>(c, scales, values, n, whole);
+    else state8_to_f32_kernel<1><<<grid, kThreads, 0, s>>>(c, scales, values, n, whole);
+    note_launch();
+    return check_launch();
+}
+
+int trc_cuda_state8_from_f32(int which, const float* values, void* codes, float* scales, int64_t n, void* stream) {
+    if (which != 0 && which != 1) return TRC_CUDA_EUNSUPPORTED;
+    if (n < 0 || n > kMaxElems) return TRC_CUDA_EINVAL;
+    if (n == 0) return TRC_CUDA_OK;
+    if (codes == nullptr || scales == nullptr || values == nullptr || !aligned_to(scales, 4) || !aligned_to(values, 4))
+        return TRC_CUDA_EINVAL;
+    const unsigned grid = static_cast<unsigned>((n + kRun - 1) / kRun);
+    const bool whole = aligned_to(codes, 4) && aligned_to(values, 16);
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    uint8_t* c = static_cast<uint8_t*>(codes);
+    if (which == 0) state8_from_f32_kernel<0><<<grid, kThreads, 0, s>>>(values, c, scales, n, whole);
+    else state8_from_f32_kernel<1><<<grid, kThreads, 0, s>>>(values, c, scales, n, whole);
+    note_launch();
+    return check_launch();
+}
+
+size_t trc_cuda_sum_sqr_many_workspace_bytes(const trc_cuda_span* spans, int n_spans) {
+    if (n_spans < 0 || (n_spans > 0 && spans == nullptr)) return 0;
+    return static_cast<size_t>(std::max<int64_t>(1, chunks_of(spans, n_spans))) * sizeof(double);
+}
+
+int trc_cuda_sum_sqr_many(const trc_cuda_span* spans, int n_spans, float* out, void* workspace,
+                          size_t workspace_bytes, void* stream) {
+    if (n_spans < 0 || (n_spans > 0 && spans == nullptr) || out == nullptr || !aligned_to(out, 4)) return TRC_CUDA_EINVAL;
+    for (int i = 0; i < n_spans; ++i) {
+        if (spans[i].n < 0 || spans[i].n > kMaxElems) return TRC_CUDA_EINVAL;
+        if (spans[i].n > 0 && (spans[i].data == nullptr || !aligned_to(spans[i].data, 4))) return TRC_CUDA_EINVAL;
+    }
+    if (workspace == nullptr || !aligned_to(workspace, 8) ||
+        workspace_bytes < trc_cuda_sum_sqr_many_workspace_bytes(spans, n_spans))
+        return TRC_CUDA_EINVAL;
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    double* partials = static_cast<double*>(workspace);
+    int64_t done = 0;
+    SpanBatch batch;
+    for (int i = 0; i < n_spans;) {
+        int64_t runs = 0;
+        batch.n_jobs = 0;
+        batch.partials = partials + done;
+        for (; i < n_spans && batch.n_jobs < kMaxSpans; ++i) {
+            const int64_t r = (spans[i].n + kChunk - 1) / kChunk;
+            if (r == 0) continue;
+            if (runs + r > INT32_MAX) break;
+            batch.job[batch.n_jobs++] = Span{spans[i].data, spans[i].n, static_cast<int32_t>(runs),
+                                             aligned_to(spans[i].data, 16) ? 1 : 0};
+            runs += r;
+        }
+        if (runs == 0) continue;
+        sum_sqr_many_kernel<<<static_cast<unsigned>(runs), kThreads, 0, s>>>(batch);
+        note_launch();
+        const int st = check_launch();
+        if (st != TRC_CUDA_OK) return st;
+        done += runs;
+    }
+    sum_sqr_many_final_kernel<<<1, kThreads, 0, s>>>(partials, done, out);
+    note_launch();
+    return check_launch();
+}
+
+}  // extern "C"

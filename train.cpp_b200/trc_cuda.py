@@ -11,6 +11,10 @@ source tree):
   cont / acc / repeat_back / repeat / add / sub / mul / div / sum
                                            src/backends/cpu/trc_cpu_ops.cpp (compute_dup :219,
                                            compute_acc :954, compute_repeat_back :932, ...)
+  lora / lora_back                         low-rank adapters of many requests beside a shared projection
+                                           (no reference counterpart)
+  AdamwMany / SumSqrMany                   opt_step_adamw and sum_sqr_acc over many tensors at once, with
+                                           states in 32 or 8 bits (no reference counterpart)
 
 Tensors are torch CUDA tensors used purely as device memory. A ggml tensor with
 ne = [ne0, ne1, ne2, ne3] is a torch tensor of shape (ne3, ne2, ne1, ne0); any torch stride
@@ -42,6 +46,20 @@ BIN_ADD, BIN_SUB, BIN_MUL, BIN_DIV = 0, 1, 2, 3
 
 class TrcCudaError(RuntimeError):
     pass
+
+
+class LoraAdapter(ctypes.Structure):
+    _fields_ = [("a", ctypes.c_void_p), ("b", ctypes.c_void_p), ("da", ctypes.c_void_p), ("db", ctypes.c_void_p),
+                ("scale", ctypes.c_float), ("rank", ctypes.c_int32)]
+
+
+class AdamwJob(ctypes.Structure):
+    _fields_ = [("param", ctypes.c_void_p), ("grad", ctypes.c_void_p), ("m", ctypes.c_void_p), ("v", ctypes.c_void_p),
+                ("m_scale", ctypes.c_void_p), ("v_scale", ctypes.c_void_p), ("n", ctypes.c_int64)]
+
+
+class Span(ctypes.Structure):
+    _fields_ = [("data", ctypes.c_void_p), ("n", ctypes.c_int64)]
 
 
 class View(ctypes.Structure):
@@ -108,6 +126,15 @@ def lib() -> ctypes.CDLL:
         "trc_cuda_sum_sqr_workspace_bytes": (SZ, [I64]),
         "trc_cuda_sum_sqr_acc": (I, [P, P, I64, P, SZ, P]),
         "trc_cuda_clip_scale_inplace": (I, [P, I64, P, ctypes.c_float, ctypes.c_float, P]),
+        "trc_cuda_lora_h_ld": (I64, [ctypes.POINTER(LoraAdapter), I]),
+        "trc_cuda_lora": (I, [I, ctypes.POINTER(LoraAdapter), I, P, VP, VP, VP, P, P]),
+        "trc_cuda_lora_back_workspace_bytes": (SZ, [ctypes.POINTER(LoraAdapter), I, I64]),
+        "trc_cuda_lora_back": (I, [I, ctypes.POINTER(LoraAdapter), I, P, VP, VP, P, VP, VP, P, SZ, U32, P]),
+        "trc_cuda_opt_step_adamw_many": (I, [ctypes.POINTER(AdamwJob), I, I, P, P, ctypes.c_float, ctypes.c_float, P]),
+        "trc_cuda_state8_to_f32": (I, [I, P, P, P, I64, P]),
+        "trc_cuda_state8_from_f32": (I, [I, P, P, P, I64, P]),
+        "trc_cuda_sum_sqr_many_workspace_bytes": (SZ, [ctypes.POINTER(Span), I]),
+        "trc_cuda_sum_sqr_many": (I, [ctypes.POINTER(Span), I, P, P, SZ, P]),
     }
     for name, (res, args) in sig.items():
         fn = getattr(L, name)
@@ -682,3 +709,311 @@ def clip_scale_(a: torch.Tensor, norm: torch.Tensor, max_norm: float, eps: float
     """a *= min(1, max_norm / (sqrt(norm[0]) + eps)), the clip graph's OP_CLIP_SCALE_INPLACE."""
     _check(lib().trc_cuda_clip_scale_inplace(_flat(a, "a"), a.numel(), _flat(norm, "norm"), max_norm, eps,
                                              _stream(stream)), "trc_cuda_clip_scale_inplace")
+
+
+# ------------------------------------------------------------------ scratch and device checks
+
+def _scratch(numel: int, dtype: torch.dtype, device, stream) -> torch.Tensor:
+    """Memory for a call's own use on `stream`: it belongs to that stream, so that it is not handed out
+    again while the call's kernels still use it."""
+    if stream is None:
+        return torch.empty(numel, dtype=dtype, device=device)
+    with torch.cuda.stream(stream):
+        return torch.empty(numel, dtype=dtype, device=device)
+
+
+def _on_current_device(t: torch.Tensor, what: str) -> None:
+    if not t.is_cuda:
+        raise TrcCudaError(f"{what}: expected a CUDA tensor (device memory)")
+    if t.device.index != torch.cuda.current_device():
+        raise TrcCudaError(f"{what}: the tensor is on {t.device}, the current device is cuda:{torch.cuda.current_device()}")
+
+
+def _no_overlap(tensors: Sequence[torch.Tensor], what: str) -> None:
+    """Raises if two of these contiguous tensors, all of them written by one launch, share memory."""
+    spans = sorted((t.data_ptr(), t.data_ptr() + t.numel() * t.element_size()) for t in tensors if t.numel())
+    for (_, end), (start, _) in zip(spans, spans[1:]):
+        if start < end:
+            raise TrcCudaError(f"{what}: two of the written tensors share memory")
+
+
+# ------------------------------------------------------------------ low-rank adapters
+
+TYPE_F16, TYPE_BF16 = 1, 30
+LORA_MAX_ADAPTERS, LORA_MAX_RANK = 256, 256
+_LORA_TYPES = {torch.float32: TYPE_F32, torch.float16: TYPE_F16, torch.bfloat16: TYPE_BF16}
+
+
+class LoraAdapters:
+    """The low-rank adapters of one projection: (A, B, scale) with A of torch shape (rank, K) and B (N, rank)
+    -- ggml's lora_a, ne = [K, rank], and lora_b, ne = [rank, N] -- all float32, float16 or bfloat16.
+    Ranks may differ. grads: (dA, dB) for each adapter, float32 tensors of the factors' shapes that
+    lora_back writes; None (for an adapter or in a pair) where no gradient is wanted.
+    The table is checked and built once; the tensors are used in place, so a step of an optimizer on
+    them needs no new table."""
+
+    def __init__(self, adapters: Sequence[tuple[torch.Tensor, torch.Tensor, float]], grads=None):
+        if len(adapters) > LORA_MAX_ADAPTERS:
+            raise TrcCudaError(f"{len(adapters)} adapters: one call takes at most {LORA_MAX_ADAPTERS}")
+        if grads is not None and len(grads) != len(adapters):
+            raise TrcCudaError("grads needs one entry for each adapter")
+        self._keep, self._n, self._arr = [], len(adapters), (LoraAdapter * max(1, len(adapters)))()
+        self.k = self.n = self.type = self.device = None
+        written = []
+        for i, (a, b, scale) in enumerate(adapters):
+            if a.dim() != 2 or b.dim() != 2 or a.shape[0] != b.shape[1]:
+                raise TrcCudaError(f"adapter {i}: A is (rank, K) and B (N, rank), got {tuple(a.shape)} and {tuple(b.shape)}")
+            if not 1 <= a.shape[0] <= LORA_MAX_RANK:
+                raise TrcCudaError(f"adapter {i}: rank {a.shape[0]} is outside 1..{LORA_MAX_RANK}")
+            if a.dtype not in _LORA_TYPES or b.dtype != a.dtype:
+                raise TrcCudaError(f"adapter {i}: both factors are float32, float16 or bfloat16")
+            if not a.is_contiguous() or not b.is_contiguous():
+                raise TrcCudaError(f"adapter {i}: the factors must be contiguous")
+            _on_current_device(a, f"adapter {i}")
+            _on_current_device(b, f"adapter {i}")
+            what = (a.shape[1], b.shape[0], _LORA_TYPES[a.dtype], a.device)
+            if i == 0:
+                self.k, self.n, self.type, self.device = what
+            elif what != (self.k, self.n, self.type, self.device):
+                raise TrcCudaError(f"adapter {i}: the adapters of a projection share its sizes, type and device")
+            e = self._arr[i]
+            e.a, e.b, e.scale, e.rank = a.data_ptr(), b.data_ptr(), float(scale), a.shape[0]
+            pair = (None, None) if grads is None or grads[i] is None else grads[i]
+            for name, g, w in (("da", pair[0], a), ("db", pair[1], b)):
+                if g is None:
+                    continue
+                if g.dtype != torch.float32 or g.shape != w.shape or not g.is_contiguous() or g.device != w.device:
+                    raise TrcCudaError(f"adapter {i}: {name} must be contiguous float32 of its factor's shape and device")
+                setattr(e, name, g.data_ptr())
+                written.append(g)
+            self._keep.append((a, b, pair))
+        _no_overlap(written, "LoraAdapters: gradients")
+        self.ld = int(lib().trc_cuda_lora_h_ld(self._arr, self._n))
+        if self.ld < 0:
+            _check(self.ld, "trc_cuda_lora_h_ld")
+
+    def __len__(self) -> int:
+        return self._n
+
+
+_I4 = ctypes.c_int64 * 4
+
+
+def _rows_view(t: torch.Tensor, what: str) -> View:
+    """view_of, for a tensor whose last dimension is a row (ne0)."""
+    if t.dtype != torch.float32 or not t.is_cuda:
+        raise TrcCudaError(f"{what}: expected a float32 CUDA tensor")
+    if t.dim() == 2:  # the usual case, without the general form's work
+        (n1, n0), (s1, s0) = t.shape, t.stride()
+        return View(t.data_ptr(), _I4(n0, n1, 1, 1), _I4(4 * s0, 4 * s1, 4 * s1 * n1, 4 * s1 * n1))
+    return view_of(t)
+
+
+def _lora_args(ad: LoraAdapters, x: torch.Tensor, ids: torch.Tensor | None, out_len: int | None, what: str) -> int:
+    """Checks what lora and lora_back share; returns the number of rows."""
+    _on_current_device(x, what)
+    if not 1 <= x.dim() <= 4:
+        raise TrcCudaError(f"{what}: x has one to four dimensions")
+    rows = x.numel() // x.shape[-1] if x.shape[-1] else 0
+    if ad.k is not None and (x.shape[-1] != ad.k or x.device != ad.device):
+        raise TrcCudaError(f"{what}: x has rows of {x.shape[-1]} on {x.device}, the adapters take {ad.k} on {ad.device}")
+    if out_len is not None and ad.n is not None and out_len != ad.n:
+        raise TrcCudaError(f"{what}: base, out or dy has rows of {out_len}, the adapters give {ad.n}")
+    if ids is None:
+        if len(ad) != 1:
+            raise TrcCudaError(f"{what}: ids may be left out for a single adapter only")
+    elif ids.dtype != torch.int32 or not ids.is_contiguous() or ids.numel() != rows or ids.device != x.device:
+        raise TrcCudaError(f"{what}: ids must be a contiguous int32 tensor with one entry for each of the {rows} rows")
+    return rows
+
+
+def _same_rows(t: torch.Tensor, x: torch.Tensor, length: int, what: str) -> None:
+    same = t.shape[:-1] == x.shape[:-1] or ggml_ne(t)[1:] == ggml_ne(x)[1:]  # leading dimensions of 1 may differ
+    if not same or t.shape[-1] != length or t.device != x.device:
+        raise TrcCudaError(f"{what}: expected {tuple(x.shape[:-1]) + (length,)} on {x.device}, got {tuple(t.shape)} on {t.device}")
+
+
+def _check_h(h: torch.Tensor, ad: LoraAdapters, x: torch.Tensor, rows: int, what: str) -> None:
+    if h.dtype != torch.float32 or h.device != x.device or not h.is_contiguous() or h.numel() != rows * ad.ld:
+        raise TrcCudaError(f"{what}: h must be what lora_h gives for x")
+
+
+def lora_h(adapters: LoraAdapters, x: torch.Tensor) -> torch.Tensor:
+    """An empty buffer for the rows' scale * A x, which lora fills and lora_back takes."""
+    rows = x.numel() // x.shape[-1] if x.shape[-1] else 0
+    return torch.empty((rows, adapters.ld), dtype=torch.float32, device=x.device)
+
+
+def lora(adapters: LoraAdapters, x: torch.Tensor, ids: torch.Tensor | None = None, base: torch.Tensor | None = None,
+         out: torch.Tensor | None = None, h: torch.Tensor | None = None, stream=None) -> torch.Tensor:
+    """out[t] = base[t] + scale * B (A x[t]) with the adapter ids[t] of each row t of x (..., K); a row
+    whose id is no adapter's (-1) keeps its base. base (..., N) is the shared projection's output (None: 0)
+    and may be `out` itself. ids: int32, one for each row; None: the single adapter everywhere.
+    h: a buffer of lora_h to keep for lora_back."""
+    n = base.shape[-1] if base is not None else out.shape[-1] if out is not None else adapters.n
+    if n is None:
+        raise TrcCudaError("lora: without adapters, base or out has to say how long an output is")
+    rows = _lora_args(adapters, x, ids, n, "lora")
+    if out is None:
+        out = _scratch(x.shape[:-1] + (n,), torch.float32, x.device, stream)
+    _same_rows(out, x, n, "lora: out")
+    if base is not None:
+        _same_rows(base, x, n, "lora: base")
+    if h is None:
+        h = _scratch((rows, adapters.ld), torch.float32, x.device, stream)
+    _check_h(h, adapters, x, rows, "lora")
+    vx, vd = _rows_view(x, "lora: x"), _rows_view(out, "lora: out")
+    vb = ctypes.byref(_rows_view(base, "lora: base")) if base is not None else None
+    _check(lib().trc_cuda_lora(adapters.type or 0, adapters._arr, adapters._n, None if ids is None else ids.data_ptr(),
+                               ctypes.byref(vx), vb, ctypes.byref(vd), h.data_ptr(), _stream(stream)), "trc_cuda_lora")
+    return out
+
+
+def lora_back(adapters: LoraAdapters, x: torch.Tensor, ids: torch.Tensor | None, dy: torch.Tensor, h: torch.Tensor,
+              base: torch.Tensor | None = None, dx: torch.Tensor | None = None, need_dx: bool = True,
+              accumulate: bool = False, stream=None) -> torch.Tensor | None:
+    """The gradients of lora for the upstream gradient dy (..., N): writes (accumulate: adds to) the adapters'
+    dA and dB and returns dx = base + A^T (scale * B^T dy), base being the gradient that the shared
+    projection's backward gives (None: 0; it may be `dx` itself). need_dx=False: no dx, returns None.
+    x, ids and h are those of the forward call."""
+    rows = _lora_args(adapters, x, ids, dy.shape[-1], "lora_back")
+    _same_rows(dy, x, dy.shape[-1], "lora_back: dy")
+    _check_h(h, adapters, x, rows, "lora_back")
+    if not need_dx and (dx is not None or base is not None):
+        raise TrcCudaError("lora_back: dx and base go with need_dx")
+    if need_dx and dx is None:
+        dx = _scratch(x.shape, torch.float32, x.device, stream)
+    vd = vb = None
+    if dx is not None:
+        _same_rows(dx, x, x.shape[-1], "lora_back: dx")
+        vd = ctypes.byref(_rows_view(dx, "lora_back: dx"))
+    if base is not None:
+        _same_rows(base, x, x.shape[-1], "lora_back: base")
+        vb = ctypes.byref(_rows_view(base, "lora_back: base"))
+    vx, vy = _rows_view(x, "lora_back: x"), _rows_view(dy, "lora_back: dy")
+    need = int(lib().trc_cuda_lora_back_workspace_bytes(adapters._arr, adapters._n, rows))
+    ws = _scratch(need, torch.uint8, x.device, stream)
+    _check(lib().trc_cuda_lora_back(adapters.type or 0, adapters._arr, adapters._n,
+                                    None if ids is None else ids.data_ptr(), ctypes.byref(vx), ctypes.byref(vy),
+                                    h.data_ptr(), vb, vd, ws.data_ptr(), need, MM_ACCUMULATE if accumulate else 0,
+                                    _stream(stream)), "trc_cuda_lora_back")
+    return dx
+
+
+# ------------------------------------------------------------------ the optimizer over many tensors
+
+STATE8_BLOCK = 256  # elements of a tensor that share a scale in an 8-bit state
+
+
+def _check_part(t: torch.Tensor, dtype: torch.dtype, numel: int, what: str) -> int:
+    if t.dtype != dtype or not t.is_contiguous() or t.numel() != numel:
+        raise TrcCudaError(f"{what}: expected a contiguous {dtype} tensor of {numel} elements")
+    _on_current_device(t, what)
+    return t.data_ptr()
+
+
+class AdamwMany:
+    """AdamW over many tensors at once: params and grads are lists of float32 tensors; m and v their states,
+    either float32, or int8 (m) and uint8 (v) codes with m_scale and v_scale, float32 tensors of one scale
+    for each STATE8_BLOCK elements (state8_empty gives a new tensor's). All are updated in place.
+    The table is built and checked once; a call is one step: params6 as in opt_step_adamw_; norm (a
+    float32 CUDA tensor of one element, SumSqrMany's) clips the gradients to max_norm on the way in."""
+
+    def __init__(self, params, grads, m, v, m_scale=None, v_scale=None):
+        self._n = len(params)
+        bits8 = m_scale is not None or v_scale is not None
+        lists = {"grads": grads, "m": m, "v": v, **({"m_scale": m_scale, "v_scale": v_scale} if bits8 else {})}
+        for name, part in lists.items():
+            if part is None or len(part) != self._n:
+                raise TrcCudaError(f"AdamwMany: {name} needs one tensor for each of the {self._n} parameters")
+        self._bits = 8 if bits8 else 32
+        self._arr = (AdamwJob * max(1, self._n))()
+        self._keep = (list(params), *(list(part) for part in lists.values()))
+        for i, p in enumerate(params):
+            e, n = self._arr[i], p.numel()
+            e.n = n
+            e.param = _check_part(p, torch.float32, n, f"AdamwMany: params[{i}]")
+            e.grad = _check_part(grads[i], torch.float32, n, f"AdamwMany: grads[{i}]")
+            e.m = _check_part(m[i], torch.int8 if bits8 else torch.float32, n, f"AdamwMany: m[{i}]")
+            e.v = _check_part(v[i], torch.uint8 if bits8 else torch.float32, n, f"AdamwMany: v[{i}]")
+            if bits8:
+                blocks = -(-n // STATE8_BLOCK)
+                e.m_scale = _check_part(m_scale[i], torch.float32, blocks, f"AdamwMany: m_scale[{i}]")
+                e.v_scale = _check_part(v_scale[i], torch.float32, blocks, f"AdamwMany: v_scale[{i}]")
+        written = [*params, *m, *v, *(m_scale or ()), *(v_scale or ())]
+        _no_overlap(written, "AdamwMany")
+        self._device = params[0].device if self._n else None
+
+    def __len__(self) -> int:
+        return self._n
+
+    def __call__(self, params6, norm: torch.Tensor | None = None, max_norm: float = 1.0, clip_eps: float = 1e-6,
+                 stream=None) -> None:
+        if self._device is not None and self._device.index != torch.cuda.current_device():
+            raise TrcCudaError(f"AdamwMany: the tensors are on {self._device}, which is not the current device")
+        ptr = None
+        if norm is not None:
+            ptr = _check_part(norm, torch.float32, 1, "AdamwMany: norm")
+        _check(lib().trc_cuda_opt_step_adamw_many(self._arr, self._n, self._bits, _params6(params6), ptr, max_norm,
+                                                  clip_eps, _stream(stream)), "trc_cuda_opt_step_adamw_many")
+
+
+class SumSqrMany:
+    """The squared norm of many float32 tensors together; a call returns it as a tensor of one element."""
+
+    def __init__(self, tensors: Sequence[torch.Tensor]):
+        self._n, self._keep = len(tensors), list(tensors)
+        self._arr = (Span * max(1, self._n))()
+        for i, t in enumerate(tensors):
+            self._arr[i].data = _check_part(t, torch.float32, t.numel(), f"SumSqrMany: tensor {i}")
+            self._arr[i].n = t.numel()
+        self._bytes = int(lib().trc_cuda_sum_sqr_many_workspace_bytes(self._arr, self._n))
+
+    def __len__(self) -> int:
+        return self._n
+
+    def __call__(self, out: torch.Tensor | None = None, stream=None) -> torch.Tensor:
+        device = self._keep[0].device if self._n else torch.device("cuda", torch.cuda.current_device())
+        if device.index != torch.cuda.current_device():
+            raise TrcCudaError(f"SumSqrMany: the tensors are on {device}, which is not the current device")
+        if out is None:
+            out = _scratch(1, torch.float32, device, stream)
+        ws = _scratch(self._bytes, torch.uint8, device, stream)
+        _check(lib().trc_cuda_sum_sqr_many(self._arr, self._n, _check_part(out, torch.float32, 1, "SumSqrMany: out"),
+                                           ws.data_ptr(), self._bytes, _stream(stream)), "trc_cuda_sum_sqr_many")
+        return out
+
+
+def state8_empty(n: int, which: str, device="cuda") -> tuple[torch.Tensor, torch.Tensor]:
+    """Codes and scales of a zero state for n elements; which: "m" (int8 codes) or "v" (uint8)."""
+    if which not in ("m", "v"):
+        raise TrcCudaError('state8: which is "m" or "v"')
+    return (torch.zeros(n, dtype=torch.int8 if which == "m" else torch.uint8, device=device),
+            torch.zeros(-(-n // STATE8_BLOCK), dtype=torch.float32, device=device))
+
+
+def _state8_which(codes: torch.Tensor, what: str) -> int:
+    if codes.dtype not in (torch.int8, torch.uint8):
+        raise TrcCudaError(f"{what}: codes are int8 (first moment) or uint8 (second moment)")
+    return 0 if codes.dtype == torch.int8 else 1
+
+
+def state8_to_f32(codes: torch.Tensor, scales: torch.Tensor, out: torch.Tensor | None = None, stream=None) -> torch.Tensor:
+    """The values of an 8-bit state, as a checkpoint holds them."""
+    which, n = _state8_which(codes, "state8_to_f32"), codes.numel()
+    if out is None:
+        out = _scratch(n, torch.float32, codes.device, stream)
+    _check(lib().trc_cuda_state8_to_f32(which, _check_part(codes, codes.dtype, n, "state8_to_f32: codes"),
+                                        _check_part(scales, torch.float32, -(-n // STATE8_BLOCK), "state8_to_f32: scales"),
+                                        _check_part(out, torch.float32, n, "state8_to_f32: out"), n, _stream(stream)),
+           "trc_cuda_state8_to_f32")
+    return out
+
+
+def state8_from_f32(values: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, stream=None) -> None:
+    """Writes a state's values (a loaded checkpoint's) into its codes and scales."""
+    which, n = _state8_which(codes, "state8_from_f32"), codes.numel()
+    _check(lib().trc_cuda_state8_from_f32(which, _check_part(values, torch.float32, n, "state8_from_f32: values"),
+                                          _check_part(codes, codes.dtype, n, "state8_from_f32: codes"),
+                                          _check_part(scales, torch.float32, -(-n // STATE8_BLOCK), "state8_from_f32: scales"),
+                                          n, _stream(stream)), "trc_cuda_state8_from_f32")
