@@ -49,7 +49,7 @@ def build_cuda(force: bool = False) -> Path:
     deps += [ROOT / "include" / "trc_cuda.h", ROOT / "include" / "trc_cuda_runtime.h"]
     if not force and not _stale(out, deps):
         return out
-    cmd = [NVCC, *ARCH, "-lineinfo", "-O3", "-std=c++17", "-rdc=true", "-shared",
+    cmd = [NVCC, *ARCH, "-lineinfo", "-O3", "-std=c++17", "-rdc=true", "-shared", "-t", "0",
            "-Xcompiler", "-fPIC", "-Xptxas", "-v", f"-I{ROOT / 'include'}",
            "-o", str(out), *[str(CSRC / s) for s in CU_SOURCES]]
     _run(cmd, LIB / "libtrc_cuda.build.log")
