@@ -11,6 +11,7 @@
 
 #include <algorithm>
 #include <cstdint>
+#include <type_traits>
 
 #include "trc_internal.h"
 #include "trc_ptx.cuh"
@@ -39,9 +40,10 @@ struct Rows {
     char*   data;
     int64_t nb0, nb1, nb2, nb3;
     int32_t n1, n2;
-    int32_t flat;  // rows are nb1 apart throughout
+    int32_t step;  // rows are this many floats apart throughout; -1: they are not
+    template <bool EVEN>
     __device__ __forceinline__ char* row(int64_t t) const {
-        if (flat) return data + t * nb1;
+        if (EVEN || step >= 0) return data + 4 * (t * step);
         const int64_t i1 = t % n1, r = t / n1;
         return data + i1 * nb1 + (r % n2) * nb2 + (r / n2) * nb3;
     }
@@ -93,56 +95,113 @@ __device__ __forceinline__ void split_b(float x, uint32_t& head, uint32_t& tail)
     }
 }
 
-// Four consecutive factor values from p[i], as floats; those at lim and beyond are zero. `vec`: p and
-// every i are multiples of four values.
-template <typename W>
-__device__ __forceinline__ void load_w4(const W* p, int64_t i, int have, bool vec, float (&w)[4]) {
-    if (vec && have >= 4) {
-        if constexpr (sizeof(W) == 4) {
-            const float4 t = __ldg(reinterpret_cast<const float4*>(p + i));
-            w[0] = t.x; w[1] = t.y; w[2] = t.z; w[3] = t.w;
-        } else {
-            const uint2 t = __ldg(reinterpret_cast<const uint2*>(p + i));
-            const W* e = reinterpret_cast<const W*>(&t);
+// N factor values held in the words of one load, as floats.
+template <typename W, int N>
+__device__ __forceinline__ void widen(const uint32_t (&raw)[N * sizeof(W) / 4], float (&w)[N]) {
+    if constexpr (sizeof(W) == 4) {
 #pragma unroll
-            for (int j = 0; j < 4; ++j) w[j] = static_cast<float>(e[j]);
-        }
+        for (int j = 0; j < N; ++j) w[j] = __uint_as_float(raw[j]);
     } else {
+        const W* e = reinterpret_cast<const W*>(raw);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) w[j] = j < have ? static_cast<float>(p[i + j]) : 0.0f;
+        for (int j = 0; j < N; ++j) w[j] = static_cast<float>(e[j]);
     }
 }
 
-// Two consecutive factor values.
-template <typename W>
-__device__ __forceinline__ void load_w2(const W* p, int64_t i, int have, bool vec, float (&w)[2]) {
-    if (vec && have >= 2) {
-        if constexpr (sizeof(W) == 4) {
-            const float2 t = __ldg(reinterpret_cast<const float2*>(p + i));
-            w[0] = t.x; w[1] = t.y;
-        } else {
-            const uint32_t t = __ldg(reinterpret_cast<const uint32_t*>(p + i));
-            const W* e = reinterpret_cast<const W*>(&t);
-            w[0] = static_cast<float>(e[0]);
-            w[1] = static_cast<float>(e[1]);
+// N consecutive factor values as floats, in one load (WHOLE) or one by one, as far as there are any: `have`
+// counts those from p on that are inside.
+template <typename W, int N, bool WHOLE>
+__device__ __forceinline__ void load_w(const W* p, int have, float (&w)[N]) {
+    if constexpr (WHOLE) {
+        constexpr int kWords = N * static_cast<int>(sizeof(W)) / 4;
+        uint32_t raw[kWords] = {};
+        if (have > 0) {
+            if constexpr (kWords == 4) {
+                const uint4 t = __ldg(reinterpret_cast<const uint4*>(p));
+                raw[0] = t.x; raw[1] = t.y; raw[2] = t.z; raw[3] = t.w;
+            } else if constexpr (kWords == 2) {
+                const uint2 t = __ldg(reinterpret_cast<const uint2*>(p));
+                raw[0] = t.x; raw[1] = t.y;
+            } else {
+                raw[0] = __ldg(reinterpret_cast<const uint32_t*>(p));
+            }
         }
+        widen<W, N>(raw, w);
     } else {
-        w[0] = have > 0 ? static_cast<float>(p[i]) : 0.0f;
-        w[1] = have > 1 ? static_cast<float>(p[i + 1]) : 0.0f;
+#pragma unroll
+        for (int j = 0; j < N; ++j) w[j] = j < have ? static_cast<float>(p[j]) : 0.0f;
     }
 }
 
-// Four consecutive activations of a row from column k on; those at k_len and beyond, and a row that is
-// null, are zero. VEC: the view's elements are side by side and every row starts at a multiple of 16 bytes.
+// What a warp works on streams through a ring in shared memory: a lane asynchronously copies the 4 - 16 bytes
+// that it will need itself into its own place (so the ring needs no barrier, only the lane's own wait), and takes
+// them into registers some steps later. In flight are thus `stages - 1` steps of every warp, without a register.
+// Loads into registers a step ahead took 15 - 30 % more time than this: the registers for it left 8 warps on
+// an SM.
+// Copies four consecutive activations of a row from column k on; those at k_len and beyond, and a row
+// that is not `live`, become zero. VEC: the view's elements are side by side, every row starts
+// at a multiple of 16 bytes and k_len is a multiple of 4.
 template <bool VEC>
-__device__ __forceinline__ void load_x4(const char* row, int64_t nb0, int k, int k_len, float (&x)[4]) {
-    if (VEC && row != nullptr && k + 4 <= k_len) {
-        const float4 t = *reinterpret_cast<const float4*>(row + 4ll * k);
-        x[0] = t.x; x[1] = t.y; x[2] = t.z; x[3] = t.w;
+__device__ __forceinline__ void ring_x4(uint32_t place, const char* row, bool live, int64_t nb0, int k, int k_len) {
+    if constexpr (VEC) {
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(place), "l"(row + 4ll * k), "r"(live && k < k_len ? 16 : 0)
+                     : "memory");
+    } else {
+        const int have = live ? min(4, k_len - k) : 0;
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(place + 4 * j),
+                         "l"(row + (j < have ? (k + j) * nb0 : 0)), "r"(j < have ? 4 : 0)
+                         : "memory");
+    }
+}
+
+__device__ __forceinline__ void ring_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void ring_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+// BYTES of a factor or of h, or zeros.
+template <int BYTES>
+__device__ __forceinline__ void ring_w(uint32_t place, const void* p, bool live) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(place), "l"(p), "n"(BYTES), "r"(live ? BYTES : 0) : "memory");
+}
+
+template <typename W, int N>
+__device__ __forceinline__ void ring_take_w(uint32_t place, float (&w)[N]) {
+    constexpr int kWords = N * static_cast<int>(sizeof(W)) / 4;
+    uint32_t raw[kWords];
+    if constexpr (kWords == 4)
+        asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(raw[0]), "=r"(raw[1]), "=r"(raw[2]), "=r"(raw[3]) : "r"(place) : "memory");
+    else if constexpr (kWords == 2)
+        asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(raw[0]), "=r"(raw[1]) : "r"(place) : "memory");
+    else
+        asm volatile("ld.shared.u32 %0, [%1];" : "=r"(raw[0]) : "r"(place) : "memory");
+    widen<W, N>(raw, w);
+}
+
+__device__ __forceinline__ void ring_take(uint32_t place, float (&x)[4]) {
+    asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(x[0]), "=f"(x[1]), "=f"(x[2]), "=f"(x[3]) : "r"(place) : "memory");
+}
+
+template <bool VEC>
+__device__ __forceinline__ void store_x4(char* row, int64_t nb0, int k, int k_len, const float (&x)[4]) {
+    if constexpr (VEC) {
+        if (k < k_len) *reinterpret_cast<float4*>(row + 4ll * k) = make_float4(x[0], x[1], x[2], x[3]);
     } else {
 #pragma unroll
         for (int j = 0; j < 4; ++j)
-            x[j] = row != nullptr && k + j < k_len ? *reinterpret_cast<const float*>(row + (k + j) * nb0) : 0.0f;
+            if (k + j < k_len) *reinterpret_cast<float*>(row + (k + j) * nb0) = x[j];
+    }
+}
+
+template <bool VEC>
+__device__ __forceinline__ void load_x4(const char* row, int64_t nb0, int k, int k_len, float (&x)[4]) {
+    if constexpr (VEC) {
+        const float4 t = k < k_len ? *reinterpret_cast<const float4*>(row + 4ll * k) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        x[0] = t.x; x[1] = t.y; x[2] = t.z; x[3] = t.w;
+    } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) x[j] = k + j < k_len ? *reinterpret_cast<const float*>(row + (k + j) * nb0) : 0.0f;
     }
 }
 
@@ -177,27 +236,59 @@ __device__ __forceinline__ uint32_t cluster_nctarank() {
 
 constexpr int kWarps = 8, kThreads = 256;
 
+// Bytes of one stage of a warp's ring: the rows' part and the factor's (grad: h's), and the stages that keep two
+// CTAs on an SM where the registers allow it (else one).
+template <typename W, int NT>
+struct DownRing {
+    static constexpr int kX = 8 * 512, kW = 2 * NT * 32 * 4 * static_cast<int>(sizeof(W)), kStage = kX + kW;
+    static constexpr int kCtas = NT == 2 ? 2 : 1;
+    static constexpr int kStages = NT == 2 ? 2 : kWarps * kStage * 3 <= 224 * 1024 ? 3 : 2;
+    static constexpr int kBytes = kWarps * kStages * kStage;
+};
+template <typename W, bool BACK, int JG>
+struct UpRing {
+    static constexpr int kX = 4 * 512, kW = JG * (BACK ? 4 : 2) * 32 * 4 * static_cast<int>(sizeof(W)), kStage = kX + kW;
+    static constexpr int kCtas = JG <= 2 ? 2 : 1;
+    static constexpr int kRoom = kCtas == 2 ? 112 * 1024 : 224 * 1024;
+    static constexpr int kStages = kWarps * kStage * 4 <= kRoom ? 4 : kWarps * kStage * 3 <= kRoom ? 3 : 2;
+    static constexpr int kBytes = kWarps * kStages * kStage;
+};
+template <int MT>
+struct GradRing {
+    static constexpr int kX = 8 * 512, kH = 8 * 32 * 8 * MT, kStage = kX + kH;
+    static constexpr int kCtas = MT == 1 ? 2 : 1;
+    static constexpr int kStages = MT == 2 ? 3 : 2;
+    static constexpr int kBytes = kWarps * kStages * kStage;
+};
+
+using True  = std::true_type;
+using False = std::false_type;
+
 // ------------------------------------------------------------------ down: h = scale * x W^T
-// One cluster per tile of 16 * MT rows and slice of the tile's adapters: each CTA takes its share of
-// the columns of x in steps of 32 (one line of every row), each warp every 8th of those; the partial sums
-// meet in shared memory and then across the cluster, always in the same order. BACK: x is dy and W is
-// B^T, whose values for one rank are `rank` apart: a lane loads V ranks of one column at once and tile i of a
-// group of V takes rank V * c + i.
-template <typename W, bool BACK, int NT, int MT, bool VEC>
-__global__ void __launch_bounds__(kThreads) down_kernel(const __grid_constant__ Adapters tab, const int32_t* ids, Rows x,
-                                                        int64_t rows, int k_len, float* h, int ld) {
+// One cluster per tile of 32 rows and slice of the tile's adapters: each CTA takes its share of the columns
+// of x in steps of 32 (one line of every row), each warp every 8th of those; the partial sums meet in
+// shared memory and then across the cluster, always in the same order. BACK: x is dy and W is B^T, whose
+// values for one rank are `rank` apart: a lane loads V ranks of one column at once and tile i of a group of V takes
+// rank V * c + i.
+template <typename W, bool BACK, int NT, bool VEC>
+__global__ void __launch_bounds__(kThreads, DownRing<W, NT>::kCtas) down_kernel(const __grid_constant__ Adapters tab,
+                                                                                   const int32_t* ids, Rows x, int64_t rows, int k_len, float* h, int ld) {
     constexpr bool HALF = sizeof(W) == 2;
-    constexpr int  V = NT < 4 ? NT : 4, kRows = 16 * MT, kCols = 8 * NT;
-    extern __shared__ float red[];  // [kWarps][kRows][kCols]
-    const int     warp = threadIdx.x >> 5, lane = threadIdx.x & 31, c = lane >> 2, q = lane & 3;
-    const int     ranks = static_cast<int>(cluster_nctarank()), rank = static_cast<int>(cluster_ctarank());
-    const int64_t row0 = static_cast<int64_t>(blockIdx.x / ranks) * kRows;
-    const TileIds tile(ids, row0, kRows, rows, tab.n);
+    constexpr int  V = NT < 4 ? NT : 4, kRows = 32, kCols = 8 * NT;
+    extern __shared__ __align__(16) float red[];  // the warps' rings, and [kWarps][kRows][kCols] partial sums
+    const int      warp = threadIdx.x >> 5, lane = threadIdx.x & 31, c = lane >> 2, q = lane & 3;
+    using Ring = DownRing<W, NT>;
+    constexpr int  kStages = Ring::kStages, kPiece = (BACK ? V : 4) * static_cast<int>(sizeof(W));  // of one load of W
+    const uint32_t ring = smem_u32(red) + warp * (kStages * Ring::kStage);
+    const int      ranks = static_cast<int>(cluster_nctarank()), rank = static_cast<int>(cluster_ctarank());
+    const int64_t  row0 = static_cast<int64_t>(blockIdx.x / ranks) * kRows;
+    const TileIds  tile(ids, row0, kRows, rows, tab.n);
     grid_dependents();
 
     if (blockIdx.y == 0 && rank == 0) {  // rows without an adapter
         for (int r = warp; r < kRows; r += kWarps) {
-            if (row0 + r < rows && __shfl_sync(0xFFFFFFFFu, tile.id, r) < 0)
+            const int id = __shfl_sync(0xFFFFFFFFu, tile.id, r);
+            if (row0 + r < rows && id < 0)
                 for (int j = lane; j < ld; j += 32) h[(row0 + r) * ld + j] = 0.0f;
         }
     }
@@ -210,72 +301,116 @@ __global__ void __launch_bounds__(kThreads) down_kernel(const __grid_constant__ 
         const Adapter& A = tab.ad[id];
         const int      r = A.rank;
         const W*       w = static_cast<const W*>(BACK ? A.b : A.a);
-        const bool     vec = (A.vec & (BACK ? 2 : 1)) != 0;
-        const char*    xr[2 * MT];  // rows c, c + 8, c + 16, c + 24
+        const char*    xr[4];  // rows c, c + 8, c + 16, c + 24
 #pragma unroll
-        for (int i = 0; i < 2 * MT; ++i) xr[i] = (mine >> (c + 8 * i)) & 1u ? x.row(row0 + c + 8 * i) : nullptr;
+        for (int i = 0; i < 4; ++i) xr[i] = VEC || ((mine >> (c + 8 * i)) & 1u) ? x.row<VEC>(row0 + c + 8 * i) : x.data;
         for (int j0 = 0; j0 < r; j0 += kCols) {
-            float acc[MT][NT][4] = {};
-            for (int k0 = 32 * (rank * kWarps + warp); k0 < k_len; k0 += 32 * kWarps * ranks) {
-                float xv[2][2 * MT][4];
+            float acc[2][NT][4] = {};
+            auto sweep = [&](auto whole) {
+                constexpr bool WV = decltype(whole)::value;
+                const int step = 32 * kWarps * ranks, k_first = 32 * (rank * kWarps + warp);
+                auto fetch = [&](int k, int stage) {
+                    const uint32_t place = ring + stage * Ring::kStage;
 #pragma unroll
-                for (int s = 0; s < 2; ++s)
+                    for (int s = 0; s < 2; ++s) {
+                        const int kg = k + 16 * s + 4 * q;
 #pragma unroll
-                    for (int i = 0; i < 2 * MT; ++i) load_x4<VEC>(xr[i], x.nb0, k0 + 16 * s + 4 * q, k_len, xv[s][i]);
+                        for (int i = 0; i < 4; ++i)
+                            ring_x4<VEC>(place + (4 * s + i) * 512 + lane * 16, xr[i], (mine >> (c + 8 * i)) & 1u, x.nb0, kg, k_len);
+                        if constexpr (WV) {
+                            const uint32_t wplace = place + Ring::kX + s * NT * 32 * 4 * sizeof(W) + lane * kPiece;
+                            if constexpr (!BACK) {
 #pragma unroll
-                for (int s = 0; s < 2; ++s) {
-                    const int kg = k0 + 16 * s + 4 * q;
-                    float wv[NT][4];
-                    if constexpr (!BACK) {
+                                for (int n = 0; n < NT; ++n) {
+                                    const int j = j0 + 8 * n + c;
+                                    ring_w<kPiece>(wplace + n * 32 * kPiece, w + static_cast<int64_t>(j) * k_len + kg, j < r && kg < k_len);
+                                }
+                            } else {
 #pragma unroll
-                        for (int n = 0; n < NT; ++n) {
-                            const int j = j0 + 8 * n + c;
-                            load_w4(w, static_cast<int64_t>(j) * k_len + kg, j < r ? k_len - kg : 0, vec, wv[n]);
-                        }
-                    } else {
+                                for (int e = 0; e < 4; ++e)
 #pragma unroll
-                        for (int e = 0; e < 4; ++e)
-#pragma unroll
-                            for (int n = 0; n < NT; n += V) {
-                                const int j = j0 + 8 * n + V * c;
-                                const int have = kg + e < k_len ? r - j : 0;
-                                float t[V];
-                                if constexpr (V == 4) load_w4(w, static_cast<int64_t>(kg + e) * r + j, have, vec, t);
-                                else load_w2(w, static_cast<int64_t>(kg + e) * r + j, have, vec, t);
-#pragma unroll
-                                for (int i = 0; i < V; ++i) wv[n + i][e] = t[i];
+                                    for (int n = 0; n < NT; n += V) {
+                                        const int j = j0 + 8 * n + V * c;
+                                        ring_w<kPiece>(wplace + (e * (NT / V) + n / V) * 32 * kPiece,
+                                                       w + static_cast<int64_t>(kg + e) * r + j, j < r && kg < k_len);
+                                    }
                             }
+                        }
                     }
-                    uint32_t ah[2][MT][4], at[2][MT][4];
+                    ring_commit();
+                };
 #pragma unroll
-                    for (int m = 0; m < MT; ++m)
+                for (int p = 0; p < kStages - 1; ++p) fetch(k_first + p * step, p);
+                int stage = 0;
+                for (int k0 = k_first; k0 < k_len; k0 += step) {
+                    fetch(k0 + (kStages - 1) * step, stage == 0 ? kStages - 1 : stage - 1);
+                    // the tensor core's own sums lose a little at every product: 32 columns at a time
+                    float d[2][NT][4] = {};
+                    ring_wait<kStages - 1>();
+                    const uint32_t place = ring + stage * Ring::kStage;
 #pragma unroll
-                        for (int u = 0; u < 2; ++u)
+                    for (int s = 0; s < 2; ++s) {
+                        const int kg = k0 + 16 * s + 4 * q;
+                        float wv[NT][4];
+                        const uint32_t wplace = place + Ring::kX + s * NT * 32 * 4 * sizeof(W) + lane * kPiece;
+                        if constexpr (!BACK) {
+#pragma unroll
+                            for (int n = 0; n < NT; ++n) {
+                                const int j = j0 + 8 * n + c;
+                                if constexpr (WV) ring_take_w<W, 4>(wplace + n * 32 * kPiece, wv[n]);
+                                else load_w<W, 4, false>(w + static_cast<int64_t>(j) * k_len + kg, j < r ? k_len - kg : 0, wv[n]);
+                            }
+                        } else {
+#pragma unroll
+                            for (int e = 0; e < 4; ++e)
+#pragma unroll
+                                for (int n = 0; n < NT; n += V) {
+                                    const int j = j0 + 8 * n + V * c;
+                                    float t[V];
+                                    if constexpr (WV) ring_take_w<W, V>(wplace + (e * (NT / V) + n / V) * 32 * kPiece, t);
+                                    else load_w<W, V, false>(w + static_cast<int64_t>(kg + e) * r + j, kg + e < k_len ? r - j : 0, t);
+#pragma unroll
+                                    for (int i = 0; i < V; ++i) wv[n + i][e] = t[i];
+                                }
+                        }
+                        uint32_t ah[2][2][4], at[2][2][4];
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            float xv[4];
+                            ring_take(place + (4 * s + i) * 512 + lane * 16, xv);
 #pragma unroll
                             for (int e = 0; e < 4; ++e)  // a[e]: row c + 8 (e & 1), value 2u + (e >> 1)
-                                split(xv[s][2 * m + (e & 1)][2 * u + (e >> 1)], ah[u][m][e], at[u][m][e]);
+                                split(xv[e], ah[e >> 1][i >> 1][(i & 1) + 2 * (e & 1)], at[e >> 1][i >> 1][(i & 1) + 2 * (e & 1)]);
+                        }
 #pragma unroll
-                    for (int n = 0; n < NT; ++n) {
-                        if (j0 + 8 * (BACK ? n / V * V : n) >= r) continue;  // the same for the whole warp
-                        uint32_t bh[2][2], bt[2][2];
+                        for (int n = 0; n < NT; ++n) {
+                            if (NT > 2 && j0 + 8 * (BACK ? n / V * V : n) >= r) continue;  // the same for the whole warp
+                            uint32_t bh[2][2], bt[2][2];
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) split_b<HALF>(wv[n][e], bh[e >> 1][e & 1], bt[e >> 1][e & 1]);
+                            for (int e = 0; e < 4; ++e) split_b<HALF>(wv[n][e], bh[e >> 1][e & 1], bt[e >> 1][e & 1]);
 #pragma unroll
-                        for (int m = 0; m < MT; ++m) {
-                            // the tensor core's own sums lose a little at every step: 16 columns at a time
-                            float d[4] = {};
-                            mma_split<HALF>(d, ah[0][m], at[0][m], bh[0], bt[0]);
-                            mma_split<HALF>(d, ah[1][m], at[1][m], bh[1], bt[1]);
+                            for (int u = 0; u < 2; ++u)
 #pragma unroll
-                            for (int e = 0; e < 4; ++e) acc[m][n][e] += d[e];
+                                for (int m = 0; m < 2; ++m) mma_split<HALF>(d[m][n], ah[u][m], at[u][m], bh[u], bt[u]);
                         }
                     }
+#pragma unroll
+                    for (int m = 0; m < 2; ++m)
+#pragma unroll
+                        for (int n = 0; n < NT; ++n)
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) acc[m][n][e] += d[m][n][e];
+                    stage = stage + 1 == kStages ? 0 : stage + 1;
                 }
-            }
+                ring_wait<0>();
+            };
+            if (VEC && (A.vec & (BACK ? 2 : 1)) != 0) sweep(True());
+            else sweep(False());
+            __syncthreads();  // the partial sums take the rings' place
             // partial sums of the 8 warps, then of the cluster
             float* mywarp = red + warp * kRows * kCols;
 #pragma unroll
-            for (int m = 0; m < MT; ++m)
+            for (int m = 0; m < 2; ++m)
 #pragma unroll
                 for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -289,7 +424,7 @@ __global__ void __launch_bounds__(kThreads) down_kernel(const __grid_constant__ 
                 float s = red[i];
 #pragma unroll
                 for (int v = 1; v < kWarps; ++v) s += red[v * kRows * kCols + i];
-                red[i] = s;  // only this thread reads or writes column i
+                red[i] = s;  // only this thread reads or writes place i
             }
             if (ranks > 1) cluster_sync();
             else __syncthreads();
@@ -316,148 +451,191 @@ __global__ void __launch_bounds__(kThreads) down_kernel(const __grid_constant__ 
 }
 
 // ------------------------------------------------------------------ up: d = base + h W^T
-// A warp takes 16 * MT rows and walks over groups of 16 columns; wr warps of a CTA stand side by side in the
-// rows (the factor's values then come from L1 for all but one), the others in the columns. The two 8-column
-// tiles of a group take columns 4 (c >> 1) + 2 i + (c & 1), i = 0, 1, so that a lane ends up with four
-// consecutive columns of a row: 16-byte loads of base and stores of d. Every row has one adapter at most,
-// so the adapters of a tile (and the slices of the grid that share them) write rows of their own.
-template <typename W, bool BACK, int JG, int MT, bool VEC>
-__global__ void __launch_bounds__(kThreads) up_kernel(const __grid_constant__ Adapters tab, const int32_t* ids, Rows base, Rows d,
-                                                      int64_t rows, int n_len, const float* h, int ld, int wr, int iters, int col_blocks) {
+// A warp takes 32 rows, holds their h, and walks over groups of 16 columns; wr warps of a CTA stand side by
+// side in the rows (the factor's values then come from L1 for all but one), the others in the columns. The two
+// 8-column tiles of a group take columns 4 (c >> 1) + 2 i + (c & 1), i = 0, 1, so that a lane ends up with four
+// consecutive columns of a row: 16-byte loads of base and stores of d. Every row has one adapter at most, so the
+// adapters of a tile (and the slices of the grid that share them) go one after the other, each with its own
+// rows.
+template <typename W, bool BACK, int JG, bool VEC>
+__global__ void __launch_bounds__(kThreads, UpRing<W, BACK, JG>::kCtas) up_kernel(const __grid_constant__ Adapters tab, const int32_t* ids,
+                                                                      Rows base, Rows d, int64_t rows, int n_len, const float* h,
+                                                                      int ld, int wr, int iters, int col_blocks) {
     constexpr bool HALF = sizeof(W) == 2;
-    constexpr int  kRows = 16 * MT;
-    const int     warp = threadIdx.x >> 5, lane = threadIdx.x & 31, c = lane >> 2, q = lane & 3;
-    const int     wn = kWarps / wr;
-    const int64_t row0 = (static_cast<int64_t>(blockIdx.x / col_blocks) * wr + warp % wr) * kRows;
-    const int     group0 = static_cast<int>(blockIdx.x % col_blocks) * wn * iters + warp / wr, groups = (n_len + 15) / 16;
-    const TileIds tile(ids, row0, kRows, rows, tab.n);
+    constexpr bool HELD = JG == 1;  // h is held as heads and tails
+    constexpr int  kRows = 32;
+    extern __shared__ __align__(16) char up_smem[];  // the warps' rings
+    const int      warp = threadIdx.x >> 5, lane = threadIdx.x & 31, c = lane >> 2, q = lane & 3;
+    using Ring = UpRing<W, BACK, JG>;
+    constexpr int  kStages = Ring::kStages, kPiece = 4 * static_cast<int>(sizeof(W)), kPieces = BACK ? 4 : 2;  // of 16 ranks
+    const uint32_t ring = smem_u32(up_smem) + warp * (kStages * Ring::kStage);
+    const int      wn = kWarps / wr;
+    const int64_t  row0 = (static_cast<int64_t>(blockIdx.x / col_blocks) * wr + warp % wr) * kRows;
+    const int      first = 16 * (static_cast<int>(blockIdx.x % col_blocks) * wn * iters + warp / wr), stride = 16 * wn;
+    const int      last = min(n_len, first + stride * iters);
+    const TileIds  tile(ids, row0, kRows, rows, tab.n);
     grid_wait();  // h is written
-    if (row0 >= rows) return;
+    if (row0 >= rows || first >= n_len) return;
 
-    float hv[JG][2 * MT][4];  // the first 16 * JG ranks of rows c, c + 8, ...: values 4q .. 4q + 3 of each 16
+    float hv[JG][4][4];  // the first 16 * JG ranks of rows c, c + 8, ...: values 4q .. 4q + 3 of each 16
+    auto load_h = [&](int j0) {
 #pragma unroll
-    for (int i = 0; i < 2 * MT; ++i) {
-        const bool live = row0 + c + 8 * i < rows;
+        for (int i = 0; i < 4; ++i)
 #pragma unroll
-        for (int g = 0; g < JG; ++g) {
-            float4 t = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            if (live && 16 * g < ld) t = *reinterpret_cast<const float4*>(h + (row0 + c + 8 * i) * ld + 16 * g + 4 * q);
-            hv[g][i][0] = t.x; hv[g][i][1] = t.y; hv[g][i][2] = t.z; hv[g][i][3] = t.w;
-        }
+            for (int g = 0; g < JG; ++g) {
+                float4 t = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                if (row0 + c + 8 * i < rows && j0 + 16 * g < ld)
+                    t = *reinterpret_cast<const float4*>(h + (row0 + c + 8 * i) * ld + j0 + 16 * g + 4 * q);
+                hv[g][i][0] = t.x; hv[g][i][1] = t.y; hv[g][i][2] = t.z; hv[g][i][3] = t.w;
+            }
+    };
+    load_h(0);
+    uint32_t hh[2][2][4], ht[2][2][4];  // [rows 16 m][step]
+    auto split_h = [&](int g) {
+#pragma unroll
+        for (int m = 0; m < 2; ++m)
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) split(hv[g][2 * m + (e & 1)][2 * u + (e >> 1)], hh[m][u][e], ht[m][u][e]);
+    };
+    if constexpr (HELD) split_h(0);
+
+    // rows without an adapter: the first slice copies their base
+    const uint32_t none = __ballot_sync(0xFFFFFFFFu, tile.id < 0 && row0 + lane < rows);
+    if (none != 0 && blockIdx.z == 0 && base.data != d.data) {
+        for (int n0 = first; n0 < last; n0 += stride)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if ((none >> (c + 8 * i)) & 1u) {
+                    const int64_t t = row0 + c + 8 * i;
+                    float y[4] = {};
+                    if (base.data != nullptr) load_x4<VEC>(base.row<VEC>(t), base.nb0, n0 + 4 * q, n_len, y);
+                    store_x4<VEC>(d.row<VEC>(t), d.nb0, n0 + 4 * q, n_len, y);
+                }
     }
-    for (int it = 0; it < iters; ++it) {
-        const int group = group0 + it * wn;
-        if (group >= groups) break;
-        const int n0 = 16 * group;
-        float y[2 * MT][4];  // columns n0 + 4q .. + 3 of rows c + 8 i
-        bool  keep[2 * MT];  // rows that this slice writes
+    int turn = 0;
+    for (uint32_t left = tile.leaders; left != 0; left &= left - 1) {
+        if (turn++ % gridDim.z != blockIdx.z) continue;
+        const int      lead = __ffs(left) - 1;
+        const int      id = __shfl_sync(0xFFFFFFFFu, tile.id, lead);
+        const uint32_t mine = __shfl_sync(0xFFFFFFFFu, tile.same, lead) >> c;  // bit 8 i: row c + 8 i
+        const Adapter& A = tab.ad[id];
+        const int      r = A.rank;
+        const W*       w = static_cast<const W*>(BACK ? A.a : A.b);
+        const bool     add = base.data != nullptr;
+        const char*    in[4];
+        char*          out[4];
 #pragma unroll
-        for (int i = 0; i < 2 * MT; ++i) {
-            const int64_t t = row0 + c + 8 * i;
-            const int     id = __shfl_sync(0xFFFFFFFFu, tile.id, c + 8 * i);
-            const uint32_t same = __shfl_sync(0xFFFFFFFFu, tile.same, c + 8 * i);
-            // the turn of the row's adapter among the tile's; rows without one go with the first slice
-            const uint32_t turn = id >= 0 ? __popc(tile.leaders & ((same & (~same + 1u)) - 1u)) % gridDim.z : 0u;
-            keep[i] = t < rows && turn == blockIdx.z;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) y[i][e] = 0.0f;
-            if (keep[i] && base.data != nullptr) load_x4<VEC>(base.row(t), base.nb0, n0 + 4 * q, n_len, y[i]);
+        for (int i = 0; i < 4; ++i) {
+            const bool live = (mine >> (8 * i)) & 1u;
+            in[i]  = (VEC || live) && add ? base.row<VEC>(row0 + c + 8 * i) : base.data;
+            out[i] = VEC || live ? d.row<VEC>(row0 + c + 8 * i) : d.data;
         }
-        int turn = 0;
-        for (uint32_t left = tile.leaders; left != 0; left &= left - 1) {
-            if (turn++ % gridDim.z != blockIdx.z) continue;
-            const int      lead = __ffs(left) - 1;
-            const int      id = __shfl_sync(0xFFFFFFFFu, tile.id, lead);
-            const uint32_t mine = __shfl_sync(0xFFFFFFFFu, tile.same, lead);
-            const Adapter& A = tab.ad[id];
-            const int      r = A.rank;
-            const W*       w = static_cast<const W*>(BACK ? A.a : A.b);
-            const bool     vec = (A.vec & (BACK ? 1 : 2)) != 0;
-            float acc[MT][2][4] = {};
-            for (int j0 = 0; j0 < r; j0 += 16 * JG) {
-                float hj[JG][2 * MT][4];
+        // RING: the factor's values come through the ring (they are whole, and all ranks are held); else straight from
+        // memory, in whole loads (WV) or one by one.
+        auto walk = [&](auto through, auto whole) {
+            constexpr bool RING = decltype(through)::value, WV = decltype(whole)::value;
+            // group g's piece i: FWD tile i's column n0 + 4 (c >> 1) + (c & 1) + 2 i, ranks 4q ..; BACK rank 4q + i, columns
+            // n0 + 4 (c >> 1) ..
+            auto piece = [&](int n0, int j0, int g, int i, int& have) -> const W* {
+                const int jq = j0 + 16 * g + 4 * q;
+                if constexpr (!BACK) {
+                    const int n = n0 + 4 * (c >> 1) + (c & 1) + 2 * i;
+                    have = n < n_len ? r - jq : 0;
+                    return w + (static_cast<int64_t>(n) * r + jq);
+                } else {
+                    const int n = n0 + 4 * (c >> 1);
+                    have = jq + i < r ? n_len - n : 0;
+                    return w + (static_cast<int64_t>(jq + i) * n_len + n);
+                }
+            };
+            auto fetch = [&](int n0, int stage) {
+                const uint32_t place = ring + stage * Ring::kStage;
+                if (add)
 #pragma unroll
-                for (int g = 0; g < JG; ++g)
-#pragma unroll
-                    for (int i = 0; i < 2 * MT; ++i)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) hj[g][i][e] = hv[g][i][e];
-                if (j0 > 0) {  // ranks beyond 16 * JG: from memory for each group of columns
+                    for (int i = 0; i < 4; ++i)
+                        ring_x4<VEC>(place + i * 512 + lane * 16, in[i], ((mine >> (8 * i)) & 1u) && n0 < last, base.nb0,
+                                     n0 + 4 * q, n_len);
+                if constexpr (RING)
 #pragma unroll
                     for (int g = 0; g < JG; ++g)
 #pragma unroll
-                        for (int i = 0; i < 2 * MT; ++i) {
-                            float4 t = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                            if (row0 + c + 8 * i < rows && j0 + 16 * g < ld)
-                                t = *reinterpret_cast<const float4*>(h + (row0 + c + 8 * i) * ld + j0 + 16 * g + 4 * q);
-                            hj[g][i][0] = t.x; hj[g][i][1] = t.y; hj[g][i][2] = t.z; hj[g][i][3] = t.w;
+                        for (int i = 0; i < kPieces; ++i) {
+                            int have;
+                            const W* p = piece(n0, 0, g, i, have);
+                            ring_w<kPiece>(place + Ring::kX + (g * kPieces + i) * 32 * kPiece + lane * kPiece, p, have > 0 && n0 < last);
                         }
-                }
+                ring_commit();
+            };
 #pragma unroll
-                for (int g = 0; g < JG; ++g) {
-                    if (j0 + 16 * g >= r) continue;
-                    const int jq = j0 + 16 * g + 4 * q;
-                    float wv[2][4];  // tile i, ranks jq .. jq + 3
-                    if constexpr (!BACK) {
+            for (int p = 0; p < kStages - 1; ++p) fetch(first + p * stride, p);
+            int stage = 0;
+            for (int n0 = first; n0 < last; n0 += stride) {
+                fetch(n0 + (kStages - 1) * stride, stage == 0 ? kStages - 1 : stage - 1);
+                const uint32_t place = ring + stage * Ring::kStage;
+                ring_wait<kStages - 1>();
+                float acc[2][2][4] = {};
+                for (int j0 = 0; j0 < (RING ? 1 : r); j0 += 16 * JG) {
+                    if (!RING && r > 16 * JG) load_h(j0);  // ranks beyond the ones held: anew for each group of columns
+                    float wv[JG][2][4];
 #pragma unroll
-                        for (int i = 0; i < 2; ++i) {
-                            const int n = n0 + 4 * (c >> 1) + 2 * i + (c & 1);
-                            load_w4(w, static_cast<int64_t>(n) * r + jq, n < n_len ? r - jq : 0, vec, wv[i]);
+                    for (int g = 0; g < JG; ++g)
+#pragma unroll
+                        for (int i = 0; i < kPieces; ++i) {
+                            float p[4];
+                            if constexpr (RING) {
+                                ring_take_w<W, 4>(place + Ring::kX + (g * kPieces + i) * 32 * kPiece + lane * kPiece, p);
+                            } else {
+                                int have;
+                                const W* from = piece(n0, j0, g, i, have);
+                                load_w<W, 4, WV>(from, have, p);
+                            }
+                            if constexpr (!BACK) {
+#pragma unroll
+                                for (int e = 0; e < 4; ++e) wv[g][i][e] = p[e];
+                            } else {
+                                wv[g][0][i] = c & 1 ? p[1] : p[0];
+                                wv[g][1][i] = c & 1 ? p[3] : p[2];
+                            }
                         }
-                    } else {
+                    float t[2][2][4] = {};
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const int n = n0 + 4 * (c >> 1);
-                            float t[4];
-                            load_w4(w, static_cast<int64_t>(jq + e) * n_len + n, jq + e < r ? n_len - n : 0, vec, t);
-                            wv[0][e] = c & 1 ? t[1] : t[0];
-                            wv[1][e] = c & 1 ? t[3] : t[2];
-                        }
-                    }
-                    uint32_t bh[2][2][2], bt[2][2][2];  // [step][tile]
+                    for (int g = 0; g < JG; ++g) {
+                        if (JG > 1 && j0 + 16 * g >= r) continue;
+                        uint32_t bh[2][2][2], bt[2][2][2];  // [tile][step]
 #pragma unroll
-                    for (int i = 0; i < 2; ++i)
+                        for (int i = 0; i < 2; ++i)
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) split_b<HALF>(wv[i][e], bh[e >> 1][i][e & 1], bt[e >> 1][i][e & 1]);
-#pragma unroll
-                    for (int m = 0; m < MT; ++m) {
-                        uint32_t ah[2][4], at[2][4];
+                            for (int e = 0; e < 4; ++e) split_b<HALF>(wv[g][i][e], bh[i][e >> 1][e & 1], bt[i][e >> 1][e & 1]);
+                        if constexpr (!HELD) split_h(g);
 #pragma unroll
                         for (int u = 0; u < 2; ++u)
 #pragma unroll
-                            for (int e = 0; e < 4; ++e)
-                                split(hj[g][2 * m + (e & 1)][2 * u + (e >> 1)], ah[u][e], at[u][e]);
+                            for (int m = 0; m < 2; ++m)
 #pragma unroll
-                        for (int i = 0; i < 2; ++i) {
-                            float t[4] = {};
-                            mma_split<HALF>(t, ah[0], at[0], bh[0][i], bt[0][i]);
-                            mma_split<HALF>(t, ah[1], at[1], bh[1][i], bt[1][i]);
-#pragma unroll
-                            for (int e = 0; e < 4; ++e) acc[m][i][e] += t[e];
-                        }
+                                for (int i = 0; i < 2; ++i) mma_split<HALF>(t[m][i], hh[m][u], ht[m][u], bh[i][u], bt[i][u]);
                     }
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) acc[e >> 3][(e >> 2) & 1][e & 3] += t[e >> 3][(e >> 2) & 1][e & 3];
                 }
-            }
 #pragma unroll
-            for (int i = 0; i < 2 * MT; ++i)  // row c + 8 i: sums 2 (i & 1) .. of tile 0, then of tile 1
-                if ((mine >> (c + 8 * i)) & 1u) {
+                for (int i = 0; i < 4; ++i) {  // row c + 8 i: sums 2 (i & 1) .. of tile 0, then of tile 1
+                    float y[4] = {};
+                    if (add) ring_take(place + i * 512 + lane * 16, y);
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) y[i][e] += acc[i >> 1][e >> 1][2 * (i & 1) + (e & 1)];
+                    for (int e = 0; e < 4; ++e) y[e] += acc[i >> 1][e >> 1][2 * (i & 1) + (e & 1)];
+                    if ((mine >> (8 * i)) & 1u) store_x4<VEC>(out[i], d.nb0, n0 + 4 * q, n_len, y);
                 }
-        }
-#pragma unroll
-        for (int i = 0; i < 2 * MT; ++i) {
-            if (!keep[i]) continue;
-            char* out = d.row(row0 + c + 8 * i);
-            const int n = n0 + 4 * q;
-            if (VEC && n + 4 <= n_len) {
-                *reinterpret_cast<float4*>(out + 4ll * n) = make_float4(y[i][0], y[i][1], y[i][2], y[i][3]);
-            } else {
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    if (n + e < n_len) *reinterpret_cast<float*>(out + (n + e) * d.nb0) = y[i][e];
+                stage = stage + 1 == kStages ? 0 : stage + 1;
             }
-        }
+            ring_wait<0>();
+        };
+        const bool whole = VEC && (A.vec & (BACK ? 1 : 2)) != 0;
+        if (whole && (JG < 4 || r <= 16 * JG)) walk(True(), True());
+        else if (JG == 4 && whole) walk(False(), True());
+        else walk(False(), False());
+        if (JG == 4 && r > 16 * JG) load_h(0);
     }
 }
 
@@ -472,16 +650,15 @@ struct GradSide {
     const float* h;
     int32_t      k_len;
     int32_t      strips;  // of 128 columns
-    int32_t      vec;
 };
 
-template <int MT>
-__global__ void __launch_bounds__(kThreads) grad_kernel(const __grid_constant__ Adapters tab, const int32_t* ids,
+template <int MT, bool VEC>
+__global__ void __launch_bounds__(kThreads, GradRing<MT>::kCtas) grad_kernel(const __grid_constant__ Adapters tab, const int32_t* ids,
                                                         const __grid_constant__ GradSide side_a,
                                                         const __grid_constant__ GradSide side_b, int64_t rows, int ld,
                                                         int accumulate) {
     constexpr int kR = 16 * MT;
-    __shared__ float sum[kR][128 + 4];
+    extern __shared__ __align__(16) char grad_smem[];  // the warps' rings, then sums of [kR][128 + 4]
     const int  warp = threadIdx.x >> 5, lane = threadIdx.x & 31, c = lane >> 2, q = lane & 3;
     const int  ranks = static_cast<int>(cluster_nctarank()), rank = static_cast<int>(cluster_ctarank());
     int        strip = static_cast<int>(blockIdx.x) / ranks;
@@ -495,37 +672,78 @@ __global__ void __launch_bounds__(kThreads) grad_kernel(const __grid_constant__ 
     if (out == nullptr || j0 >= r) return;  // the whole cluster
     const int col = strip * 128 + (warp & 3) * 32 + 4 * c;
 
+    // Steps of 32 rows t0 + q + 4 e; a step without a row of this adapter is passed over.
     float acc[MT][4][4] = {};
-    const int64_t tiles = (rows + 31) / 32;
-    for (int64_t i = rank + static_cast<int64_t>(warp >> 2) * ranks; i < tiles; i += 2 * ranks) {
-        const int64_t  t0 = i * 32;
-        const uint32_t mine = __ballot_sync(0xFFFFFFFFu, t0 + lane < rows && adapter_of(ids, t0 + lane, tab.n) == static_cast<int>(blockIdx.z));
-        if (mine == 0) continue;
+    const int64_t  steps = (rows + 31) / 32, hop = 2 * ranks;
+    using Ring = GradRing<MT>;
+    constexpr int  kStages = Ring::kStages, kPiece = MT == 1 ? 8 : 16, kPieces = MT == 4 ? 2 : 1;  // of a row's 2 MT ranks
+    const uint32_t ring = smem_u32(grad_smem) + warp * (kStages * Ring::kStage);
+    int64_t  ahead = rank + static_cast<int64_t>(warp >> 2) * ranks - hop;  // the step fetched last
+    uint32_t at_rows[kStages] = {};  // the rows of the steps in the ring, the oldest step first
+    auto fetch = [&](int stage) {
+        uint32_t mine = 0;
+        while (mine == 0 && ahead + hop < steps) {
+            ahead += hop;
+            const int64_t t = ahead * 32 + lane;
+            mine = __ballot_sync(0xFFFFFFFFu, t < rows && adapter_of(ids, t, tab.n) == static_cast<int>(blockIdx.z));
+        }
+        at_rows[kStages - 1] = mine;
+        if (mine != 0) {
+            const uint32_t place = ring + stage * Ring::kStage;
+            const int64_t  t = ahead * 32 + q;
+            const char*    xr = S.x.row<VEC>(t);
+            const float*   hr = S.h + t * ld + j0 + 2 * MT * c;
 #pragma unroll
-        for (int s = 0; s < 2; ++s) {  // 16 rows: t0 + 16 s + q + 4 e
-            if (((mine >> (16 * s)) & 0xFFFFu) == 0) continue;
-            float xv[4][4], hv[4][2 * MT];
+            for (int e = 0; e < 8; ++e) {
+                const bool live = (mine >> (q + 4 * e)) & 1u;
+                if constexpr (!VEC) xr = live ? S.x.row<VEC>(t + 4 * e) : S.x.data;
+                ring_x4<VEC>(place + e * 512 + lane * 16, xr, live, S.x.nb0, col, S.k_len);
+                if constexpr (VEC) xr += 16ll * S.x.step;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const int  l = 16 * s + q + 4 * e;
-                const bool live = (mine >> l) & 1u;
-                const char* xr = live ? S.x.row(t0 + l) : nullptr;
-                if (S.vec) load_x4<true>(xr, 4, col, S.k_len, xv[e]);
-                else load_x4<false>(xr, S.x.nb0, col, S.k_len, xv[e]);
-                const float* hr = S.h + (t0 + l) * ld + j0 + 2 * MT * c;
-#pragma unroll
-                for (int j = 0; j < 2 * MT; j += 2) {
-                    float2 t = make_float2(0.0f, 0.0f);
-                    if (live && j0 + 2 * MT * c + j < ld) t = *reinterpret_cast<const float2*>(hr + j);
-                    hv[e][j] = t.x;
-                    hv[e][j + 1] = t.y;
-                }
+                for (int i = 0; i < kPieces; ++i)
+                    ring_w<kPiece>(place + Ring::kX + ((e * kPieces + i) * 32 + lane) * kPiece, hr + 4 * i,
+                                   live && j0 + 2 * MT * c + 4 * i < ld);
+                hr += 4 * ld;
             }
-            uint32_t bh[2][4][2], bt[2][4][2];  // [8 rows][tile]
+        }
+        ring_commit();
+    };
+    auto shift = [&]() {
+#pragma unroll
+        for (int p = 0; p + 1 < kStages; ++p) at_rows[p] = at_rows[p + 1];
+    };
+#pragma unroll
+    for (int p = 0; p < kStages - 1; ++p) {
+        shift();
+        fetch(p);
+    }
+    for (int stage = 0;; stage = stage + 1 == kStages ? 0 : stage + 1) {
+        shift();
+        fetch(stage == 0 ? kStages - 1 : stage - 1);
+        if (at_rows[0] == 0) break;  // nothing follows
+        ring_wait<kStages - 1>();
+        const uint32_t place = ring + stage * Ring::kStage;
+        float d[MT][4][4] = {};
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+            float hv[4][2 * MT];
 #pragma unroll
             for (int e = 0; e < 4; ++e)
 #pragma unroll
-                for (int n = 0; n < 4; ++n) split(xv[e][n], bh[e >> 1][n][e & 1], bt[e >> 1][n][e & 1]);
+                for (int i = 0; i < kPieces; ++i) {
+                    float p[kPiece / 4];
+                    ring_take_w<float, kPiece / 4>(place + Ring::kX + (((4 * s + e) * kPieces + i) * 32 + lane) * kPiece, p);
+#pragma unroll
+                    for (int j = 0; j < kPiece / 4; ++j) hv[e][4 * i + j] = p[j];
+                }
+            uint32_t bh[2][4][2], bt[2][4][2];  // [8 rows][tile]
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                float xv[4];
+                ring_take(place + (4 * s + e) * 512 + lane * 16, xv);
+#pragma unroll
+                for (int n = 0; n < 4; ++n) split(xv[n], bh[e >> 1][n][e & 1], bt[e >> 1][n][e & 1]);
+            }
 #pragma unroll
             for (int m = 0; m < MT; ++m) {
                 uint32_t ah[2][4], at[2][4];
@@ -536,15 +754,21 @@ __global__ void __launch_bounds__(kThreads) grad_kernel(const __grid_constant__ 
                         split(hv[2 * u + (e >> 1)][2 * m + (e & 1)], ah[u][e], at[u][e]);
 #pragma unroll
                 for (int n = 0; n < 4; ++n) {
-                    float d[4] = {};
-                    mma_split<false>(d, ah[0], at[0], bh[0][n], bt[0][n]);
-                    mma_split<false>(d, ah[1], at[1], bh[1][n], bt[1][n]);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) acc[m][n][e] += d[e];
+                    mma_split<false>(d[m][n], ah[0], at[0], bh[0][n], bt[0][n]);
+                    mma_split<false>(d[m][n], ah[1], at[1], bh[1][n], bt[1][n]);
                 }
             }
         }
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+            for (int n = 0; n < 4; ++n)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) acc[m][n][e] += d[m][n][e];
     }
+    ring_wait<0>();
+    __syncthreads();  // the sums take the rings' place
+    float (*sum)[128 + 4] = reinterpret_cast<float (*)[128 + 4]>(grad_smem);
     // the two row halves of the CTA, then the cluster
     const int col0 = (warp & 3) * 32;
 #pragma unroll
@@ -638,15 +862,15 @@ Rows rows_of(const trc_cuda_view* v) {
     r.n2 = static_cast<int32_t>(v->ne[2]);
     // one stride for all rows, whichever extents are 1
     int64_t step = 0, want = 0, count = 1;
-    r.flat = 1;
+    bool    even = true;
     for (int i = 1; i < 4; ++i) {
         if (v->ne[i] == 1) continue;
         if (count == 1) step = v->nb[i];
-        else if (v->nb[i] != want) r.flat = 0;
+        else if (v->nb[i] != want) even = false;
         count *= v->ne[i];
         want = step * count;
     }
-    if (r.flat) r.nb1 = step;
+    r.step = even && step / 4 <= INT32_MAX ? static_cast<int32_t>(step / 4) : -1;
     return r;
 }
 
@@ -661,10 +885,11 @@ void make_table(Adapters& t, const trc_cuda_lora_adapter* ad, int n, int type, i
     }
 }
 
-// Rows of floats side by side that start at multiples of 16 bytes.
+// Evenly spaced rows of a multiple of four floats, side by side, that start at multiples of 16 bytes.
 bool vec_rows(const trc_cuda_view* v) {
     if (v == nullptr) return true;
-    if (!aligned_to(v->data, 16) || (v->ne[0] > 1 && v->nb[0] != 4)) return false;
+    if (rows_of(v).step < 0) return false;
+    if (!aligned_to(v->data, 16) || v->ne[0] % 4 != 0 || v->nb[0] != 4) return false;
     for (int i = 1; i < 4; ++i)
         if (v->ne[i] > 1 && (v->nb[i] & 15) != 0) return false;
     return true;
@@ -698,31 +923,37 @@ int launch(const void* kernel, dim3 grid, unsigned cluster, size_t smem, bool af
     return TRC_CUDA_OK;
 }
 
-// A power of two up to `most` that brings `count` units to about `want`.
-int power_for(int64_t count, int64_t want, int most) {
+// The largest power of two up to `most` with which `count` units stay within `room`.
+int power_for(int64_t count, int64_t room, int most) {
     int p = 1;
-    while (p < most && count * p < want) p *= 2;
+    while (p < most && 2 * p * count <= room) p *= 2;
     return p;
 }
 
 // CTAs that a launch aims at: two for each SM.
 int64_t full_grid() { return 2 * static_cast<int64_t>(std::max(1, sm_count_current())); }
 
-template <typename W, bool BACK, int NT, int MT>
+// Allows a kernel more than 48 KB of shared memory.
+int allow_smem(const void* kernel, size_t smem) {
+    if (smem <= 48 * 1024) return TRC_CUDA_OK;
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+    return e == cudaSuccess ? TRC_CUDA_OK : cuda_fail(e);
+}
+
+template <typename W, bool BACK, int NT>
 int run_down(const Adapters& tab, const int32_t* ids, const Rows& x, bool vec, int64_t rows, int k, float* h, int ld,
              cudaStream_t s) {
-    const int64_t tiles = (rows + 16 * MT - 1) / (16 * MT);
-    // the columns of one tile go to 1 - 8 CTAs while each of their warps keeps a step of 32
-    const int cluster = std::min(power_for(tiles, full_grid(), 8), power_for(1, (k + 255) / 256, 8));
-    const int64_t most = std::min<int64_t>({tab.n, 16 * MT, rows});
-    const int64_t slices = std::max<int64_t>(1, std::min(most, full_grid() / (tiles * cluster)));
-    const size_t smem = sizeof(float) * kWarps * 16 * MT * 8 * NT;
-    const void* kernel = vec ? reinterpret_cast<const void*>(&down_kernel<W, BACK, NT, MT, true>)
-                             : reinterpret_cast<const void*>(&down_kernel<W, BACK, NT, MT, false>);
-    if (smem > 48 * 1024) {
-        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
-        if (e != cudaSuccess) return cuda_fail(e);
-    }
+    const int64_t tiles = (rows + 31) / 32;
+    // one wave of CTAs: the columns of a tile go to 1 - 8 of them while each of their warps keeps a step of 32
+    const int64_t room = full_grid() * DownRing<W, NT>::kCtas / 2;
+    const int cluster = std::min(power_for(tiles, room, 8), power_for(1, (k + 255) / 256, 8));
+    const int64_t most = std::min<int64_t>({tab.n, 32, rows});
+    const int64_t slices = std::max<int64_t>(1, std::min(most, room / (tiles * cluster)));
+    const size_t smem = std::max<size_t>(sizeof(float) * kWarps * 32 * 8 * NT, DownRing<W, NT>::kBytes);
+    const void* kernel = vec ? reinterpret_cast<const void*>(&down_kernel<W, BACK, NT, true>)
+                             : reinterpret_cast<const void*>(&down_kernel<W, BACK, NT, false>);
+    const int st = allow_smem(kernel, smem);
+    if (st != TRC_CUDA_OK) return st;
     void* args[] = {const_cast<Adapters*>(&tab), &ids, const_cast<Rows*>(&x), &rows, &k, &h, &ld};
     return launch(kernel, dim3(static_cast<unsigned>(tiles * cluster), static_cast<unsigned>(slices)), cluster, smem, false, args, s);
 }
@@ -730,48 +961,41 @@ int run_down(const Adapters& tab, const int32_t* ids, const Rows& x, bool vec, i
 template <bool BACK, typename W>
 int down_of(const Adapters& tab, const int32_t* ids, const Rows& x, bool vec, int64_t rows, int k, float* h, int ld,
             cudaStream_t s) {
-    if (rows <= 16) {
-        if (ld == 16) return run_down<W, BACK, 2, 1>(tab, ids, x, vec, rows, k, h, ld, s);
-        if (ld == 32) return run_down<W, BACK, 4, 1>(tab, ids, x, vec, rows, k, h, ld, s);
-        return run_down<W, BACK, 8, 1>(tab, ids, x, vec, rows, k, h, ld, s);
-    }
-    if (ld == 16) return run_down<W, BACK, 2, 2>(tab, ids, x, vec, rows, k, h, ld, s);
-    if (ld == 32) return run_down<W, BACK, 4, 2>(tab, ids, x, vec, rows, k, h, ld, s);
-    return run_down<W, BACK, 8, 2>(tab, ids, x, vec, rows, k, h, ld, s);
+    if (ld == 16) return run_down<W, BACK, 2>(tab, ids, x, vec, rows, k, h, ld, s);
+    if (ld == 32) return run_down<W, BACK, 4>(tab, ids, x, vec, rows, k, h, ld, s);
+    return run_down<W, BACK, 8>(tab, ids, x, vec, rows, k, h, ld, s);
 }
 
-template <typename W, bool BACK, int JG, int MT>
+template <typename W, bool BACK, int JG>
 int run_up(const Adapters& tab, const int32_t* ids, const Rows& base, const Rows& d, bool vec, int64_t rows, int n,
            const float* h, int ld, cudaStream_t s) {
-    const int64_t tiles = (rows + 16 * MT - 1) / (16 * MT), groups = (n + 15) / 16;
+    const int64_t tiles = (rows + 31) / 32, groups = (n + 15) / 16;
     int wr = power_for(1, tiles, 4);  // warps side by side in the rows
     const int64_t row_blocks = (tiles + wr - 1) / wr;
-    int iters = 8;
+    int iters = 16;
     while (iters > 1 && row_blocks * (groups / (iters * (kWarps / wr))) < 2 * full_grid()) iters /= 2;
     const int64_t col_blocks = (groups + iters * (kWarps / wr) - 1) / (iters * (kWarps / wr));
-    const int64_t most = std::min<int64_t>({tab.n, 16 * MT, rows});
+    const int64_t most = std::min<int64_t>({tab.n, 32, rows});
     const int64_t slices = std::max<int64_t>(1, std::min(most, 2 * full_grid() / (row_blocks * col_blocks)));
-    const void* kernel = vec ? reinterpret_cast<const void*>(&up_kernel<W, BACK, JG, MT, true>)
-                             : reinterpret_cast<const void*>(&up_kernel<W, BACK, JG, MT, false>);
+    const void* kernel = vec ? reinterpret_cast<const void*>(&up_kernel<W, BACK, JG, true>)
+                             : reinterpret_cast<const void*>(&up_kernel<W, BACK, JG, false>);
     if (row_blocks * col_blocks > INT32_MAX) return TRC_CUDA_EUNSUPPORTED;
     const dim3 grid(static_cast<unsigned>(row_blocks * col_blocks), 1, static_cast<unsigned>(slices));
+    const size_t smem = UpRing<W, BACK, JG>::kBytes;
+    const int st = allow_smem(kernel, smem);
+    if (st != TRC_CUDA_OK) return st;
     int cols = static_cast<int>(col_blocks);
     void* args[] = {const_cast<Adapters*>(&tab), &ids, const_cast<Rows*>(&base), const_cast<Rows*>(&d), &rows, &n, &h, &ld, &wr,
                     &iters, &cols};
-    return launch(kernel, grid, 1, 0, true, args, s);
+    return launch(kernel, grid, 1, smem, true, args, s);
 }
 
 template <bool BACK, typename W>
 int up_of(const Adapters& tab, const int32_t* ids, const Rows& base, const Rows& d, bool vec, int64_t rows, int n,
           const float* h, int ld, cudaStream_t s) {
-    if (rows <= 16) {
-        if (ld == 16) return run_up<W, BACK, 1, 1>(tab, ids, base, d, vec, rows, n, h, ld, s);
-        if (ld == 32) return run_up<W, BACK, 2, 1>(tab, ids, base, d, vec, rows, n, h, ld, s);
-        return run_up<W, BACK, 4, 1>(tab, ids, base, d, vec, rows, n, h, ld, s);
-    }
-    if (ld == 16) return run_up<W, BACK, 1, 2>(tab, ids, base, d, vec, rows, n, h, ld, s);
-    if (ld == 32) return run_up<W, BACK, 2, 2>(tab, ids, base, d, vec, rows, n, h, ld, s);
-    return run_up<W, BACK, 4, 2>(tab, ids, base, d, vec, rows, n, h, ld, s);
+    if (ld == 16) return run_up<W, BACK, 1>(tab, ids, base, d, vec, rows, n, h, ld, s);
+    if (ld == 32) return run_up<W, BACK, 2>(tab, ids, base, d, vec, rows, n, h, ld, s);
+    return run_up<W, BACK, 4>(tab, ids, base, d, vec, rows, n, h, ld, s);
 }
 
 template <bool BACK>
@@ -804,19 +1028,23 @@ int grad(const Adapters& tab, const int32_t* ids, const trc_cuda_view* x, const 
         any_b = any_b || tab.ad[i].db != nullptr;
     }
     if (!any_a && !any_b) return TRC_CUDA_OK;
-    GradSide a{rows_of(x), g, static_cast<int32_t>(x->ne[0]), 0, vec_rows(x)};
-    GradSide b{rows_of(dy), h, static_cast<int32_t>(dy->ne[0]), 0, vec_rows(dy)};
+    GradSide a{rows_of(x), g, static_cast<int32_t>(x->ne[0]), 0};
+    GradSide b{rows_of(dy), h, static_cast<int32_t>(dy->ne[0]), 0};
     if (any_a) a.strips = (a.k_len + 127) / 128;
     if (any_b) b.strips = (b.k_len + 127) / 128;
     const int mt = std::min(ld / 16, 3) == 3 ? 4 : ld / 16;
     const unsigned chunks = static_cast<unsigned>((ld + 16 * mt - 1) / (16 * mt));
     const int64_t strips = a.strips + b.strips;
-    const int cluster = std::min(power_for(strips * tab.n * chunks, full_grid(), 8), power_for(1, (rows + 63) / 64, 8));
-    const void* kernel = mt == 1   ? reinterpret_cast<const void*>(&grad_kernel<1>)
-                         : mt == 2 ? reinterpret_cast<const void*>(&grad_kernel<2>)
-                                   : reinterpret_cast<const void*>(&grad_kernel<4>);
+    const int cluster = std::min(power_for(strips * tab.n * chunks, full_grid() / (mt == 1 ? 1 : 2), 8), power_for(1, (rows + 63) / 64, 8));
+    const bool vec = vec_rows(x) && vec_rows(dy);
+    const void* kernel = mt == 1   ? (vec ? reinterpret_cast<const void*>(&grad_kernel<1, true>) : reinterpret_cast<const void*>(&grad_kernel<1, false>))
+                         : mt == 2 ? (vec ? reinterpret_cast<const void*>(&grad_kernel<2, true>) : reinterpret_cast<const void*>(&grad_kernel<2, false>))
+                                   : (vec ? reinterpret_cast<const void*>(&grad_kernel<4, true>) : reinterpret_cast<const void*>(&grad_kernel<4, false>));
+    const size_t smem = mt == 1 ? GradRing<1>::kBytes : mt == 2 ? GradRing<2>::kBytes : GradRing<4>::kBytes;
+    const int st = allow_smem(kernel, smem);
+    if (st != TRC_CUDA_OK) return st;
     void* args[] = {const_cast<Adapters*>(&tab), &ids, &a, &b, &rows, &ld, &accumulate};
-    return launch(kernel, dim3(static_cast<unsigned>(strips * cluster), chunks, static_cast<unsigned>(tab.n)), cluster, 0,
+    return launch(kernel, dim3(static_cast<unsigned>(strips * cluster), chunks, static_cast<unsigned>(tab.n)), cluster, smem,
                   false, args, s);
 }
 
