@@ -362,6 +362,10 @@ typedef struct trc_cuda_lora_adapter {
  * negative status if one of them is not valid. */
 int64_t trc_cuda_lora_h_ld(const trc_cuda_lora_adapter* adapters, int n_adapters);
 
+/* 1 if trc_cuda_lora has to be given h for so many rows, 0 if h may be null (a decode batch, whose two
+ * products are one launch); a negative status if an adapter is not valid. */
+int trc_cuda_lora_needs_h(const trc_cuda_lora_adapter* adapters, int n_adapters, int64_t rows);
+
 /* d[:, t] = base[:, t] + scale * B (A x[:, t]) with the adapter ids[t] of row t.
  * x has ne = {K, n1, n2, n3}, base and d have ne = {N, n1, n2, n3}, any byte strides; t counts the
  * n1*n2*n3 rows in ggml order. `type` is the element type of every A and B: TRC_CUDA_TYPE_F32,
@@ -373,9 +377,9 @@ int64_t trc_cuda_lora_h_ld(const trc_cuda_lora_adapter* adapters, int n_adapters
  *     base in another way.
  *   - h: device buffer of rows * trc_cuda_lora_h_ld() floats, 16-byte aligned. It receives
  *     scale * A x (zeros behind a row's rank, and for a row without an adapter), which
- *     trc_cuda_lora_back takes.
- * Each output is the same whatever the other rows hold. A row with an infinity or a NaN in x
- * gives infinities or NaN in that row alone. */
+ *     trc_cuda_lora_back takes; see trc_cuda_lora_needs_h for when it may be null.
+ * What x holds in one row changes no other row's output: an infinity or a NaN there (values within
+ * 2^-12 of the largest float count as infinite) gives infinities or NaN in that row alone. */
 int trc_cuda_lora(int type, const trc_cuda_lora_adapter* adapters, int n_adapters, const int32_t* ids,
                   const trc_cuda_view* x, const trc_cuda_view* base, const trc_cuda_view* d, float* h,
                   void* stream);

@@ -128,6 +128,24 @@ def test_forward_and_gradients_half_factors(tc, kind, rows, k, n, ranks, order, 
 
 def test_256_adapters(tc):
     check_all(tc, 300, 64, 96, (2, 5, 9, 16) * 64, "f32", "mixed", 0)
+    check_all(tc, 256, 64, 96, (2, 5, 9, 16) * 64, "f32", "mixed", 0)
+
+
+@pytest.mark.parametrize("rows", [16, 17, 33, 256])
+@pytest.mark.parametrize("kind", ["f32", "f16"])
+def test_small_batches_with_all_rows_on_one_adapter(tc, rows, kind):
+    """A batch that is small for its many adapters, but only one of them (and -1) occurs: more rows than a tile."""
+    ad, ids, x, base, dy = make(rows, 200, 136, (8, 20, 16, 33) * 5, kind, order="mixed")
+    ids = torch.where(torch.arange(rows, device="cuda") % 9 == 4, -1, 6).int()
+    handle = tc.LoraAdapters(ad)
+    h = tc.lora_h(handle, x).fill_(float("nan"))
+    want = formula(ad, ids, x, base)[0]
+    y = tc.lora(handle, x, ids, base=base, h=h)
+    near(y, want)
+    assert torch.equal(tc.lora(handle, x, ids, base=base), y)  # with and without keeping h
+    a, _, c = ad[6]
+    near(h[ids == 6][:, :16], c * (x[ids == 6].double().cpu() @ a.double().cpu().t()))
+    assert bool((h[ids == 6][:, 16:] == 0).all()) and bool((h[ids == -1] == 0).all())
 
 
 @pytest.mark.parametrize("layout", ["offset", "transposed", "batched", "padded"])

@@ -36,8 +36,7 @@ def table(*entries):
 def lora(adapters=None, kind=F32, ids=0x100, x=None, base=None, d=None, h=H0):
     arr, n = adapters if adapters is not None else table((A0, B0, 4))
     x, d = x or view(64, 3, X0), d or view(32, 3, Y0)
-    ref = ctypes.byref
-    return trc_cuda.lib().trc_cuda_lora(kind, arr, n, ids, ref(x), None if base is None else ref(base), ref(d), h, None)
+    return trc_cuda.lib().trc_cuda_lora(kind, arr, n, ids, bytes(x), None if base is None else bytes(base), bytes(d), h, None)
 
 
 def test_constants_match_the_header():
@@ -55,8 +54,10 @@ def test_h_row_length_is_the_largest_rank_rounded_up():
         assert L.trc_cuda_lora_h_ld(arr, n) == ld
     assert L.trc_cuda_lora_h_ld(None, 0) == 16
     assert L.trc_cuda_lora_h_ld(None, 1) == EINVAL
+    assert L.trc_cuda_lora_needs_h(*table((A0, B0, 16)), 1) == 0 and L.trc_cuda_lora_needs_h(*table((A0, B0, 16)), 1000) == 1
+    assert L.trc_cuda_lora_needs_h(*table((A0, B0, 256)), 1) == 1
     arr, n = table((A0, B0, 257))
-    assert L.trc_cuda_lora_h_ld(arr, n) == EUNSUPPORTED
+    assert L.trc_cuda_lora_h_ld(arr, n) == EUNSUPPORTED and L.trc_cuda_lora_needs_h(arr, n, 1) == EUNSUPPORTED
     assert L.trc_cuda_lora_back_workspace_bytes(arr, n, 4) == 0
     assert L.trc_cuda_lora_back_workspace_bytes(*table((A0, B0, 17)), 4) >= 4 * 32 * 4
 
@@ -84,7 +85,7 @@ def test_h_row_length_is_the_largest_rank_rounded_up():
     (EUNSUPPORTED, {"x": view(64, 1 << 31, X0), "d": view(32, 1 << 31, Y0)}),
     (EUNSUPPORTED, {"x": view(64, 1 << 20, X0, n2=1 << 20), "d": view(32, 1 << 20, Y0, n2=1 << 20)}),
     (EINVAL, {"ids": 0x102}),
-    (EINVAL, {"h": None}),
+    (EINVAL, {"x": view(64, 300, X0), "d": view(32, 300, Y0), "h": None}),  # many rows: their h goes through memory
     (EINVAL, {"h": H0 + 4}),
     (0, {"x": view(64, 0, X0), "d": view(32, 0, Y0), "h": None}),    # no rows: nothing to do
 ])
@@ -107,7 +108,7 @@ def test_lora_checks_its_arguments(want, kw):
 def test_lora_back_checks_its_arguments(want, kw):
     arr, n = table((A0, B0, 4))
     k = {"flags": 0, "x": view(64, 3, X0), "dy": view(32, 3, Y0), "h": H0, "base": None, "dx": None, "ws": W0, "ws_bytes": 1 << 20, **kw}
-    ref = lambda v: None if v is None else ctypes.byref(v)  # noqa: E731
+    ref = lambda v: None if v is None else bytes(v)  # noqa: E731
     got = trc_cuda.lib().trc_cuda_lora_back(F32, arr, n, 0x100, ref(k["x"]), ref(k["dy"]), k["h"], ref(k["base"]), ref(k["dx"]),
                                             k["ws"], k["ws_bytes"], k["flags"], None)
     assert got == want

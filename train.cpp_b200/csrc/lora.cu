@@ -639,6 +639,238 @@ __global__ void __launch_bounds__(kThreads, UpRing<W, BACK, JG>::kCtas) up_kerne
     }
 }
 
+// ------------------------------------------------------------------ few rows: both products in one launch
+// A decode batch: up to 256 rows, each a request of its own, so the time is what it takes to bring the
+// adapters' factors in once. One cluster of 8 CTAs takes one adapter (and, where there are few of them, one of gridDim.x / 8
+// parts of the columns): it looks its rows up in ids, gathers them 16 at a time, and computes their h with the columns
+// of x shared among its 64 warps; every CTA then adds the 8 CTAs' partial sums up for itself and goes on with its share of
+// the output's columns, whose factor values are already on their way. The last slice of the grid takes the rows without an
+// adapter. Against the two launches of down and up: 64 rows of 16 adapters (ranks 8 - 64, 4096 -> 11008, bf16)
+// @@, one row of one adapter (rank 16, 4096 -> 4096, f16) @@.
+constexpr int kFewRows = 256, kFewCtas = 8;
+
+template <typename W, int NT>
+struct FewRing {
+    static constexpr int kDownX = 4 * 512, kDownW = 2 * NT * 32 * 4 * static_cast<int>(sizeof(W));
+    static constexpr int kUpX = 2 * 512, kUpW = NT * 32 * 4 * static_cast<int>(sizeof(W));
+    static constexpr int kStage = kDownX + kDownW, kStages = 2;
+    static constexpr int kUpStages = 2 * kStage / (kUpX + kUpW) >= 4 ? 4 : 2 * kStage / (kUpX + kUpW);
+    static constexpr int kWarp = kStages * kStage;
+    static constexpr int kPart = 16 * 8 * NT;  // floats of one warp's partial sums
+    static constexpr int kBytes = kWarps * kWarp + (kWarps + 1) * kPart * 4;
+};
+
+template <typename W, int NT, bool VEC>
+__global__ void __launch_bounds__(kThreads) few_kernel(const __grid_constant__ Adapters tab, const int32_t* ids, Rows x, Rows base,
+                                                       Rows d, int rows, int k_len, int n_len, float* h, int ld) {
+    constexpr bool HALF = sizeof(W) == 2;
+    using Ring = FewRing<W, NT>;
+    constexpr int JG = NT / 2, kCols = 8 * NT, kPiece = 4 * static_cast<int>(sizeof(W));
+    extern __shared__ __align__(16) char few_smem[];
+    __shared__ int16_t list[kFewRows];
+    __shared__ int     counts[kWarps];
+    const int      warp = threadIdx.x >> 5, lane = threadIdx.x & 31, c = lane >> 2, q = lane & 3;
+    const uint32_t ring = smem_u32(few_smem) + warp * Ring::kWarp;
+    float* part = reinterpret_cast<float*>(few_smem + kWarps * Ring::kWarp);
+    float* hs = part + kWarps * Ring::kPart;
+    const int rank = static_cast<int>(cluster_ctarank());
+    const int a = static_cast<int>(blockIdx.y);
+    const bool none = a == tab.n;
+
+    // this adapter's rows, in their order
+    int total = 0;
+    {
+        const int      t = static_cast<int>(threadIdx.x);
+        const int      id = t < rows ? adapter_of(ids, t, tab.n) : -2;
+        const bool     hit = id == (none ? -1 : a);
+        const uint32_t hits = __ballot_sync(0xFFFFFFFFu, hit);
+        if (lane == 0) counts[warp] = __popc(hits);
+        __syncthreads();
+        int before = 0;
+#pragma unroll
+        for (int v = 0; v < kWarps; ++v) {
+            if (v < warp) before += counts[v];
+            total += counts[v];
+        }
+        if (hit) list[before + __popc(hits & ((1u << lane) - 1u))] = static_cast<int16_t>(t);
+        __syncthreads();
+    }
+    if (total == 0) return;  // the whole cluster
+
+    const int first = 16 * (static_cast<int>(blockIdx.x) * kWarps + warp), stride = 16 * kWarps * static_cast<int>(gridDim.x);
+    if (none) {
+        for (int i = 0; i < total; ++i) {
+            const int64_t t = list[i];
+            if (h != nullptr && blockIdx.x == 0)
+                for (int j = threadIdx.x; j < ld; j += kThreads) h[t * ld + j] = 0.0f;
+            if (base.data == d.data) continue;
+            for (int n = blockIdx.x * kThreads + threadIdx.x; n < n_len; n += kThreads * gridDim.x)
+                *reinterpret_cast<float*>(d.row<false>(t) + n * d.nb0) =
+                    base.data != nullptr ? *reinterpret_cast<const float*>(base.row<false>(t) + n * base.nb0) : 0.0f;
+        }
+        return;
+    }
+    const Adapter& A = tab.ad[a];
+    const int      r = A.rank;
+    const W*       wa = static_cast<const W*>(A.a);
+    const W*       wb = static_cast<const W*>(A.b);
+    const bool     whole_a = VEC && (A.vec & 1) != 0, whole_b = VEC && (A.vec & 2) != 0;
+    const bool     add = base.data != nullptr;
+    for (int at = 0; at < total; at += 16) {
+        int  t[2];
+        bool live[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            live[i] = at + c + 8 * i < total;
+            t[i] = live[i] ? list[at + c + 8 * i] : 0;
+        }
+        // h: this warp's steps of 32 columns
+        float acc[NT][4] = {};
+        const char* xr[2] = {x.row<VEC>(t[0]), x.row<VEC>(t[1])};
+        const int   step = 32 * kWarps * kFewCtas;
+        auto fetch = [&](int k, int stage) {
+            const uint32_t place = ring + stage * Ring::kStage;
+#pragma unroll
+            for (int s = 0; s < 2; ++s) {
+                const int kg = k + 16 * s + 4 * q;
+                if (whole_a)
+#pragma unroll
+                    for (int n = 0; n < NT; ++n)
+                        ring_w<kPiece>(place + Ring::kDownX + ((s * NT + n) * 32 + lane) * kPiece,
+                                       wa + static_cast<int64_t>(8 * n + c) * k_len + kg, 8 * n + c < r && kg < k_len);
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+                    ring_x4<VEC>(place + (2 * s + i) * 512 + lane * 16, xr[i], live[i], x.nb0, kg, k_len);
+            }
+            ring_commit();
+        };
+        int k0 = 32 * (rank * kWarps + warp), stage = 0;
+        fetch(k0, 0);
+        for (; k0 < k_len; k0 += step, stage ^= 1) {
+            fetch(k0 + step, stage ^ 1);
+            ring_wait<1>();
+            const uint32_t place = ring + stage * Ring::kStage;
+            float dsum[NT][4] = {};
+#pragma unroll
+            for (int s = 0; s < 2; ++s) {
+                uint32_t ah[2][4], at_[2][4];
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    float xv[4];
+                    ring_take(place + (2 * s + i) * 512 + lane * 16, xv);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) split(xv[e], ah[e >> 1][i + 2 * (e & 1)], at_[e >> 1][i + 2 * (e & 1)]);
+                }
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    if (NT > 2 && 8 * n >= r) continue;
+                    const int kg = k0 + 16 * s + 4 * q, j = 8 * n + c;
+                    float wv[4];
+                    if (whole_a) ring_take_w<W, 4>(place + Ring::kDownX + ((s * NT + n) * 32 + lane) * kPiece, wv);
+                    else load_w<W, 4, false>(wa + static_cast<int64_t>(j) * k_len + kg, j < r ? k_len - kg : 0, wv);
+                    uint32_t bh[2][2], bt[2][2];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) split_b<HALF>(wv[e], bh[e >> 1][e & 1], bt[e >> 1][e & 1]);
+                    mma_split<HALF>(dsum[n], ah[0], at_[0], bh[0], bt[0]);
+                    mma_split<HALF>(dsum[n], ah[1], at_[1], bh[1], bt[1]);
+                }
+            }
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) acc[n][e] += dsum[n][e];
+        }
+        ring_wait<0>();
+        // the first groups of columns set out
+        const char* in[2] = {add ? base.row<VEC>(t[0]) : nullptr, add ? base.row<VEC>(t[1]) : nullptr};
+        char*       out[2] = {d.row<VEC>(t[0]), d.row<VEC>(t[1])};
+        auto fetch_up = [&](int n0, int st) {
+            const uint32_t place = ring + st * (Ring::kUpX + Ring::kUpW);
+            if (whole_b)
+#pragma unroll
+                for (int g = 0; g < JG; ++g)
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        const int n = n0 + 4 * (c >> 1) + (c & 1) + 2 * i, jq = 16 * g + 4 * q;
+                        ring_w<kPiece>(place + Ring::kUpX + ((g * 2 + i) * 32 + lane) * kPiece, wb + (static_cast<int64_t>(n) * r + jq),
+                                       n < n_len && jq < r);
+                    }
+            if (add)
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+                    ring_x4<VEC>(place + i * 512 + lane * 16, in[i], live[i] && n0 < n_len, base.nb0, n0 + 4 * q, n_len);
+            ring_commit();
+        };
+#pragma unroll
+        for (int p = 0; p < Ring::kUpStages - 1; ++p) fetch_up(first + p * stride, p);
+        // partial sums: of the CTA's warps, then of the cluster's CTAs
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                part[warp * Ring::kPart + (c + 8 * (e >> 1)) * kCols + 8 * n + 2 * q + (e & 1)] = acc[n][e];
+        __syncthreads();
+        for (int i = threadIdx.x; i < Ring::kPart; i += kThreads) {
+            float s = part[i];
+#pragma unroll
+            for (int v = 1; v < kWarps; ++v) s += part[v * Ring::kPart + i];
+            part[i] = s;
+        }
+        cluster_sync();
+        for (int i = threadIdx.x; i < Ring::kPart; i += kThreads) {
+            float s = 0.0f;
+#pragma unroll
+            for (int v = 0; v < kFewCtas; ++v) s += ld_cluster(mapa_shared(part + i, v));
+            s = i % kCols < r ? s * A.scale : 0.0f;
+            hs[i] = s;
+            if (h != nullptr && blockIdx.x == 0 && at + i / kCols < total && i % kCols < ld)
+                h[static_cast<int64_t>(list[at + i / kCols]) * ld + i % kCols] = s;
+        }
+        cluster_sync();  // every CTA has read the partial sums, and this one's h is complete
+        for (int n0 = first, st = 0; n0 < n_len; n0 += stride, st = st + 1 == Ring::kUpStages ? 0 : st + 1) {
+            fetch_up(n0 + (Ring::kUpStages - 1) * stride, st == 0 ? Ring::kUpStages - 1 : st - 1);
+            ring_wait<Ring::kUpStages - 1>();
+            const uint32_t place = ring + st * (Ring::kUpX + Ring::kUpW);
+            float y[2][4] = {};
+#pragma unroll
+            for (int g = 0; g < JG; ++g) {
+                if (JG > 1 && 16 * g >= r) continue;
+                uint32_t ah[2][4], at_[2][4];
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const float4 hv = *reinterpret_cast<const float4*>(hs + (c + 8 * i) * kCols + 16 * g + 4 * q);
+                    split(hv.x, ah[0][i], at_[0][i]);
+                    split(hv.y, ah[0][i + 2], at_[0][i + 2]);
+                    split(hv.z, ah[1][i], at_[1][i]);
+                    split(hv.w, ah[1][i + 2], at_[1][i + 2]);
+                }
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const int n = n0 + 4 * (c >> 1) + (c & 1) + 2 * i, jq = 16 * g + 4 * q;
+                    float wv[4];
+                    if (whole_b) ring_take_w<W, 4>(place + Ring::kUpX + ((g * 2 + i) * 32 + lane) * kPiece, wv);
+                    else load_w<W, 4, false>(wb + (static_cast<int64_t>(n) * r + jq), n < n_len ? r - jq : 0, wv);
+                    uint32_t bh[2][2], bt[2][2];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) split_b<HALF>(wv[e], bh[e >> 1][e & 1], bt[e >> 1][e & 1]);
+                    mma_split<HALF>(y[i], ah[0], at_[0], bh[0], bt[0]);
+                    mma_split<HALF>(y[i], ah[1], at_[1], bh[1], bt[1]);
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {  // row c + 8 i
+                float v[4] = {};
+                if (add) ring_take(place + i * 512 + lane * 16, v);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[e] += y[e >> 1][2 * i + (e & 1)];
+                if (live[i]) store_x4<VEC>(out[i], d.nb0, n0 + 4 * q, n_len, v);
+            }
+        }
+        ring_wait<0>();
+        __syncthreads();  // hs and the rings before the next rows
+    }
+}
+
 // ------------------------------------------------------------------ gradients of the factors
 // out(j, k) (+)= sum over the adapter's rows t of h[t, j] x[t, k]; dA (h = g, x) is j-major, dB (h, x = dy)
 // k-major. The ranks are the 16-row side of the tensor core's tile, so a warp holds all ranks (up to 64)
@@ -940,6 +1172,11 @@ int allow_smem(const void* kernel, size_t smem) {
     return e == cudaSuccess ? TRC_CUDA_OK : cuda_fail(e);
 }
 
+// Into how many slices the adapters of a tile go, with `most` of them there and `room` for slices in a full grid:
+// at least 4, so that the tiles at the borders between requests, which have two adapters or three, do not take two or three
+// times as long as the rest (2048 rows, ranks 64, 32, 64: @@); a slice without work ends at once.
+int64_t slices_for(int64_t most, int64_t room) { return std::max<int64_t>(1, std::min(most, std::max<int64_t>(room, 4))); }
+
 template <typename W, bool BACK, int NT>
 int run_down(const Adapters& tab, const int32_t* ids, const Rows& x, bool vec, int64_t rows, int k, float* h, int ld,
              cudaStream_t s) {
@@ -948,7 +1185,7 @@ int run_down(const Adapters& tab, const int32_t* ids, const Rows& x, bool vec, i
     const int64_t room = full_grid() * DownRing<W, NT>::kCtas / 2;
     const int cluster = std::min(power_for(tiles, room, 8), power_for(1, (k + 255) / 256, 8));
     const int64_t most = std::min<int64_t>({tab.n, 32, rows});
-    const int64_t slices = std::max<int64_t>(1, std::min(most, room / (tiles * cluster)));
+    const int64_t slices = slices_for(most, room / (tiles * cluster));
     const size_t smem = std::max<size_t>(sizeof(float) * kWarps * 32 * 8 * NT, DownRing<W, NT>::kBytes);
     const void* kernel = vec ? reinterpret_cast<const void*>(&down_kernel<W, BACK, NT, true>)
                              : reinterpret_cast<const void*>(&down_kernel<W, BACK, NT, false>);
@@ -972,11 +1209,12 @@ int run_up(const Adapters& tab, const int32_t* ids, const Rows& base, const Rows
     const int64_t tiles = (rows + 31) / 32, groups = (n + 15) / 16;
     int wr = power_for(1, tiles, 4);  // warps side by side in the rows
     const int64_t row_blocks = (tiles + wr - 1) / wr;
+    const int64_t slots = full_grid() * UpRing<W, BACK, JG>::kCtas / 2;
     int iters = 16;
-    while (iters > 1 && row_blocks * (groups / (iters * (kWarps / wr))) < 2 * full_grid()) iters /= 2;
+    while (iters > 1 && 2 * row_blocks * (groups / (iters * (kWarps / wr))) < 3 * slots) iters /= 2;
     const int64_t col_blocks = (groups + iters * (kWarps / wr) - 1) / (iters * (kWarps / wr));
     const int64_t most = std::min<int64_t>({tab.n, 32, rows});
-    const int64_t slices = std::max<int64_t>(1, std::min(most, 2 * full_grid() / (row_blocks * col_blocks)));
+    const int64_t slices = std::max<int64_t>(1, std::min(most, slots / (row_blocks * col_blocks)));
     const void* kernel = vec ? reinterpret_cast<const void*>(&up_kernel<W, BACK, JG, true>)
                              : reinterpret_cast<const void*>(&up_kernel<W, BACK, JG, false>);
     if (row_blocks * col_blocks > INT32_MAX) return TRC_CUDA_EUNSUPPORTED;
@@ -996,6 +1234,45 @@ int up_of(const Adapters& tab, const int32_t* ids, const Rows& base, const Rows&
     if (ld == 16) return run_up<W, BACK, 1>(tab, ids, base, d, vec, rows, n, h, ld, s);
     if (ld == 32) return run_up<W, BACK, 2>(tab, ids, base, d, vec, rows, n, h, ld, s);
     return run_up<W, BACK, 4>(tab, ids, base, d, vec, rows, n, h, ld, s);
+}
+
+// Both products for a batch of few rows (h may be null: then it is not wanted).
+template <typename W, int NT>
+int run_few(const Adapters& tab, const int32_t* ids, const Rows& x, const Rows& base, const Rows& d, bool vec, int rows, int k,
+            int n, float* h, int ld, cudaStream_t s) {
+    const void* kernel = vec ? reinterpret_cast<const void*>(&few_kernel<W, NT, true>) : reinterpret_cast<const void*>(&few_kernel<W, NT, false>);
+    const size_t smem = FewRing<W, NT>::kBytes;
+    const int st = allow_smem(kernel, smem);
+    if (st != TRC_CUDA_OK) return st;
+    // parts of the columns: one CTA for each SM as long as a part has a group of 16 for every warp
+    const int64_t groups = (n + 15) / 16, present = std::max(1, std::min(tab.n, rows));
+    const int64_t parts = std::max<int64_t>(1, std::min(full_grid() / 2 / (present * kFewCtas), groups / (kFewCtas * kWarps)));
+    void* args[] = {const_cast<Adapters*>(&tab), &ids, const_cast<Rows*>(&x), const_cast<Rows*>(&base), const_cast<Rows*>(&d), &rows, &k, &n, &h, &ld};
+    return launch(kernel, dim3(static_cast<unsigned>(parts * kFewCtas), static_cast<unsigned>(tab.n + 1)), kFewCtas, smem, false, args, s);
+}
+
+template <typename W>
+int few_of(const Adapters& tab, const int32_t* ids, const Rows& x, const Rows& base, const Rows& d, bool vec, int rows, int k,
+           int n, float* h, int ld, cudaStream_t s) {
+    if (ld == 16) return run_few<W, 2>(tab, ids, x, base, d, vec, rows, k, n, h, ld, s);
+    if (ld == 32) return run_few<W, 4>(tab, ids, x, base, d, vec, rows, k, n, h, ld, s);
+    return run_few<W, 8>(tab, ids, x, base, d, vec, rows, k, n, h, ld, s);
+}
+
+// Whether the one-launch form takes a batch: its clusters go through an adapter's rows 16 at a time, one after the other, so
+// it is for batches of about that many rows for each adapter, and for ranks whose partial sums fit its shared memory.
+bool is_few(int64_t rows, int n_adapters, int64_t ld) {
+    return ld <= 64 && (rows <= 16 || (rows <= kFewRows && rows <= 16 * static_cast<int64_t>(n_adapters)));
+}
+
+int few(int type, const Adapters& tab, const int32_t* ids, const trc_cuda_view* x, const trc_cuda_view* base,
+        const trc_cuda_view* d, int64_t rows, float* h, int ld, cudaStream_t s) {
+    const Rows rx = rows_of(x), rb = rows_of(base), rd = rows_of(d);
+    const int k = static_cast<int>(x->ne[0]), n = static_cast<int>(d->ne[0]), t = static_cast<int>(rows);
+    const bool vec = vec_rows(x) && vec_rows(base) && vec_rows(d);
+    if (type == TRC_CUDA_TYPE_F32) return few_of<float>(tab, ids, rx, rb, rd, vec, t, k, n, h, ld, s);
+    if (type == TRC_CUDA_TYPE_F16) return few_of<__half>(tab, ids, rx, rb, rd, vec, t, k, n, h, ld, s);
+    return few_of<__nv_bfloat16>(tab, ids, rx, rb, rd, vec, t, k, n, h, ld, s);
 }
 
 template <bool BACK>
@@ -1062,6 +1339,13 @@ int64_t trc_cuda_lora_h_ld(const trc_cuda_lora_adapter* adapters, int n_adapters
     return st == TRC_CUDA_OK ? ld : st;
 }
 
+int trc_cuda_lora_needs_h(const trc_cuda_lora_adapter* adapters, int n_adapters, int64_t rows) {
+    int64_t ld = 0;
+    const int st = check_adapters(adapters, n_adapters, 1, &ld);
+    if (st != TRC_CUDA_OK) return st;
+    return rows <= 0 || is_few(rows, n_adapters, ld) ? 0 : 1;
+}
+
 int trc_cuda_lora(int type, const trc_cuda_lora_adapter* adapters, int n_adapters, const int32_t* ids,
                   const trc_cuda_view* x, const trc_cuda_view* base, const trc_cuda_view* d, float* h, void* stream) {
     if (type != TRC_CUDA_TYPE_F32 && type != TRC_CUDA_TYPE_F16 && type != TRC_CUDA_TYPE_BF16) return TRC_CUDA_EUNSUPPORTED;
@@ -1075,10 +1359,12 @@ int trc_cuda_lora(int type, const trc_cuda_lora_adapter* adapters, int n_adapter
     if (!aligned_to(ids, 4)) return TRC_CUDA_EINVAL;
     const int64_t rows = d->ne[1] * d->ne[2] * d->ne[3];
     if (rows == 0) return TRC_CUDA_OK;
-    if (h == nullptr || !aligned_to(h, 16)) return TRC_CUDA_EINVAL;
+    const bool in_one = is_few(rows, n_adapters, ld);
+    if ((h == nullptr && !in_one) || !aligned_to(h, 16)) return TRC_CUDA_EINVAL;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     Adapters tab;
     make_table(tab, adapters, n_adapters, type, x->ne[0]);
+    if (in_one) return few(type, tab, ids, x, base, d, rows, h, static_cast<int>(ld), s);
     st = down<false>(type, tab, ids, x, rows, h, static_cast<int>(ld), s);
     if (st != TRC_CUDA_OK) return st;
     return up<false>(type, tab, ids, base, d, rows, h, static_cast<int>(ld), s);

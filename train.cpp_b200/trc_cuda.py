@@ -26,6 +26,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 from pathlib import Path
 from typing import Sequence
 
@@ -127,9 +128,11 @@ def lib() -> ctypes.CDLL:
         "trc_cuda_sum_sqr_acc": (I, [P, P, I64, P, SZ, P]),
         "trc_cuda_clip_scale_inplace": (I, [P, I64, P, ctypes.c_float, ctypes.c_float, P]),
         "trc_cuda_lora_h_ld": (I64, [ctypes.POINTER(LoraAdapter), I]),
-        "trc_cuda_lora": (I, [I, ctypes.POINTER(LoraAdapter), I, P, VP, VP, VP, P, P]),
+        "trc_cuda_lora_needs_h": (I, [ctypes.POINTER(LoraAdapter), I, I64]),
+        # views are passed as View structures or as their bytes
+        "trc_cuda_lora": (I, [I, ctypes.POINTER(LoraAdapter), I, P, P, P, P, P, P]),
         "trc_cuda_lora_back_workspace_bytes": (SZ, [ctypes.POINTER(LoraAdapter), I, I64]),
-        "trc_cuda_lora_back": (I, [I, ctypes.POINTER(LoraAdapter), I, P, VP, VP, P, VP, VP, P, SZ, U32, P]),
+        "trc_cuda_lora_back": (I, [I, ctypes.POINTER(LoraAdapter), I, P, P, P, P, P, P, P, SZ, U32, P]),
         "trc_cuda_opt_step_adamw_many": (I, [ctypes.POINTER(AdamwJob), I, I, P, P, ctypes.c_float, ctypes.c_float, P]),
         "trc_cuda_state8_to_f32": (I, [I, P, P, P, I64, P]),
         "trc_cuda_state8_from_f32": (I, [I, P, P, P, I64, P]),
@@ -712,20 +715,27 @@ def clip_scale_(a: torch.Tensor, norm: torch.Tensor, max_norm: float, eps: float
 
 
 # ------------------------------------------------------------------ scratch and device checks
+# The calls below are made for every layer and token, so their checks read each property of a tensor once.
 
-def _scratch(numel: int, dtype: torch.dtype, device, stream) -> torch.Tensor:
-    """Memory for a call's own use on `stream`: it belongs to that stream, so that it is not handed out
-    again while the call's kernels still use it."""
+def _raw_stream(stream: torch.cuda.Stream | None) -> int:
+    if stream is not None:
+        return stream.cuda_stream
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
+
+
+def _scratch(shape, dtype: torch.dtype, device, stream) -> torch.Tensor:
+    """Memory that a call on `stream` writes: it belongs to that stream, so that it is not handed out again
+    while the call's kernels still use it."""
     if stream is None:
-        return torch.empty(numel, dtype=dtype, device=device)
+        return torch.empty(shape, dtype=dtype, device=device)
     with torch.cuda.stream(stream):
-        return torch.empty(numel, dtype=dtype, device=device)
+        return torch.empty(shape, dtype=dtype, device=device)
 
 
 def _on_current_device(t: torch.Tensor, what: str) -> None:
     if not t.is_cuda:
         raise TrcCudaError(f"{what}: expected a CUDA tensor (device memory)")
-    if t.device.index != torch.cuda.current_device():
+    if t.get_device() != torch.cuda.current_device():
         raise TrcCudaError(f"{what}: the tensor is on {t.device}, the current device is cuda:{torch.cuda.current_device()}")
 
 
@@ -758,7 +768,8 @@ class LoraAdapters:
         if grads is not None and len(grads) != len(adapters):
             raise TrcCudaError("grads needs one entry for each adapter")
         self._keep, self._n, self._arr = [], len(adapters), (LoraAdapter * max(1, len(adapters)))()
-        self.k = self.n = self.type = self.device = None
+        self.k = self.n = self.device = None
+        self.type = TYPE_F32
         written = []
         for i, (a, b, scale) in enumerate(adapters):
             if a.dim() != 2 or b.dim() != 2 or a.shape[0] != b.shape[1]:
@@ -771,7 +782,7 @@ class LoraAdapters:
                 raise TrcCudaError(f"adapter {i}: the factors must be contiguous")
             _on_current_device(a, f"adapter {i}")
             _on_current_device(b, f"adapter {i}")
-            what = (a.shape[1], b.shape[0], _LORA_TYPES[a.dtype], a.device)
+            what = (a.shape[1], b.shape[0], _LORA_TYPES[a.dtype], a.get_device())
             if i == 0:
                 self.k, self.n, self.type, self.device = what
             elif what != (self.k, self.n, self.type, self.device):
@@ -796,46 +807,51 @@ class LoraAdapters:
         return self._n
 
 
-_I4 = ctypes.c_int64 * 4
+_VIEW = struct.Struct("9q").pack  # trc_cuda_view: data, ne[4], nb[4]
 
 
-def _rows_view(t: torch.Tensor, what: str) -> View:
-    """view_of, for a tensor whose last dimension is a row (ne0)."""
-    if t.dtype != torch.float32 or not t.is_cuda:
-        raise TrcCudaError(f"{what}: expected a float32 CUDA tensor")
-    if t.dim() == 2:  # the usual case, without the general form's work
-        (n1, n0), (s1, s0) = t.shape, t.stride()
-        return View(t.data_ptr(), _I4(n0, n1, 1, 1), _I4(4 * s0, 4 * s1, 4 * s1 * n1, 4 * s1 * n1))
-    return view_of(t)
+def _rows_view(t: torch.Tensor, device: int, lead: torch.Size, length: int, what: str) -> bytes:
+    """The ggml view of a tensor of rows: lead + (length,), or the same up to leading dimensions of 1."""
+    if t.dtype is not torch.float32 or t.get_device() != device:
+        raise TrcCudaError(f"{what}: expected a float32 CUDA tensor on cuda:{device}, got {t.dtype} on {t.device}")
+    shape = t.shape
+    if len(shape) == 2 and len(lead) == 1:  # the usual case
+        n1, n0 = shape
+        if n0 == length and n1 == lead[0]:
+            s1, s0 = t.stride()
+            return _VIEW(t.data_ptr(), n0, n1, 1, 1, 4 * s0, 4 * s1, 4 * s1 * n1, 4 * s1 * n1)
+    want = [1] * (4 - len(lead) - 1) + list(lead) + [length]
+    if ggml_ne(t) != want[::-1]:
+        raise TrcCudaError(f"{what}: expected {tuple(lead) + (length,)}, got {tuple(shape)}")
+    return bytes(view_of(t))
 
 
-def _lora_args(ad: LoraAdapters, x: torch.Tensor, ids: torch.Tensor | None, out_len: int | None, what: str) -> int:
-    """Checks what lora and lora_back share; returns the number of rows."""
-    _on_current_device(x, what)
-    if not 1 <= x.dim() <= 4:
+def _lora_args(ad: LoraAdapters, x: torch.Tensor, ids: torch.Tensor | None, out_len: int, what: str) -> tuple[int, int]:
+    """Checks what lora and lora_back share; returns x's device and its number of rows."""
+    device, dims = x.get_device(), x.dim()
+    if device < 0 or device != torch.cuda.current_device():
+        _on_current_device(x, what)
+    if not 1 <= dims <= 4:
         raise TrcCudaError(f"{what}: x has one to four dimensions")
-    rows = x.numel() // x.shape[-1] if x.shape[-1] else 0
-    if ad.k is not None and (x.shape[-1] != ad.k or x.device != ad.device):
-        raise TrcCudaError(f"{what}: x has rows of {x.shape[-1]} on {x.device}, the adapters take {ad.k} on {ad.device}")
-    if out_len is not None and ad.n is not None and out_len != ad.n:
-        raise TrcCudaError(f"{what}: base, out or dy has rows of {out_len}, the adapters give {ad.n}")
+    k = x.shape[-1]
+    rows = x.shape[0] if dims == 2 else x.numel() // k if k else 0
+    if ad.k is not None:
+        if k != ad.k or device != ad.device:
+            raise TrcCudaError(f"{what}: x has rows of {k} on cuda:{device}, the adapters take {ad.k} on cuda:{ad.device}")
+        if out_len != ad.n:
+            raise TrcCudaError(f"{what}: base, out or dy has rows of {out_len}, the adapters give {ad.n}")
     if ids is None:
-        if len(ad) != 1:
+        if ad._n != 1:
             raise TrcCudaError(f"{what}: ids may be left out for a single adapter only")
-    elif ids.dtype != torch.int32 or not ids.is_contiguous() or ids.numel() != rows or ids.device != x.device:
+    elif ids.dtype is not torch.int32 or ids.get_device() != device or ids.numel() != rows or not ids.is_contiguous():
         raise TrcCudaError(f"{what}: ids must be a contiguous int32 tensor with one entry for each of the {rows} rows")
-    return rows
+    return device, rows
 
 
-def _same_rows(t: torch.Tensor, x: torch.Tensor, length: int, what: str) -> None:
-    same = t.shape[:-1] == x.shape[:-1] or ggml_ne(t)[1:] == ggml_ne(x)[1:]  # leading dimensions of 1 may differ
-    if not same or t.shape[-1] != length or t.device != x.device:
-        raise TrcCudaError(f"{what}: expected {tuple(x.shape[:-1]) + (length,)} on {x.device}, got {tuple(t.shape)} on {t.device}")
-
-
-def _check_h(h: torch.Tensor, ad: LoraAdapters, x: torch.Tensor, rows: int, what: str) -> None:
-    if h.dtype != torch.float32 or h.device != x.device or not h.is_contiguous() or h.numel() != rows * ad.ld:
+def _check_h(h: torch.Tensor, ad: LoraAdapters, device: int, rows: int, what: str) -> int:
+    if h.dtype is not torch.float32 or h.get_device() != device or h.numel() != rows * ad.ld or not h.is_contiguous():
         raise TrcCudaError(f"{what}: h must be what lora_h gives for x")
+    return h.data_ptr()
 
 
 def lora_h(adapters: LoraAdapters, x: torch.Tensor) -> torch.Tensor:
@@ -850,22 +866,23 @@ def lora(adapters: LoraAdapters, x: torch.Tensor, ids: torch.Tensor | None = Non
     whose id is no adapter's (-1) keeps its base. base (..., N) is the shared projection's output (None: 0)
     and may be `out` itself. ids: int32, one for each row; None: the single adapter everywhere.
     h: a buffer of lora_h to keep for lora_back."""
-    n = base.shape[-1] if base is not None else out.shape[-1] if out is not None else adapters.n
+    n = adapters.n if base is None and out is None else (base if base is not None else out).shape[-1]
     if n is None:
         raise TrcCudaError("lora: without adapters, base or out has to say how long an output is")
-    rows = _lora_args(adapters, x, ids, n, "lora")
+    device, rows = _lora_args(adapters, x, ids, n, "lora")
+    lead, L = x.shape[:-1], lib()
+    vx = _rows_view(x, device, lead, x.shape[-1], "lora: x")
+    vb = None if base is None else _rows_view(base, device, lead, n, "lora: base")
     if out is None:
-        out = _scratch(x.shape[:-1] + (n,), torch.float32, x.device, stream)
-    _same_rows(out, x, n, "lora: out")
-    if base is not None:
-        _same_rows(base, x, n, "lora: base")
-    if h is None:
+        out = _scratch(lead + (n,), torch.float32, x.device, stream)
+    vd = _rows_view(out, device, lead, n, "lora: out")
+    if h is None and L.trc_cuda_lora_needs_h(adapters._arr, adapters._n, rows):
         h = _scratch((rows, adapters.ld), torch.float32, x.device, stream)
-    _check_h(h, adapters, x, rows, "lora")
-    vx, vd = _rows_view(x, "lora: x"), _rows_view(out, "lora: out")
-    vb = ctypes.byref(_rows_view(base, "lora: base")) if base is not None else None
-    _check(lib().trc_cuda_lora(adapters.type or 0, adapters._arr, adapters._n, None if ids is None else ids.data_ptr(),
-                               ctypes.byref(vx), vb, ctypes.byref(vd), h.data_ptr(), _stream(stream)), "trc_cuda_lora")
+    ptr = None if h is None else _check_h(h, adapters, device, rows, "lora")
+    status = L.trc_cuda_lora(adapters.type, adapters._arr, adapters._n, None if ids is None else ids.data_ptr(), vx, vb, vd,
+                             ptr, _raw_stream(stream))
+    if status:
+        _check(status, "trc_cuda_lora")
     return out
 
 
@@ -876,27 +893,24 @@ def lora_back(adapters: LoraAdapters, x: torch.Tensor, ids: torch.Tensor | None,
     dA and dB and returns dx = base + A^T (scale * B^T dy), base being the gradient that the shared
     projection's backward gives (None: 0; it may be `dx` itself). need_dx=False: no dx, returns None.
     x, ids and h are those of the forward call."""
-    rows = _lora_args(adapters, x, ids, dy.shape[-1], "lora_back")
-    _same_rows(dy, x, dy.shape[-1], "lora_back: dy")
-    _check_h(h, adapters, x, rows, "lora_back")
+    k, n = x.shape[-1], dy.shape[-1]
+    device, rows = _lora_args(adapters, x, ids, n, "lora_back")
+    lead, L = x.shape[:-1], lib()
+    vx = _rows_view(x, device, lead, k, "lora_back: x")
+    vy = _rows_view(dy, device, lead, n, "lora_back: dy")
+    ptr = _check_h(h, adapters, device, rows, "lora_back")
     if not need_dx and (dx is not None or base is not None):
         raise TrcCudaError("lora_back: dx and base go with need_dx")
     if need_dx and dx is None:
         dx = _scratch(x.shape, torch.float32, x.device, stream)
-    vd = vb = None
-    if dx is not None:
-        _same_rows(dx, x, x.shape[-1], "lora_back: dx")
-        vd = ctypes.byref(_rows_view(dx, "lora_back: dx"))
-    if base is not None:
-        _same_rows(base, x, x.shape[-1], "lora_back: base")
-        vb = ctypes.byref(_rows_view(base, "lora_back: base"))
-    vx, vy = _rows_view(x, "lora_back: x"), _rows_view(dy, "lora_back: dy")
-    need = int(lib().trc_cuda_lora_back_workspace_bytes(adapters._arr, adapters._n, rows))
+    vd = None if dx is None else _rows_view(dx, device, lead, k, "lora_back: dx")
+    vb = None if base is None else _rows_view(base, device, lead, k, "lora_back: base")
+    need = L.trc_cuda_lora_back_workspace_bytes(adapters._arr, adapters._n, rows)
     ws = _scratch(need, torch.uint8, x.device, stream)
-    _check(lib().trc_cuda_lora_back(adapters.type or 0, adapters._arr, adapters._n,
-                                    None if ids is None else ids.data_ptr(), ctypes.byref(vx), ctypes.byref(vy),
-                                    h.data_ptr(), vb, vd, ws.data_ptr(), need, MM_ACCUMULATE if accumulate else 0,
-                                    _stream(stream)), "trc_cuda_lora_back")
+    status = L.trc_cuda_lora_back(adapters.type, adapters._arr, adapters._n, None if ids is None else ids.data_ptr(), vx, vy,
+                                  ptr, vb, vd, ws.data_ptr(), need, MM_ACCUMULATE if accumulate else 0, _raw_stream(stream))
+    if status:
+        _check(status, "trc_cuda_lora_back")
     return dx
 
 
@@ -942,20 +956,20 @@ class AdamwMany:
                 e.v_scale = _check_part(v_scale[i], torch.float32, blocks, f"AdamwMany: v_scale[{i}]")
         written = [*params, *m, *v, *(m_scale or ()), *(v_scale or ())]
         _no_overlap(written, "AdamwMany")
-        self._device = params[0].device if self._n else None
+        self._device = params[0].get_device() if self._n else None
 
     def __len__(self) -> int:
         return self._n
 
     def __call__(self, params6, norm: torch.Tensor | None = None, max_norm: float = 1.0, clip_eps: float = 1e-6,
                  stream=None) -> None:
-        if self._device is not None and self._device.index != torch.cuda.current_device():
-            raise TrcCudaError(f"AdamwMany: the tensors are on {self._device}, which is not the current device")
-        ptr = None
-        if norm is not None:
-            ptr = _check_part(norm, torch.float32, 1, "AdamwMany: norm")
-        _check(lib().trc_cuda_opt_step_adamw_many(self._arr, self._n, self._bits, _params6(params6), ptr, max_norm,
-                                                  clip_eps, _stream(stream)), "trc_cuda_opt_step_adamw_many")
+        if self._device is not None and self._device != torch.cuda.current_device():
+            raise TrcCudaError(f"AdamwMany: the tensors are on cuda:{self._device}, which is not the current device")
+        ptr = None if norm is None else _check_part(norm, torch.float32, 1, "AdamwMany: norm")
+        status = lib().trc_cuda_opt_step_adamw_many(self._arr, self._n, self._bits, _params6(params6), ptr, max_norm, clip_eps,
+                                                    _raw_stream(stream))
+        if status:
+            _check(status, "trc_cuda_opt_step_adamw_many")
 
 
 class SumSqrMany:
@@ -968,19 +982,21 @@ class SumSqrMany:
             self._arr[i].data = _check_part(t, torch.float32, t.numel(), f"SumSqrMany: tensor {i}")
             self._arr[i].n = t.numel()
         self._bytes = int(lib().trc_cuda_sum_sqr_many_workspace_bytes(self._arr, self._n))
+        self._device = tensors[0].device if self._n else torch.device("cuda", torch.cuda.current_device())
 
     def __len__(self) -> int:
         return self._n
 
     def __call__(self, out: torch.Tensor | None = None, stream=None) -> torch.Tensor:
-        device = self._keep[0].device if self._n else torch.device("cuda", torch.cuda.current_device())
-        if device.index != torch.cuda.current_device():
-            raise TrcCudaError(f"SumSqrMany: the tensors are on {device}, which is not the current device")
+        if self._device.index != torch.cuda.current_device():
+            raise TrcCudaError(f"SumSqrMany: the tensors are on {self._device}, which is not the current device")
         if out is None:
-            out = _scratch(1, torch.float32, device, stream)
-        ws = _scratch(self._bytes, torch.uint8, device, stream)
-        _check(lib().trc_cuda_sum_sqr_many(self._arr, self._n, _check_part(out, torch.float32, 1, "SumSqrMany: out"),
-                                           ws.data_ptr(), self._bytes, _stream(stream)), "trc_cuda_sum_sqr_many")
+            out = _scratch(1, torch.float32, self._device, stream)
+        ptr = _check_part(out, torch.float32, 1, "SumSqrMany: out")
+        ws = _scratch(self._bytes, torch.uint8, self._device, stream)
+        status = lib().trc_cuda_sum_sqr_many(self._arr, self._n, ptr, ws.data_ptr(), self._bytes, _raw_stream(stream))
+        if status:
+            _check(status, "trc_cuda_sum_sqr_many")
         return out
 
 
