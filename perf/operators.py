@@ -25,13 +25,20 @@ BLOCK = 256  # elements that share a scale in an 8-bit state
 UNIT_M, UNIT_V = float(np.float32(1 / 127 ** 2)), float(np.float32(1 / 255 ** 2))
 
 
-def _tc():
-    pkg = str(Path(__file__).resolve().parent.parent / "train.cpp_b200")
-    if pkg not in sys.path:
-        sys.path.insert(0, pkg)
-    import trc_cuda
+_module = None
 
-    return trc_cuda
+
+def _tc():
+    """The framework's Python module, imported once."""
+    global _module
+    if _module is None:
+        pkg = str(Path(__file__).resolve().parent.parent / "train.cpp_b200")
+        if pkg not in sys.path:
+            sys.path.insert(0, pkg)
+        import trc_cuda
+
+        _module = trc_cuda
+    return _module
 
 
 # ------------------------------------------------------------------ the cases
