@@ -649,20 +649,25 @@ __global__ void __launch_bounds__(kThreads, UpRing<W, BACK, JG>::kCtas) up_kerne
 // @@, one row of one adapter (rank 16, 4096 -> 4096, f16) @@.
 constexpr int kFewRows = 256, kFewCtas = 8;
 
+// Two CTAs fit an SM (registers and shared memory). With more than 16 ranks two groups of warps take half of them each in the
+// first product.
 template <typename W, int NT>
 struct FewRing {
-    static constexpr int kDownX = 4 * 512, kDownW = 2 * NT * 32 * 4 * static_cast<int>(sizeof(W));
+    static constexpr int kGroups = NT == 2 ? 1 : 2, kTiles = NT / kGroups;  // of ranks: 8-rank tiles of a warp
+    static constexpr int kKWarps = kWarps / kGroups;                        // warps that share the columns of x
+    static constexpr int kDownX = 4 * 512, kDownW = 2 * kTiles * 32 * 4 * static_cast<int>(sizeof(W));
     static constexpr int kUpX = 2 * 512, kUpW = NT * 32 * 4 * static_cast<int>(sizeof(W));
     static constexpr int kStage = kDownX + kDownW, kStages = 2;
-    static constexpr int kUpStages = 2 * kStage / (kUpX + kUpW) >= 4 ? 4 : 2 * kStage / (kUpX + kUpW);
+    static constexpr int kFit = 2 * kStage / (kUpX + kUpW), kUpStages = kFit >= 4 ? 4 : kFit;
     static constexpr int kWarp = kStages * kStage;
-    static constexpr int kPart = 16 * 8 * NT;  // floats of one warp's partial sums
-    static constexpr int kBytes = kWarps * kWarp + (kWarps + 1) * kPart * 4;
+    static constexpr int kPart = 16 * 8 * NT;  // floats of one set of partial sums
+    static constexpr int kBytes = kWarps * kWarp + kKWarps * kPart * 4;
+    static_assert(kUpStages >= 2 && kBytes <= 112 * 1024, "two CTAs on an SM");
 };
 
 template <typename W, int NT, bool VEC>
-__global__ void __launch_bounds__(kThreads) few_kernel(const __grid_constant__ Adapters tab, const int32_t* ids, Rows x, Rows base,
-                                                       Rows d, int rows, int k_len, int n_len, float* h, int ld) {
+__global__ void __launch_bounds__(kThreads, 2) few_kernel(const __grid_constant__ Adapters tab, const int32_t* ids, Rows x, Rows base,
+                                                       Rows d, int rows, int k_len, int n_len, float* h, int ld, int share) {
     constexpr bool HALF = sizeof(W) == 2;
     using Ring = FewRing<W, NT>;
     constexpr int JG = NT / 2, kCols = 8 * NT, kPiece = 4 * static_cast<int>(sizeof(W));
@@ -672,10 +677,15 @@ __global__ void __launch_bounds__(kThreads) few_kernel(const __grid_constant__ A
     const int      warp = threadIdx.x >> 5, lane = threadIdx.x & 31, c = lane >> 2, q = lane & 3;
     const uint32_t ring = smem_u32(few_smem) + warp * Ring::kWarp;
     float* part = reinterpret_cast<float*>(few_smem + kWarps * Ring::kWarp);
-    float* hs = part + kWarps * Ring::kPart;
+    float* hs = part + Ring::kPart;  // the second set's place, once the first holds their sum
+    constexpr int TN = Ring::kTiles;
+    const int kwarp = warp % Ring::kKWarps, tile0 = warp / Ring::kKWarps * TN;  // this warp's ranks: 8 tile0 ..
     const int rank = static_cast<int>(cluster_ctarank());
     const int a = static_cast<int>(blockIdx.y);
     const bool none = a == tab.n;
+    // clusters of this adapter: `share` for each 16 of its ranks
+    const int clusters = min(static_cast<int>(gridDim.x) / kFewCtas, none ? 1 : share * ((tab.ad[a].rank + 15) / 16));
+    if (static_cast<int>(blockIdx.x) >= clusters * kFewCtas) return;
 
     // this adapter's rows, in their order
     int total = 0;
@@ -697,14 +707,14 @@ __global__ void __launch_bounds__(kThreads) few_kernel(const __grid_constant__ A
     }
     if (total == 0) return;  // the whole cluster
 
-    const int first = 16 * (static_cast<int>(blockIdx.x) * kWarps + warp), stride = 16 * kWarps * static_cast<int>(gridDim.x);
+    const int first = 16 * (static_cast<int>(blockIdx.x) * kWarps + warp), stride = 16 * kWarps * kFewCtas * clusters;
     if (none) {
         for (int i = 0; i < total; ++i) {
             const int64_t t = list[i];
             if (h != nullptr && blockIdx.x == 0)
                 for (int j = threadIdx.x; j < ld; j += kThreads) h[t * ld + j] = 0.0f;
             if (base.data == d.data) continue;
-            for (int n = blockIdx.x * kThreads + threadIdx.x; n < n_len; n += kThreads * gridDim.x)
+            for (int n = blockIdx.x * kThreads + threadIdx.x; n < n_len; n += kThreads * kFewCtas)
                 *reinterpret_cast<float*>(d.row<false>(t) + n * d.nb0) =
                     base.data != nullptr ? *reinterpret_cast<const float*>(base.row<false>(t) + n * base.nb0) : 0.0f;
         }
@@ -725,76 +735,87 @@ __global__ void __launch_bounds__(kThreads) few_kernel(const __grid_constant__ A
             t[i] = live[i] ? list[at + c + 8 * i] : 0;
         }
         // h: this warp's steps of 32 columns
-        float acc[NT][4] = {};
+        float acc[TN][4] = {};
         const char* xr[2] = {x.row<VEC>(t[0]), x.row<VEC>(t[1])};
-        const int   step = 32 * kWarps * kFewCtas;
+        const int   step = 32 * Ring::kKWarps * kFewCtas;
+        const W*    wa_lane = wa + (static_cast<int64_t>(8 * tile0 + c) * k_len + 4 * q);
         auto fetch = [&](int k, int stage) {
             const uint32_t place = ring + stage * Ring::kStage;
+            const W* p = wa_lane + k;
+            if (whole_a)
 #pragma unroll
-            for (int s = 0; s < 2; ++s) {
-                const int kg = k + 16 * s + 4 * q;
-                if (whole_a)
+                for (int n = 0; n < TN; ++n) {
+                    const bool some = 8 * (tile0 + n) + c < r;
 #pragma unroll
-                    for (int n = 0; n < NT; ++n)
-                        ring_w<kPiece>(place + Ring::kDownX + ((s * NT + n) * 32 + lane) * kPiece,
-                                       wa + static_cast<int64_t>(8 * n + c) * k_len + kg, 8 * n + c < r && kg < k_len);
+                    for (int s = 0; s < 2; ++s)
+                        ring_w<kPiece>(place + Ring::kDownX + ((s * TN + n) * 32 + lane) * kPiece, p + 16 * s,
+                                       some && k + 16 * s + 4 * q < k_len);
+                    p += 8ll * k_len;
+                }
+#pragma unroll
+            for (int s = 0; s < 2; ++s)
 #pragma unroll
                 for (int i = 0; i < 2; ++i)
-                    ring_x4<VEC>(place + (2 * s + i) * 512 + lane * 16, xr[i], live[i], x.nb0, kg, k_len);
-            }
+                    ring_x4<VEC>(place + (2 * s + i) * 512 + lane * 16, xr[i], live[i], x.nb0, k + 16 * s + 4 * q, k_len);
             ring_commit();
         };
-        int k0 = 32 * (rank * kWarps + warp), stage = 0;
-        fetch(k0, 0);
-        for (; k0 < k_len; k0 += step, stage ^= 1) {
-            fetch(k0 + step, stage ^ 1);
-            ring_wait<1>();
-            const uint32_t place = ring + stage * Ring::kStage;
-            float dsum[NT][4] = {};
+        if (8 * tile0 < r) {
+            int k0 = 32 * (rank * Ring::kKWarps + kwarp), stage = 0;
+            fetch(k0, 0);
+            for (; k0 < k_len; k0 += step, stage ^= 1) {
+                fetch(k0 + step, stage ^ 1);
+                ring_wait<1>();
+                const uint32_t place = ring + stage * Ring::kStage;
+                float dsum[TN][4] = {};
 #pragma unroll
-            for (int s = 0; s < 2; ++s) {
-                uint32_t ah[2][4], at_[2][4];
+                for (int s = 0; s < 2; ++s) {
+                    uint32_t ah[2][4], at_[2][4];
 #pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    float xv[4];
-                    ring_take(place + (2 * s + i) * 512 + lane * 16, xv);
+                    for (int i = 0; i < 2; ++i) {
+                        float xv[4];
+                        ring_take(place + (2 * s + i) * 512 + lane * 16, xv);
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) split(xv[e], ah[e >> 1][i + 2 * (e & 1)], at_[e >> 1][i + 2 * (e & 1)]);
+                        for (int e = 0; e < 4; ++e) split(xv[e], ah[e >> 1][i + 2 * (e & 1)], at_[e >> 1][i + 2 * (e & 1)]);
+                    }
+#pragma unroll
+                    for (int n = 0; n < TN; ++n) {
+                        if (NT > 2 && 8 * (tile0 + n) >= r) continue;
+                        const int kg = k0 + 16 * s + 4 * q, j = 8 * (tile0 + n) + c;
+                        float wv[4];
+                        if (whole_a) ring_take_w<W, 4>(place + Ring::kDownX + ((s * TN + n) * 32 + lane) * kPiece, wv);
+                        else load_w<W, 4, false>(wa + static_cast<int64_t>(j) * k_len + kg, j < r ? k_len - kg : 0, wv);
+                        uint32_t bh[2][2], bt[2][2];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) split_b<HALF>(wv[e], bh[e >> 1][e & 1], bt[e >> 1][e & 1]);
+                        mma_split<HALF>(dsum[n], ah[0], at_[0], bh[0], bt[0]);
+                        mma_split<HALF>(dsum[n], ah[1], at_[1], bh[1], bt[1]);
+                    }
                 }
 #pragma unroll
-                for (int n = 0; n < NT; ++n) {
-                    if (NT > 2 && 8 * n >= r) continue;
-                    const int kg = k0 + 16 * s + 4 * q, j = 8 * n + c;
-                    float wv[4];
-                    if (whole_a) ring_take_w<W, 4>(place + Ring::kDownX + ((s * NT + n) * 32 + lane) * kPiece, wv);
-                    else load_w<W, 4, false>(wa + static_cast<int64_t>(j) * k_len + kg, j < r ? k_len - kg : 0, wv);
-                    uint32_t bh[2][2], bt[2][2];
+                for (int n = 0; n < TN; ++n)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) split_b<HALF>(wv[e], bh[e >> 1][e & 1], bt[e >> 1][e & 1]);
-                    mma_split<HALF>(dsum[n], ah[0], at_[0], bh[0], bt[0]);
-                    mma_split<HALF>(dsum[n], ah[1], at_[1], bh[1], bt[1]);
-                }
+                    for (int e = 0; e < 4; ++e) acc[n][e] += dsum[n][e];
             }
-#pragma unroll
-            for (int n = 0; n < NT; ++n)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) acc[n][e] += dsum[n][e];
+            ring_wait<0>();
         }
-        ring_wait<0>();
         // the first groups of columns set out
         const char* in[2] = {add ? base.row<VEC>(t[0]) : nullptr, add ? base.row<VEC>(t[1]) : nullptr};
         char*       out[2] = {d.row<VEC>(t[0]), d.row<VEC>(t[1])};
+        const int n_lane = 4 * (c >> 1) + (c & 1);
+        const W*  wb_lane = wb + (static_cast<int64_t>(n_lane) * r + 4 * q);
         auto fetch_up = [&](int n0, int st) {
             const uint32_t place = ring + st * (Ring::kUpX + Ring::kUpW);
             if (whole_b)
 #pragma unroll
-                for (int g = 0; g < JG; ++g)
+                for (int i = 0; i < 2; ++i) {
+                    const W* p = wb_lane + static_cast<int64_t>(n0 + 2 * i) * r;
+                    const bool some = n0 + n_lane + 2 * i < n_len;
 #pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        const int n = n0 + 4 * (c >> 1) + (c & 1) + 2 * i, jq = 16 * g + 4 * q;
-                        ring_w<kPiece>(place + Ring::kUpX + ((g * 2 + i) * 32 + lane) * kPiece, wb + (static_cast<int64_t>(n) * r + jq),
-                                       n < n_len && jq < r);
+                    for (int g = 0; g < JG; ++g) {
+                        if (JG > 1 && 16 * g >= r) break;
+                        ring_w<kPiece>(place + Ring::kUpX + ((g * 2 + i) * 32 + lane) * kPiece, p + 16 * g, some && 16 * g + 4 * q < r);
                     }
+                }
             if (add)
 #pragma unroll
                 for (int i = 0; i < 2; ++i)
@@ -805,15 +826,15 @@ __global__ void __launch_bounds__(kThreads) few_kernel(const __grid_constant__ A
         for (int p = 0; p < Ring::kUpStages - 1; ++p) fetch_up(first + p * stride, p);
         // partial sums: of the CTA's warps, then of the cluster's CTAs
 #pragma unroll
-        for (int n = 0; n < NT; ++n)
+        for (int n = 0; n < TN; ++n)
 #pragma unroll
             for (int e = 0; e < 4; ++e)
-                part[warp * Ring::kPart + (c + 8 * (e >> 1)) * kCols + 8 * n + 2 * q + (e & 1)] = acc[n][e];
+                part[kwarp * Ring::kPart + (c + 8 * (e >> 1)) * kCols + 8 * (tile0 + n) + 2 * q + (e & 1)] = acc[n][e];
         __syncthreads();
         for (int i = threadIdx.x; i < Ring::kPart; i += kThreads) {
             float s = part[i];
 #pragma unroll
-            for (int v = 1; v < kWarps; ++v) s += part[v * Ring::kPart + i];
+            for (int v = 1; v < Ring::kKWarps; ++v) s += part[v * Ring::kPart + i];
             part[i] = s;
         }
         cluster_sync();
@@ -827,6 +848,17 @@ __global__ void __launch_bounds__(kThreads) few_kernel(const __grid_constant__ A
                 h[static_cast<int64_t>(list[at + i / kCols]) * ld + i % kCols] = s;
         }
         cluster_sync();  // every CTA has read the partial sums, and this one's h is complete
+        uint32_t hh[JG][2][4], ht[JG][2][4];
+#pragma unroll
+        for (int g = 0; g < JG; ++g)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const float4 v = *reinterpret_cast<const float4*>(hs + (c + 8 * i) * kCols + 16 * g + 4 * q);
+                split(v.x, hh[g][0][i], ht[g][0][i]);
+                split(v.y, hh[g][0][i + 2], ht[g][0][i + 2]);
+                split(v.z, hh[g][1][i], ht[g][1][i]);
+                split(v.w, hh[g][1][i + 2], ht[g][1][i + 2]);
+            }
         for (int n0 = first, st = 0; n0 < n_len; n0 += stride, st = st + 1 == Ring::kUpStages ? 0 : st + 1) {
             fetch_up(n0 + (Ring::kUpStages - 1) * stride, st == 0 ? Ring::kUpStages - 1 : st - 1);
             ring_wait<Ring::kUpStages - 1>();
@@ -835,15 +867,6 @@ __global__ void __launch_bounds__(kThreads) few_kernel(const __grid_constant__ A
 #pragma unroll
             for (int g = 0; g < JG; ++g) {
                 if (JG > 1 && 16 * g >= r) continue;
-                uint32_t ah[2][4], at_[2][4];
-#pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    const float4 hv = *reinterpret_cast<const float4*>(hs + (c + 8 * i) * kCols + 16 * g + 4 * q);
-                    split(hv.x, ah[0][i], at_[0][i]);
-                    split(hv.y, ah[0][i + 2], at_[0][i + 2]);
-                    split(hv.z, ah[1][i], at_[1][i]);
-                    split(hv.w, ah[1][i + 2], at_[1][i + 2]);
-                }
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
                     const int n = n0 + 4 * (c >> 1) + (c & 1) + 2 * i, jq = 16 * g + 4 * q;
@@ -853,8 +876,8 @@ __global__ void __launch_bounds__(kThreads) few_kernel(const __grid_constant__ A
                     uint32_t bh[2][2], bt[2][2];
 #pragma unroll
                     for (int e = 0; e < 4; ++e) split_b<HALF>(wv[e], bh[e >> 1][e & 1], bt[e >> 1][e & 1]);
-                    mma_split<HALF>(y[i], ah[0], at_[0], bh[0], bt[0]);
-                    mma_split<HALF>(y[i], ah[1], at_[1], bh[1], bt[1]);
+                    mma_split<HALF>(y[i], hh[g][0], ht[g][0], bh[0], bt[0]);
+                    mma_split<HALF>(y[i], hh[g][1], ht[g][1], bh[1], bt[1]);
                 }
             }
 #pragma unroll
@@ -1244,10 +1267,16 @@ int run_few(const Adapters& tab, const int32_t* ids, const Rows& x, const Rows& 
     const size_t smem = FewRing<W, NT>::kBytes;
     const int st = allow_smem(kernel, smem);
     if (st != TRC_CUDA_OK) return st;
-    // parts of the columns: one CTA for each SM as long as a part has a group of 16 for every warp
-    const int64_t groups = (n + 15) / 16, present = std::max(1, std::min(tab.n, rows));
-    const int64_t parts = std::max<int64_t>(1, std::min(full_grid() / 2 / (present * kFewCtas), groups / (kFewCtas * kWarps)));
-    void* args[] = {const_cast<Adapters*>(&tab), &ids, const_cast<Rows*>(&x), const_cast<Rows*>(&base), const_cast<Rows*>(&d), &rows, &k, &n, &h, &ld};
+    // Every 16 ranks of an adapter get `share` clusters, so that adapters of all ranks take about the same time; together
+    // they fill the SMs if every adapter occurs, as long as each warp has a group of 16 columns.
+    int64_t units = 0;
+    for (int i = 0; i < tab.n; ++i) units += (tab.ad[i].rank + 15) / 16;
+    units = std::max<int64_t>(1, std::min<int64_t>(units, static_cast<int64_t>(rows) * (ld / 16)));
+    const int64_t most = std::max<int64_t>(1, (n + 16 * kFewCtas * kWarps - 1) / (16 * kFewCtas * kWarps));
+    int share = static_cast<int>(std::max<int64_t>(1, full_grid() / (units * kFewCtas)));
+    const int64_t parts = std::min<int64_t>(most, static_cast<int64_t>(share) * (ld / 16));
+    void* args[] = {const_cast<Adapters*>(&tab), &ids, const_cast<Rows*>(&x), const_cast<Rows*>(&base), const_cast<Rows*>(&d), &rows, &k, &n, &h, &ld,
+                    &share};
     return launch(kernel, dim3(static_cast<unsigned>(parts * kFewCtas), static_cast<unsigned>(tab.n + 1)), kFewCtas, smem, false, args, s);
 }
 
