@@ -428,7 +428,8 @@ typedef struct trc_cuda_adamw_job {
 
 /* AdamW over n_jobs tensors (HOST array). params6 as for trc_cuda_opt_step_adamw; state_bits is 32
  * (each element bit for bit what trc_cuda_opt_step_adamw gives) or 8 (the same step from the decoded
- * states, in fp32; the new states are rounded to their codes after the parameter took its step).
+ * states: the new moments in the same fp32 operations, the parameter's step within 5 * 2^-23 of itself;
+ * the new states are rounded to their codes after the parameter took its step).
  * norm (one float, device; may be null): the gradients are first multiplied by
  * min(1, max_norm / (sqrt(norm[0]) + clip_eps)) as trc_cuda_clip_scale_inplace does; grad itself is left as it
  * is. Two jobs may not share memory, except that gradients may be shared. */

@@ -5,8 +5,13 @@
 // per tensor costs more than its work. Here the tensors of a call are a table in the kernel's parameters,
 // cut into runs of 2048 elements; one CTA takes one run.
 //
-// Every fp32 operation is rounded by itself, in the order of train_ops.cu's adamw_kernel, so the 32-bit
-// form is bit-exact with the one-tensor step and the 8-bit form is the same on every machine.
+// 32-bit states: every fp32 operation is rounded by itself, in the order of train_ops.cu's adamw_kernel, so the
+// step is bit-exact with the one-tensor step. 28 bytes for each element leave room for its two divisions and square
+// root.
+// 8-bit states: 16 bytes for each element leave about 60 instructions. The new moments and their codes are still
+// those of separately rounded operations; only the parameter's own step takes the approximate quotient and square
+// root (5 * 2^-23 of the step at most). A code is round(sqrt(x * per)): the approximate square root (2^-23)
+// decides it except within 2^-11 of a border, where the rounded one does.
 #include <cuda_runtime.h>
 
 #include <algorithm>
@@ -129,6 +134,20 @@ __device__ __forceinline__ float block_max(const float (&x)[8]) {
     return __all_sync(0xFFFFFFFFu, fine) ? top : __int_as_float(0x7FC00000);
 }
 
+__device__ __forceinline__ float sqrt_approx(float x) {  // relative error 2^-23
+    float r;
+    asm("sqrt.approx.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+
+// The approximate root `a` of a code (at most 255.001, error below 255 * 4 * 2^-23 < 2^-13) as a whole number;
+// near: it is too close to a border to tell, and the rounded operations have to decide.
+__device__ __forceinline__ int code_of(float a, bool& near) {
+    const float c = rintf(a);
+    near = near || fabsf(fabsf(a - c) - 0.5f) < 0x1p-11f;
+    return static_cast<int>(c);
+}
+
 // One block's new codes from the warp's 8 values per lane (a lane's values 0-3 in w[0], 4-7 in
 // w[1]); returns the scale.
 __device__ __forceinline__ float encode_m(const float (&m)[8], uint32_t (&w)[2]) {
@@ -139,26 +158,36 @@ __device__ __forceinline__ float encode_m(const float (&m)[8], uint32_t (&w)[2])
     if (top < kTinyM) top = 0.0f;
     const float per = top > 0.0f ? __fdiv_rn(16129.0f, top) : 0.0f;  // 0 for NaN too
     w[0] = w[1] = 0;
+    if (per > 0.0f) {
+        int  c[8];
+        bool near = false;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-        const int c = per > 0.0f ? __float2int_rn(__fsqrt_rn(__fmul_rn(x[e], per))) : 0;
-        w[e >> 2] |= static_cast<uint32_t>((m[e] < 0.0f ? -c : c) & 0xFF) << (8 * (e & 3));
+        for (int e = 0; e < 8; ++e) c[e] = code_of(sqrt_approx(__fmul_rn(x[e], per)), near);
+        if (near)
+            for (int e = 0; e < 8; ++e) c[e] = __float2int_rn(__fsqrt_rn(__fmul_rn(x[e], per)));
+#pragma unroll
+        for (int e = 0; e < 8; ++e) w[e >> 2] |= static_cast<uint32_t>((m[e] < 0.0f ? -c[e] : c[e]) & 0xFF) << (8 * (e & 3));
     }
     return __fmul_rn(top, kUnitM);
 }
 
+// The largest root is the root of the largest value: rounding keeps the order. A negative v counts as NaN.
 __device__ __forceinline__ float encode_v(const float (&v)[8], uint32_t (&w)[2]) {
-    float u[8];
+    float x[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) u[e] = __fsqrt_rn(v[e]);  // NaN for a negative v
-    const float top = block_max(u);
+    for (int e = 0; e < 8; ++e) x[e] = v[e] < 0.0f ? __int_as_float(0x7FC00000) : v[e];
+    const float top = __fsqrt_rn(block_max(x));
     const float per = top > 0.0f ? __fdiv_rn(65025.0f, top) : 0.0f;
     w[0] = w[1] = 0;
+    if (per > 0.0f) {
+        int  c[8];
+        bool near = false;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-        int c = per > 0.0f ? __float2int_rn(__fsqrt_rn(__fmul_rn(u[e], per))) : 0;
-        if (per > 0.0f && u[e] > 0.0f) c = max(c, 1);
-        w[e >> 2] |= static_cast<uint32_t>(c) << (8 * (e & 3));
+        for (int e = 0; e < 8; ++e) c[e] = code_of(sqrt_approx(__fmul_rn(sqrt_approx(x[e]), per)), near);
+        if (near)
+            for (int e = 0; e < 8; ++e) c[e] = __float2int_rn(__fsqrt_rn(__fmul_rn(__fsqrt_rn(x[e]), per)));
+#pragma unroll
+        for (int e = 0; e < 8; ++e) w[e >> 2] |= static_cast<uint32_t>(x[e] > 0.0f ? max(c[e], 1) : 0) << (8 * (e & 3));
     }
     return __fmul_rn(top, kUnitV);
 }
@@ -170,6 +199,16 @@ __device__ __forceinline__ void adamw_one(float& p, float g, float& m, float& v,
     v = __fadd_rn(__fmul_rn(v, a.beta2), __fmul_rn(__fmul_rn(g, g), one_b2));
     const float denom = __fadd_rn(__fdiv_rn(__fsqrt_rn(v), a.bc2_sqrt), a.eps);
     p = __fsub_rn(__fmul_rn(p, a.decay), __fmul_rn(a.step_sz, __fdiv_rn(m, denom)));
+}
+
+// The same with 8-bit states: m and v as above, the parameter's step with approximate operations (inv_bc2 is
+// 1 / bc2_sqrt rounded; the quotient is within 2 units, the root and the two products within one: 5 * 2^-23).
+__device__ __forceinline__ void adamw_one_8(float& p, float g, float& m, float& v, const AdamwParams& a, float one_b1,
+                                            float one_b2, float inv_bc2) {
+    m = __fadd_rn(m, __fmul_rn(__fsub_rn(g, m), one_b1));
+    v = __fadd_rn(__fmul_rn(v, a.beta2), __fmul_rn(__fmul_rn(g, g), one_b2));
+    const float denom = fmaf(sqrt_approx(v), inv_bc2, a.eps);
+    p = __fsub_rn(__fmul_rn(p, a.decay), __fmul_rn(a.step_sz, __fdividef(m, denom)));
 }
 
 template <int BITS>
@@ -185,6 +224,7 @@ __global__ void __launch_bounds__(kThreads) adamw_many_kernel(const __grid_const
     if (b0 * kBlock >= n) return;
     const bool  whole = J.aligned != 0;
     const float one_b1 = __fsub_rn(1.0f, a.beta1), one_b2 = __fsub_rn(1.0f, a.beta2);
+    [[maybe_unused]] const float inv_bc2 = __fdiv_rn(1.0f, a.bc2_sqrt);
     float clip = 1.0f;
     if (batch.norm != nullptr) {  // clip_scale_kernel's factor
         clip = __fdiv_rn(a.max_norm, __fadd_rn(__fsqrt_rn(batch.norm[0]), a.clip_eps));
@@ -220,7 +260,8 @@ __global__ void __launch_bounds__(kThreads) adamw_many_kernel(const __grid_const
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             const float ge = batch.norm != nullptr ? __fmul_rn(g[h][e], clip) : g[h][e];
-            adamw_one(p[h][e], ge, m[4 * h + e], v[4 * h + e], a, one_b1, one_b2);
+            if constexpr (BITS == 32) adamw_one(p[h][e], ge, m[4 * h + e], v[4 * h + e], a, one_b1, one_b2);
+            else adamw_one_8(p[h][e], ge, m[4 * h + e], v[4 * h + e], a, one_b1, one_b2, inv_bc2);
         }
 #pragma unroll
     for (int h = 0; h < 2; ++h) store4(J.p, i0 + 128 * h, n, whole, p[h]);
@@ -250,22 +291,31 @@ __global__ void __launch_bounds__(kThreads) adamw_many_kernel(const __grid_const
 }
 
 // ------------------------------------------------------------------ 8-bit states <-> values
-// One warp per block of 256.
+// To values: a warp takes four blocks of 256 (one left 22 % more time at 202 M elements), back: one.
+constexpr int kToF32 = 4;
+
 template <int WHICH>
 __global__ void __launch_bounds__(kThreads) state8_to_f32_kernel(const uint8_t* codes, const float* scales, float* values,
                                                                  int64_t n, bool whole) {
-    const int64_t b = static_cast<int64_t>(blockIdx.x) * (kThreads / 32) + (threadIdx.x >> 5);
+    const int64_t b = (static_cast<int64_t>(blockIdx.x) * (kThreads / 32) + (threadIdx.x >> 5)) * kToF32;
     const int64_t i0 = b * kBlock + (threadIdx.x & 31) * 4;
-    if (b * kBlock >= n) return;
-    const float s = scales[b];
+    uint32_t w[kToF32][2];
+    float    s[kToF32];
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-        const uint32_t w = load4c(codes, i0 + 128 * h, n, whole);
-        float x[4];
+    for (int k = 0; k < kToF32; ++k) {
+        s[k] = (b + k) * kBlock < n ? scales[b + k] : 0.0f;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) x[e] = WHICH == 0 ? decode_m(w, e, s) : decode_v(w, e, s);
-        store4(values, i0 + 128 * h, n, whole, x);
+        for (int h = 0; h < 2; ++h) w[k][h] = load4c(codes, i0 + kBlock * k + 128 * h, n, whole);
     }
+#pragma unroll
+    for (int k = 0; k < kToF32; ++k)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            float x[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[e] = WHICH == 0 ? decode_m(w[k][h], e, s[k]) : decode_v(w[k][h], e, s[k]);
+            store4(values, i0 + kBlock * k + 128 * h, n, whole, x);
+        }
 }
 
 template <int WHICH>
@@ -319,17 +369,21 @@ __global__ void __launch_bounds__(kThreads) sum_sqr_many_kernel(const __grid_con
     const int     run = static_cast<int>(blockIdx.x);
     const Span&   J   = batch.job[job_of(batch.job, batch.n_jobs, run)];
     const int64_t lo = static_cast<int64_t>(run - J.run_begin) * kChunk, hi = min(J.n, lo + kChunk);
-    double s = 0.0;
-#pragma unroll 4
-    for (int64_t i = lo + threadIdx.x * 4; i < hi; i += kThreads * 4) {
-        float x[4];
-        load4(J.a, i, hi, J.aligned != 0, x);
+    // 8 loads on their way at a time, four sums of their own
+    double part[4] = {};
+    for (int64_t i = lo + threadIdx.x * 4; i < hi; i += kThreads * 32) {
+        float x[8][4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const double d = static_cast<double>(x[e]);
-            s = fma(d, d, s);
-        }
+        for (int u = 0; u < 8; ++u) load4(J.a, i + kThreads * 4 * u, hi, J.aligned != 0, x[u]);
+#pragma unroll
+        for (int u = 0; u < 8; ++u)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const double d = static_cast<double>(x[u][e]);
+                part[e] = fma(d, d, part[e]);
+            }
     }
+    double s = __dadd_rn(__dadd_rn(part[0], part[1]), __dadd_rn(part[2], part[3]));
     s = block_sum(s);
     if (threadIdx.x == 0) batch.partials[run] = s;
 }
@@ -426,7 +480,7 @@ int trc_cuda_state8_to_f32(int which, const void* codes, const float* scales, fl
     if (n == 0) return TRC_CUDA_OK;
     if (codes == nullptr || scales == nullptr || values == nullptr || !aligned_to(scales, 4) || !aligned_to(values, 4))
         return TRC_CUDA_EINVAL;
-    const unsigned grid = static_cast<unsigned>((n + kRun - 1) / kRun);
+    const unsigned grid = static_cast<unsigned>((n + kRun * kToF32 - 1) / (kRun * kToF32));
     const bool whole = aligned_to(codes, 4) && aligned_to(values, 16);
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     const uint8_t* c = static_cast<const uint8_t*>(codes);
