@@ -3,7 +3,7 @@
 //
 // A low-rank adapter gives two small tensors for every projection, hundreds for a model, so one launch
 // per tensor costs more than its work. Here the tensors of a call are a table in the kernel's parameters,
-// cut into runs of 2048 elements; one CTA takes one run.
+// cut into runs of 2048 - 8192 elements; one CTA takes one run.
 //
 // 32-bit states: every fp32 operation is rounded by itself, in the order of train_ops.cu's adamw_kernel, so the
 // step is bit-exact with the one-tensor step. 28 bytes for each element leave room for its two divisions and square
@@ -11,7 +11,9 @@
 // 8-bit states: 16 bytes for each element leave about 60 instructions. The new moments and their codes are still
 // those of separately rounded operations; only the parameter's own step takes the approximate quotient and square
 // root (5 * 2^-23 of the step at most). A code is round(sqrt(x * per)): the approximate square root (2^-23)
-// decides it except within 2^-11 of a border, where the rounded one does.
+// decides it except next to a border, where the rounded one does. Codes become numbers and numbers codes through
+// the low bits of 2^23 + c, because the conversion unit is the one that the roots need (together they bound
+// the kernel: @@).
 #include <cuda_runtime.h>
 
 #include <algorithm>
@@ -24,7 +26,7 @@ namespace trc {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kRun     = 2048;  // elements of one CTA: 8 per thread, 8 blocks of an 8-bit state
+constexpr int kRun     = 2048;  // elements that a CTA takes at a time: 8 per thread, 8 blocks of an 8-bit state
 constexpr int kBlock   = TRC_CUDA_STATE8_BLOCK;
 constexpr int kMaxJobs = 480;   // tensors of one launch (31 KB of kernel parameters)
 static_assert(kRun == kThreads * 8 && kBlock == 256, "a warp takes one block of 256, 8 elements per lane");
@@ -54,6 +56,7 @@ struct StepBatch {
     const float* norm;
     AdamwParams  a;
     int32_t      n_jobs;
+    int32_t      per;  // a run is kRun * per elements
 };
 static_assert(sizeof(StepBatch) <= 32764, "kernel parameter limit");
 
@@ -110,46 +113,53 @@ __device__ __forceinline__ void store4c(uint8_t* q, int64_t i, int64_t n, bool w
     }
 }
 
+// The whole number in byte e of w, exactly: 0x4B0000cc is the float 2^23 + c.
+__device__ __forceinline__ float byte_value(uint32_t w, int e, float bias) {
+    return __fsub_rn(__uint_as_float(__byte_perm(w, 0x4B000000u, 0x7440u + e)), bias);
+}
+
 __device__ __forceinline__ float decode_m(uint32_t w, int e, float scale) {
-    const int c = static_cast<int8_t>(w >> (8 * e));
-    return __fmul_rn(static_cast<float>(c * abs(c)), scale);
+    const float c = byte_value(w ^ 0x80808080u, e, 8388608.0f + 128.0f);
+    return __fmul_rn(__fmul_rn(c, fabsf(c)), scale);  // c * |c| is exact
 }
 
 __device__ __forceinline__ float decode_v(uint32_t w, int e, float scale) {
-    const int c = static_cast<int>((w >> (8 * e)) & 0xFFu);
-    const float u = __fmul_rn(static_cast<float>(c * c), scale);
+    const float c = byte_value(w, e, 8388608.0f);
+    const float u = __fmul_rn(__fmul_rn(c, c), scale);
     return __fmul_rn(u, u);
 }
 
-// The largest of the warp's values, NaN if one of them is infinite or NaN (values are not negative).
+// The largest of the warp's values, NaN if one of them is infinite, NaN or negative: the bits of floats that are not
+// negative are in their order, and the bits of the others are larger.
 __device__ __forceinline__ float block_max(const float (&x)[8]) {
-    float top = 0.0f;
-    bool  fine = true;
+    uint32_t top = 0;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-        top  = fmaxf(top, x[e]);
-        fine = fine && x[e] <= 3.402823466e+38f;
-    }
-    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
-    return __all_sync(0xFFFFFFFFu, fine) ? top : __int_as_float(0x7FC00000);
+    for (int e = 0; e < 8; ++e) top = max(top, __float_as_uint(x[e]));
+    top = __reduce_max_sync(0xFFFFFFFFu, top);
+    return top >= 0x7F800000u ? __uint_as_float(0x7FC00000u) : __uint_as_float(top);
 }
 
-__device__ __forceinline__ float sqrt_approx(float x) {  // relative error 2^-23
+__device__ __forceinline__ float sqrt_approx(float x) {  // relative error 2^-23; 0 below 2^-126
     float r;
-    asm("sqrt.approx.f32 %0, %1;" : "=f"(r) : "f"(x));
+    asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
     return r;
 }
 
-// The approximate root `a` of a code (at most 255.001, error below 255 * 4 * 2^-23 < 2^-13) as a whole number;
-// near: it is too close to a border to tell, and the rounded operations have to decide.
-__device__ __forceinline__ int code_of(float a, bool& near) {
-    const float c = rintf(a);
-    near = near || fabsf(fabsf(a - c) - 0.5f) < 0x1p-11f;
-    return static_cast<int>(c);
+// a, 0 <= a <= 256, rounded to nearest even: the low bits of 1.5 * 2^23 + a. near: a is closer to a border than `margin`.
+__device__ __forceinline__ uint32_t code_of(float a, float margin, bool& near) {
+    const float up = __fadd_rn(a, 12582912.0f), off = __fsub_rn(a, __fsub_rn(up, 12582912.0f));
+    near = near || fabsf(off) > 0.5f - margin;
+    return __float_as_uint(up);
+}
+
+__device__ __forceinline__ uint32_t pack4(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {  // their low bytes
+    return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
 }
 
 // One block's new codes from the warp's 8 values per lane (a lane's values 0-3 in w[0], 4-7 in
-// w[1]); returns the scale.
+// w[1]); returns the scale. The margins: a root is at most 127.001 or 255.001; for m the approximate and the
+// rounded root of the same product differ by 1.5 * 2^-23 of it, below 2^-15; for v the product's own root is
+// approximate too, together 2.75 * 2^-23, below 2^-13.
 __device__ __forceinline__ float encode_m(const float (&m)[8], uint32_t (&w)[2]) {
     float x[8];
 #pragma unroll
@@ -158,36 +168,41 @@ __device__ __forceinline__ float encode_m(const float (&m)[8], uint32_t (&w)[2])
     if (top < kTinyM) top = 0.0f;
     const float per = top > 0.0f ? __fdiv_rn(16129.0f, top) : 0.0f;  // 0 for NaN too
     w[0] = w[1] = 0;
-    if (per > 0.0f) {
-        int  c[8];
-        bool near = false;
+    if (per > 0.0f) {  // the same for the whole warp
+        uint32_t c[8];
+        bool     near = false;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) c[e] = code_of(sqrt_approx(__fmul_rn(x[e], per)), near);
+        for (int e = 0; e < 8; ++e) c[e] = code_of(sqrt_approx(__fmul_rn(x[e], per)), 0x1p-15f, near);
         if (near)
-            for (int e = 0; e < 8; ++e) c[e] = __float2int_rn(__fsqrt_rn(__fmul_rn(x[e], per)));
 #pragma unroll
-        for (int e = 0; e < 8; ++e) w[e >> 2] |= static_cast<uint32_t>((m[e] < 0.0f ? -c[e] : c[e]) & 0xFF) << (8 * (e & 3));
+            for (int e = 0; e < 8; ++e) c[e] = __float2uint_rn(__fsqrt_rn(__fmul_rn(x[e], per)));
+#pragma unroll
+        for (int e = 0; e < 8; ++e) c[e] = m[e] < 0.0f ? 0u - c[e] : c[e];
+        w[0] = pack4(c[0], c[1], c[2], c[3]);
+        w[1] = pack4(c[4], c[5], c[6], c[7]);
     }
     return __fmul_rn(top, kUnitM);
 }
 
-// The largest root is the root of the largest value: rounding keeps the order. A negative v counts as NaN.
+// The largest root is the root of the largest value: rounding keeps the order. Where it is tiny, values that the
+// approximate root takes for zero may have codes of their own: below 2^-40 the rounded one decides everything
+// (above it, a v below 2^-126 has sqrt(u * per) < 0.1).
 __device__ __forceinline__ float encode_v(const float (&v)[8], uint32_t (&w)[2]) {
-    float x[8];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) x[e] = v[e] < 0.0f ? __int_as_float(0x7FC00000) : v[e];
-    const float top = __fsqrt_rn(block_max(x));
+    const float top = __fsqrt_rn(block_max(v));
     const float per = top > 0.0f ? __fdiv_rn(65025.0f, top) : 0.0f;
     w[0] = w[1] = 0;
     if (per > 0.0f) {
-        int  c[8];
-        bool near = false;
+        uint32_t c[8];
+        bool     near = top < 0x1p-40f;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) c[e] = code_of(sqrt_approx(__fmul_rn(sqrt_approx(x[e]), per)), near);
+        for (int e = 0; e < 8; ++e) c[e] = code_of(sqrt_approx(__fmul_rn(sqrt_approx(v[e]), per)), 0x1p-13f, near);
         if (near)
-            for (int e = 0; e < 8; ++e) c[e] = __float2int_rn(__fsqrt_rn(__fmul_rn(__fsqrt_rn(x[e]), per)));
 #pragma unroll
-        for (int e = 0; e < 8; ++e) w[e >> 2] |= static_cast<uint32_t>(x[e] > 0.0f ? max(c[e], 1) : 0) << (8 * (e & 3));
+            for (int e = 0; e < 8; ++e) c[e] = __float2uint_rn(__fsqrt_rn(__fmul_rn(__fsqrt_rn(v[e]), per)));
+#pragma unroll
+        for (int e = 0; e < 8; ++e) c[e] = v[e] > 0.0f ? max(c[e] & 0xFFu, 1u) : 0u;
+        w[0] = pack4(c[0], c[1], c[2], c[3]);
+        w[1] = pack4(c[4], c[5], c[6], c[7]);
     }
     return __fmul_rn(top, kUnitV);
 }
@@ -207,47 +222,36 @@ __device__ __forceinline__ void adamw_one_8(float& p, float g, float& m, float& 
                                             float one_b2, float inv_bc2) {
     m = __fadd_rn(m, __fmul_rn(__fsub_rn(g, m), one_b1));
     v = __fadd_rn(__fmul_rn(v, a.beta2), __fmul_rn(__fmul_rn(g, g), one_b2));
-    const float denom = fmaf(sqrt_approx(v), inv_bc2, a.eps);
+    float root = sqrt_approx(v);
+    if (__float_as_uint(v) - 1u < 0x007FFFFFu) root = __fsqrt_rn(v);  // 0 < v < 2^-126
+    const float denom = fmaf(root, inv_bc2, a.eps);
     p = __fsub_rn(__fmul_rn(p, a.decay), __fmul_rn(a.step_sz, __fdividef(m, denom)));
 }
 
-template <int BITS>
-__global__ void __launch_bounds__(kThreads) adamw_many_kernel(const __grid_constant__ StepBatch batch) {
-    // From the last run to the first: the norm's pass read the gradients from the first to the last, so
-    // those that are still in L2 come first.
-    const int      run = static_cast<int>(gridDim.x - 1 - blockIdx.x);
-    const StepJob& J   = batch.job[job_of(batch.job, batch.n_jobs, run)];
-    const AdamwParams& a = batch.a;
-    const int     warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int64_t b0 = static_cast<int64_t>(run - J.run_begin) * (kRun / kBlock) + warp;  // this warp's block
-    const int64_t i0 = b0 * kBlock + lane * 4, n = J.n;
-    if (b0 * kBlock >= n) return;
-    const bool  whole = J.aligned != 0;
-    const float one_b1 = __fsub_rn(1.0f, a.beta1), one_b2 = __fsub_rn(1.0f, a.beta2);
-    [[maybe_unused]] const float inv_bc2 = __fdiv_rn(1.0f, a.bc2_sqrt);
-    float clip = 1.0f;
-    if (batch.norm != nullptr) {  // clip_scale_kernel's factor
-        clip = __fdiv_rn(a.max_norm, __fadd_rn(__fsqrt_rn(batch.norm[0]), a.clip_eps));
-        if (clip > 1.0f) clip = 1.0f;
-    }
+// One block of 256 by one warp, 8 elements per lane. FULL: the block lies inside the tensor and may be loaded whole.
+template <int BITS, bool FULL>
+__device__ __forceinline__ void step_block(const StepJob& J, int64_t b0, const AdamwParams& a, bool clipped, float clip) {
+    const int     lane = threadIdx.x & 31;
+    const int64_t i0 = b0 * kBlock + lane * 4, n = FULL ? INT64_MAX : J.n;
+    const float   one_b1 = __fsub_rn(1.0f, a.beta1), one_b2 = __fsub_rn(1.0f, a.beta2);
     float p[2][4], g[2][4], m[8], v[8];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-        load4(J.p, i0 + 128 * h, n, whole, p[h]);
-        load4(J.g, i0 + 128 * h, n, whole, g[h]);
+        load4(J.p, i0 + 128 * h, n, FULL, p[h]);
+        load4(J.g, i0 + 128 * h, n, FULL, g[h]);
     }
     if constexpr (BITS == 32) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-            load4(static_cast<const float*>(J.m), i0 + 128 * h, n, whole, reinterpret_cast<float (&)[4]>(m[4 * h]));
-            load4(static_cast<const float*>(J.v), i0 + 128 * h, n, whole, reinterpret_cast<float (&)[4]>(v[4 * h]));
+            load4(static_cast<const float*>(J.m), i0 + 128 * h, n, FULL, reinterpret_cast<float (&)[4]>(m[4 * h]));
+            load4(static_cast<const float*>(J.v), i0 + 128 * h, n, FULL, reinterpret_cast<float (&)[4]>(v[4 * h]));
         }
     } else {
         const float sm = J.m_scale[b0], sv = J.v_scale[b0];
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-            const uint32_t wm = load4c(static_cast<const uint8_t*>(J.m), i0 + 128 * h, n, whole);
-            const uint32_t wv = load4c(static_cast<const uint8_t*>(J.v), i0 + 128 * h, n, whole);
+            const uint32_t wm = load4c(static_cast<const uint8_t*>(J.m), i0 + 128 * h, n, FULL);
+            const uint32_t wv = load4c(static_cast<const uint8_t*>(J.v), i0 + 128 * h, n, FULL);
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 m[4 * h + e] = decode_m(wm, e, sm);
@@ -255,38 +259,61 @@ __global__ void __launch_bounds__(kThreads) adamw_many_kernel(const __grid_const
             }
         }
     }
+    [[maybe_unused]] const float inv_bc2 = __fdiv_rn(1.0f, a.bc2_sqrt);
 #pragma unroll
     for (int h = 0; h < 2; ++h)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            const float ge = batch.norm != nullptr ? __fmul_rn(g[h][e], clip) : g[h][e];
+            const float ge = clipped ? __fmul_rn(g[h][e], clip) : g[h][e];
             if constexpr (BITS == 32) adamw_one(p[h][e], ge, m[4 * h + e], v[4 * h + e], a, one_b1, one_b2);
             else adamw_one_8(p[h][e], ge, m[4 * h + e], v[4 * h + e], a, one_b1, one_b2, inv_bc2);
         }
 #pragma unroll
-    for (int h = 0; h < 2; ++h) store4(J.p, i0 + 128 * h, n, whole, p[h]);
+    for (int h = 0; h < 2; ++h) store4(J.p, i0 + 128 * h, n, FULL, p[h]);
     if constexpr (BITS == 32) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-            store4(static_cast<float*>(J.m), i0 + 128 * h, n, whole, reinterpret_cast<float (&)[4]>(m[4 * h]));
-            store4(static_cast<float*>(J.v), i0 + 128 * h, n, whole, reinterpret_cast<float (&)[4]>(v[4 * h]));
+            store4(static_cast<float*>(J.m), i0 + 128 * h, n, FULL, reinterpret_cast<float (&)[4]>(m[4 * h]));
+            store4(static_cast<float*>(J.v), i0 + 128 * h, n, FULL, reinterpret_cast<float (&)[4]>(v[4 * h]));
         }
     } else {
-        // what lies behind the tensor's end is not part of its last block
+        if constexpr (!FULL)  // what lies behind the tensor's end is not part of its last block
 #pragma unroll
-        for (int e = 0; e < 8; ++e)
-            if (i0 + 128 * (e >> 2) + (e & 3) >= n) m[e] = v[e] = 0.0f;
+            for (int e = 0; e < 8; ++e)
+                if (i0 + 128 * (e >> 2) + (e & 3) >= n) m[e] = v[e] = 0.0f;
         uint32_t wm[2], wv[2];
         const float sm = encode_m(m, wm), sv = encode_v(v, wv);
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-            store4c(static_cast<uint8_t*>(J.m), i0 + 128 * h, n, whole, wm[h]);
-            store4c(static_cast<uint8_t*>(J.v), i0 + 128 * h, n, whole, wv[h]);
+            store4c(static_cast<uint8_t*>(J.m), i0 + 128 * h, n, FULL, wm[h]);
+            store4c(static_cast<uint8_t*>(J.v), i0 + 128 * h, n, FULL, wv[h]);
         }
         if (lane == 0) {
             J.m_scale[b0] = sm;
             J.v_scale[b0] = sv;
         }
+    }
+}
+
+template <int BITS>
+__global__ void __launch_bounds__(kThreads, 4) adamw_many_kernel(const __grid_constant__ StepBatch batch) {
+    // From the last run to the first: the norm's pass read the gradients from the first to the last, so
+    // those that are still in L2 come first.
+    const int      run = static_cast<int>(gridDim.x - 1 - blockIdx.x);
+    const StepJob& J   = batch.job[job_of(batch.job, batch.n_jobs, run)];
+    const bool     clipped = batch.norm != nullptr;
+    float clip = 1.0f;
+    if (clipped) {  // clip_scale_kernel's factor
+        clip = __fdiv_rn(batch.a.max_norm, __fadd_rn(__fsqrt_rn(batch.norm[0]), batch.a.clip_eps));
+        if (clip > 1.0f) clip = 1.0f;
+    }
+    // batch.per blocks for each warp
+    int64_t b0 = static_cast<int64_t>(run - J.run_begin) * (kRun / kBlock) * batch.per + (threadIdx.x >> 5);
+#pragma unroll 1
+    for (int k = 0; k < batch.per; ++k, b0 += kRun / kBlock) {
+        if (b0 * kBlock >= J.n) return;
+        if (J.aligned && (b0 + 1) * kBlock <= J.n) step_block<BITS, true>(J, b0, batch.a, clipped, clip);
+        else step_block<BITS, false>(J, b0, batch.a, clipped, clip);
     }
 }
 
@@ -327,6 +354,8 @@ __global__ void __launch_bounds__(kThreads) state8_from_f32_kernel(const float* 
     float x[8];
     load4(values, i0, n, whole, reinterpret_cast<float (&)[4]>(x[0]));
     load4(values, i0 + 128, n, whole, reinterpret_cast<float (&)[4]>(x[4]));
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = __fadd_rn(x[e], 0.0f);  // no -0
     uint32_t w[2];
     const float s = WHICH == 0 ? encode_m(x, w) : encode_v(x, w);
     store4c(codes, i0, n, whole, w[0]);
@@ -434,6 +463,13 @@ int trc_cuda_opt_step_adamw_many(const trc_cuda_adamw_job* jobs, int n_jobs, int
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     StepBatch batch;
     batch.norm = norm;
+    // Long runs share the search for their tensor; runs stay short where there are few: 1 - 4 blocks for each warp, as long as
+    // every SM has 8 runs (202 M elements of 8-bit state, 1 / 2 / 4 blocks: @@).
+    int64_t total = 0;
+    for (int i = 0; i < n_jobs; ++i) total += jobs[i].n;
+    const int64_t wave = 8 * static_cast<int64_t>(std::max(1, sm_count_current())) * kRun;
+    batch.per = total >= 4 * wave ? 4 : total >= 2 * wave ? 2 : 1;
+    const int64_t run_len = static_cast<int64_t>(kRun) * batch.per;
     batch.a = AdamwParams{params6[0], params6[1], params6[2], params6[3], params6[4], params6[5], max_norm, clip_eps};
     // Batches from the last tensor to the first, as the runs inside a launch.
     for (int last = n_jobs; last > 0;) {
@@ -441,7 +477,7 @@ int trc_cuda_opt_step_adamw_many(const trc_cuda_adamw_job* jobs, int n_jobs, int
         int first = last;
         batch.n_jobs = 0;
         while (first > 0 && last - first < kMaxJobs) {
-            const int64_t r = (jobs[first - 1].n + kRun - 1) / kRun;
+            const int64_t r = (jobs[first - 1].n + run_len - 1) / run_len;
             if (runs + r > INT32_MAX) break;
             runs += r;
             --first;
@@ -461,7 +497,7 @@ int trc_cuda_opt_step_adamw_many(const trc_cuda_adamw_job* jobs, int n_jobs, int
             J.run_begin = static_cast<int32_t>(runs);
             J.aligned   = aligned_to(in.param, 16) && aligned_to(in.grad, 16) && aligned_to(in.m, 4 * state_bytes) &&
                         aligned_to(in.v, 4 * state_bytes);
-            runs += (in.n + kRun - 1) / kRun;
+            runs += (in.n + run_len - 1) / run_len;
         }
         last = first;
         if (runs == 0) continue;
