@@ -145,11 +145,16 @@ __device__ __forceinline__ float sqrt_approx(float x) {  // relative error 2^-23
     return r;
 }
 
-// a, 0 <= a <= 256, rounded to nearest even: the low bits of 1.5 * 2^23 + a. near: a is closer to a border than `margin`.
-__device__ __forceinline__ uint32_t code_of(float a, float margin, bool& near) {
-    const float up = __fadd_rn(a, 12582912.0f), off = __fsub_rn(a, __fsub_rn(up, 12582912.0f));
-    near = near || fabsf(off) > 0.5f - margin;
+// a, |a| <= 256, rounded to nearest even: the low byte of 1.5 * 2^23 + a (of a two's complement number where a < 0).
+// off: how far a is from it, at most 1/2.
+__device__ __forceinline__ uint32_t code_of(float a, float& off) {
+    const float up = __fadd_rn(a, 12582912.0f);
+    off = fmaxf(off, fabsf(__fsub_rn(a, __fsub_rn(up, 12582912.0f))));
     return __float_as_uint(up);
+}
+
+__device__ __forceinline__ float with_sign(float a, float of) {
+    return __uint_as_float(__float_as_uint(a) | (__float_as_uint(of) & 0x80000000u));
 }
 
 __device__ __forceinline__ uint32_t pack4(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {  // their low bytes
@@ -157,9 +162,9 @@ __device__ __forceinline__ uint32_t pack4(uint32_t a, uint32_t b, uint32_t c, ui
 }
 
 // One block's new codes from the warp's 8 values per lane (a lane's values 0-3 in w[0], 4-7 in
-// w[1]); returns the scale. The margins: a root is at most 127.001 or 255.001; for m the approximate and the
-// rounded root of the same product differ by 1.5 * 2^-23 of it, below 2^-15; for v the product's own root is
-// approximate too, together 2.75 * 2^-23, below 2^-13.
+// w[1]); returns the scale. The borders that the rounded operations decide: a root is at most 127.001 or 255.001; for
+// m the approximate and the rounded root of the same product differ by 1.5 * 2^-23 of it, below 2^-15; for v the
+// product's own root is approximate too, together 2.75 * 2^-23, below 2^-13.
 __device__ __forceinline__ float encode_m(const float (&m)[8], uint32_t (&w)[2]) {
     float x[8];
 #pragma unroll
@@ -170,41 +175,44 @@ __device__ __forceinline__ float encode_m(const float (&m)[8], uint32_t (&w)[2])
     w[0] = w[1] = 0;
     if (per > 0.0f) {  // the same for the whole warp
         uint32_t c[8];
-        bool     near = false;
+        float    off = 0.0f;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) c[e] = code_of(sqrt_approx(__fmul_rn(x[e], per)), 0x1p-15f, near);
-        if (near)
+        for (int e = 0; e < 8; ++e) c[e] = code_of(with_sign(sqrt_approx(__fmul_rn(x[e], per)), m[e]), off);
+        if (off > 0.5f - 0x1p-15f)
 #pragma unroll
-            for (int e = 0; e < 8; ++e) c[e] = __float2uint_rn(__fsqrt_rn(__fmul_rn(x[e], per)));
-#pragma unroll
-        for (int e = 0; e < 8; ++e) c[e] = m[e] < 0.0f ? 0u - c[e] : c[e];
+            for (int e = 0; e < 8; ++e) c[e] = code_of(with_sign(__fsqrt_rn(__fmul_rn(x[e], per)), m[e]), off);
         w[0] = pack4(c[0], c[1], c[2], c[3]);
         w[1] = pack4(c[4], c[5], c[6], c[7]);
     }
     return __fmul_rn(top, kUnitM);
 }
 
-// The largest root is the root of the largest value: rounding keeps the order. Where it is tiny, values that the
-// approximate root takes for zero may have codes of their own: below 2^-40 the rounded one decides everything
-// (above it, a v below 2^-126 has sqrt(u * per) < 0.1).
-__device__ __forceinline__ float encode_v(const float (&v)[8], uint32_t (&w)[2]) {
+// root: the approximate roots of v, exact ones below 2^-126. The largest root is the root of the largest value:
+// rounding keeps the order. A v > 0 takes the code 1 at least.
+__device__ __forceinline__ float encode_v(const float (&v)[8], const float (&root)[8], uint32_t (&w)[2]) {
     const float top = __fsqrt_rn(block_max(v));
     const float per = top > 0.0f ? __fdiv_rn(65025.0f, top) : 0.0f;
     w[0] = w[1] = 0;
     if (per > 0.0f) {
         uint32_t c[8];
-        bool     near = top < 0x1p-40f;
+        float    off = 0.0f;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) c[e] = code_of(sqrt_approx(__fmul_rn(sqrt_approx(v[e]), per)), 0x1p-13f, near);
-        if (near)
+        for (int e = 0; e < 8; ++e)
+            c[e] = code_of(fmaxf(sqrt_approx(__fmul_rn(root[e], per)), v[e] > 0.0f ? 1.0f : 0.0f), off);
+        if (off > 0.5f - 0x1p-13f)
 #pragma unroll
-            for (int e = 0; e < 8; ++e) c[e] = __float2uint_rn(__fsqrt_rn(__fmul_rn(__fsqrt_rn(v[e]), per)));
-#pragma unroll
-        for (int e = 0; e < 8; ++e) c[e] = v[e] > 0.0f ? max(c[e] & 0xFFu, 1u) : 0u;
+            for (int e = 0; e < 8; ++e)
+                c[e] = code_of(fmaxf(__fsqrt_rn(__fmul_rn(__fsqrt_rn(v[e]), per)), v[e] > 0.0f ? 1.0f : 0.0f), off);
         w[0] = pack4(c[0], c[1], c[2], c[3]);
         w[1] = pack4(c[4], c[5], c[6], c[7]);
     }
     return __fmul_rn(top, kUnitV);
+}
+
+__device__ __forceinline__ float root_of(float v) {
+    float root = sqrt_approx(v);
+    if (__float_as_uint(v) - 1u < 0x007FFFFFu) root = __fsqrt_rn(v);  // 0 < v < 2^-126
+    return root;
 }
 
 // One element's step: train_ops.cu's adamw_kernel.
@@ -218,12 +226,11 @@ __device__ __forceinline__ void adamw_one(float& p, float g, float& m, float& v,
 
 // The same with 8-bit states: m and v as above, the parameter's step with approximate operations (inv_bc2 is
 // 1 / bc2_sqrt rounded; the quotient is within 2 units, the root and the two products within one: 5 * 2^-23).
-__device__ __forceinline__ void adamw_one_8(float& p, float g, float& m, float& v, const AdamwParams& a, float one_b1,
-                                            float one_b2, float inv_bc2) {
+__device__ __forceinline__ void adamw_one_8(float& p, float g, float& m, float& v, float& root,
+                                            const AdamwParams& a, float one_b1, float one_b2, float inv_bc2) {
     m = __fadd_rn(m, __fmul_rn(__fsub_rn(g, m), one_b1));
     v = __fadd_rn(__fmul_rn(v, a.beta2), __fmul_rn(__fmul_rn(g, g), one_b2));
-    float root = sqrt_approx(v);
-    if (__float_as_uint(v) - 1u < 0x007FFFFFu) root = __fsqrt_rn(v);  // 0 < v < 2^-126
+    root = root_of(v);
     const float denom = fmaf(root, inv_bc2, a.eps);
     p = __fsub_rn(__fmul_rn(p, a.decay), __fmul_rn(a.step_sz, __fdividef(m, denom)));
 }
@@ -260,13 +267,14 @@ __device__ __forceinline__ void step_block(const StepJob& J, int64_t b0, const A
         }
     }
     [[maybe_unused]] const float inv_bc2 = __fdiv_rn(1.0f, a.bc2_sqrt);
+    [[maybe_unused]] float root[8];
 #pragma unroll
     for (int h = 0; h < 2; ++h)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             const float ge = clipped ? __fmul_rn(g[h][e], clip) : g[h][e];
             if constexpr (BITS == 32) adamw_one(p[h][e], ge, m[4 * h + e], v[4 * h + e], a, one_b1, one_b2);
-            else adamw_one_8(p[h][e], ge, m[4 * h + e], v[4 * h + e], a, one_b1, one_b2, inv_bc2);
+            else adamw_one_8(p[h][e], ge, m[4 * h + e], v[4 * h + e], root[4 * h + e], a, one_b1, one_b2, inv_bc2);
         }
 #pragma unroll
     for (int h = 0; h < 2; ++h) store4(J.p, i0 + 128 * h, n, FULL, p[h]);
@@ -280,9 +288,9 @@ __device__ __forceinline__ void step_block(const StepJob& J, int64_t b0, const A
         if constexpr (!FULL)  // what lies behind the tensor's end is not part of its last block
 #pragma unroll
             for (int e = 0; e < 8; ++e)
-                if (i0 + 128 * (e >> 2) + (e & 3) >= n) m[e] = v[e] = 0.0f;
+                if (i0 + 128 * (e >> 2) + (e & 3) >= n) m[e] = v[e] = root[e] = 0.0f;
         uint32_t wm[2], wv[2];
-        const float sm = encode_m(m, wm), sv = encode_v(v, wv);
+        const float sm = encode_m(m, wm), sv = encode_v(v, root, wv);
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             store4c(static_cast<uint8_t*>(J.m), i0 + 128 * h, n, FULL, wm[h]);
@@ -357,7 +365,15 @@ __global__ void __launch_bounds__(kThreads) state8_from_f32_kernel(const float* 
 #pragma unroll
     for (int e = 0; e < 8; ++e) x[e] = __fadd_rn(x[e], 0.0f);  // no -0
     uint32_t w[2];
-    const float s = WHICH == 0 ? encode_m(x, w) : encode_v(x, w);
+    float s;
+    if constexpr (WHICH == 0) {
+        s = encode_m(x, w);
+    } else {
+        float root[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) root[e] = root_of(x[e]);
+        s = encode_v(x, root, w);
+    }
     store4c(codes, i0, n, whole, w[0]);
     store4c(codes, i0 + 128, n, whole, w[1]);
     if ((threadIdx.x & 31) == 0) scales[b] = s;
