@@ -111,6 +111,11 @@ SIZES = [
     (300, 2048, 1088, (16, 16), "runs", 37),
     (1031, 516, 1030, (24, 3), "mixed", 0),
     (2050, 640, 416, (64,), "runs", 2),
+    (128, 64, 36, (16,), "runs", 0),
+    (129, 100, 164, (30,), "runs", 1),
+    (200, 96, 160, (16, 7, 64), "mixed", 9),
+    (400, 512, 260, (4, 8, 20, 16, 32, 3) * 4, "mixed", 17),
+    (513, 1024, 2052, (40, 48, 64), "runs", 130),      # a tile of rows without an adapter
 ]
 
 
@@ -120,8 +125,8 @@ def test_forward_and_gradients_f32(tc, rows, k, n, ranks, order, none):
 
 
 @pytest.mark.parametrize("kind", ["f16", "bf16"])
-@pytest.mark.parametrize("rows,k,n,ranks,order,none", [SIZES[i] for i in (0, 1, 2, 5, 7, 8, 11, 12, 13)],
-                         ids=[f"{SIZES[i][0]}x{SIZES[i][1]}x{SIZES[i][2]}" for i in (0, 1, 2, 5, 7, 8, 11, 12, 13)])
+@pytest.mark.parametrize("rows,k,n,ranks,order,none", [SIZES[i] for i in (0, 1, 2, 5, 7, 8, 11, 12, 13, 17, 18, 20)],
+                         ids=[f"{SIZES[i][0]}x{SIZES[i][1]}x{SIZES[i][2]}" for i in (0, 1, 2, 5, 7, 8, 11, 12, 13, 17, 18, 20)])
 def test_forward_and_gradients_half_factors(tc, kind, rows, k, n, ranks, order, none):
     check_all(tc, rows, k, n, ranks, kind, order, none)
 
@@ -229,9 +234,10 @@ def test_rows_without_an_adapter_keep_their_base(tc):
     assert bool((tc.lora(handle, x, ids, out=torch.full_like(base, 5.0))[out_of] == 0).all())  # no base: zero
 
 
-def test_bad_values_stay_in_their_rows(tc):
+@pytest.mark.parametrize("rows", [48, 100, 300])
+def test_bad_values_stay_in_their_rows(tc, rows):
     """A NaN or an infinity in one row, or in one adapter's weights, reaches that row, or that adapter's rows."""
-    rows, k, n = 48, 128, 64
+    k, n = 128, 64
     ad, ids, x, base, dy = make(rows, k, n, (16, 16, 16), order="mixed")
     clean = formula(ad, ids, x, base, dy)
     x[5, 3], x[6, 0] = float("nan"), float("inf")

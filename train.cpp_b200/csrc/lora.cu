@@ -5,54 +5,17 @@
 //   g[t]  = scale * B^T dy[t]          (down, with B in A's place)
 //   dx[t] = base[t] + A^T g[t]         (up, with A in B's place)
 //   dA    = sum g[t] x[t]^T,  dB = sum dy[t] h[t]^T   (over the adapter's rows)
-#include <cuda_bf16.h>
-#include <cuda_fp16.h>
-#include <cuda_runtime.h>
-
 #include <algorithm>
 #include <cstdint>
 #include <type_traits>
 
-#include "trc_internal.h"
-#include "trc_ptx.cuh"
+#include "lora_common.cuh"
 
 namespace trc {
 
+using namespace lora;
+
 namespace {
-
-struct Adapter {
-    const void* a;
-    const void* b;
-    float*      da;
-    float*      db;
-    float       scale;
-    int16_t     rank;
-    int16_t     vec;  // bit 0: A may be loaded four values at a time, bit 1: B
-};
-
-struct Adapters {
-    Adapter ad[TRC_CUDA_LORA_MAX_ADAPTERS];
-    int32_t n;
-};
-
-// The rows of a ggml view: row t = (i1, i2, i3) in ggml order.
-struct Rows {
-    char*   data;
-    int64_t nb0, nb1, nb2, nb3;
-    int32_t n1, n2;
-    int32_t step;  // rows are this many floats apart throughout; -1: they are not
-    template <bool EVEN>
-    __device__ __forceinline__ char* row(int64_t t) const {
-        if (EVEN || step >= 0) return data + 4 * (t * step);
-        const int64_t i1 = t % n1, r = t / n1;
-        return data + i1 * nb1 + (r % n2) * nb2 + (r / n2) * nb3;
-    }
-};
-
-__device__ __forceinline__ int adapter_of(const int32_t* ids, int64_t t, int n) {
-    const int id = ids == nullptr ? 0 : ids[t];
-    return id >= 0 && id < n ? id : -1;
-}
 
 // ------------------------------------------------------------------ tensor-core pieces
 // All products run as m16n8k8 TF32 with fp32 sums. In a warp, lane = 4 * c + q (c = 0..7, q = 0..3):
@@ -66,13 +29,6 @@ __device__ __forceinline__ void mma8(float (&d)[4], const uint32_t (&a)[4], cons
     asm("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]));
-}
-
-// x = head + tail, the head rounded to TF32's 11 bits and the tail exact; the tensor core reads the
-// tail's first 11 bits, so head + tail as it sees them are within 2^-21 of x.
-__device__ __forceinline__ void split(float x, uint32_t& head, uint32_t& tail) {
-    head = (__float_as_uint(x) + 0x1000u) & 0xFFFFE000u;
-    tail = __float_as_uint(x - __uint_as_float(head));
 }
 
 // d += a * b in three TF32 products (two where b is a half-precision factor, whose values TF32 holds
@@ -92,44 +48,6 @@ __device__ __forceinline__ void split_b(float x, uint32_t& head, uint32_t& tail)
         tail = 0;
     } else {
         split(x, head, tail);
-    }
-}
-
-// N factor values held in the words of one load, as floats.
-template <typename W, int N>
-__device__ __forceinline__ void widen(const uint32_t (&raw)[N * sizeof(W) / 4], float (&w)[N]) {
-    if constexpr (sizeof(W) == 4) {
-#pragma unroll
-        for (int j = 0; j < N; ++j) w[j] = __uint_as_float(raw[j]);
-    } else {
-        const W* e = reinterpret_cast<const W*>(raw);
-#pragma unroll
-        for (int j = 0; j < N; ++j) w[j] = static_cast<float>(e[j]);
-    }
-}
-
-// N consecutive factor values as floats, in one load (WHOLE) or one by one, as far as there are any: `have`
-// counts those from p on that are inside.
-template <typename W, int N, bool WHOLE>
-__device__ __forceinline__ void load_w(const W* p, int have, float (&w)[N]) {
-    if constexpr (WHOLE) {
-        constexpr int kWords = N * static_cast<int>(sizeof(W)) / 4;
-        uint32_t raw[kWords] = {};
-        if (have > 0) {
-            if constexpr (kWords == 4) {
-                const uint4 t = __ldg(reinterpret_cast<const uint4*>(p));
-                raw[0] = t.x; raw[1] = t.y; raw[2] = t.z; raw[3] = t.w;
-            } else if constexpr (kWords == 2) {
-                const uint2 t = __ldg(reinterpret_cast<const uint2*>(p));
-                raw[0] = t.x; raw[1] = t.y;
-            } else {
-                raw[0] = __ldg(reinterpret_cast<const uint32_t*>(p));
-            }
-        }
-        widen<W, N>(raw, w);
-    } else {
-#pragma unroll
-        for (int j = 0; j < N; ++j) w[j] = j < have ? static_cast<float>(p[j]) : 0.0f;
     }
 }
 
@@ -218,9 +136,6 @@ struct TileIds {
         leaders = __ballot_sync(0xFFFFFFFFu, id >= 0 && __ffs(same) - 1 == lane);
     }
 };
-
-__device__ __forceinline__ void grid_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
-__device__ __forceinline__ void grid_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
 __device__ __forceinline__ float ld_cluster(uint32_t addr) {
     float v;
@@ -1061,10 +976,6 @@ __global__ void __launch_bounds__(kThreads, GradRing<MT>::kCtas) grad_kernel(con
 
 constexpr int64_t kMaxLen = int64_t(1) << 30;  // rows, K and N of a call
 
-bool aligned_to(const void* p, uint64_t bytes) { return (reinterpret_cast<uint64_t>(p) & (bytes - 1)) == 0; }
-
-int64_t item_bytes(int type) { return type == TRC_CUDA_TYPE_F32 ? 4 : 2; }
-
 // TRC_CUDA_OK if the adapters are valid for trc_cuda_lora*; *ld = the row length of h.
 int check_adapters(const trc_cuda_lora_adapter* ad, int n, int64_t item, int64_t* ld) {
     if (n < 0 || (n > 0 && ad == nullptr)) return TRC_CUDA_EINVAL;
@@ -1320,6 +1231,10 @@ int up(int type, const Adapters& tab, const int32_t* ids, const trc_cuda_view* b
     const Rows rb = rows_of(base), rd = rows_of(d);
     const int n = static_cast<int>(d->ne[0]);
     const bool vec = vec_rows(base) && vec_rows(d);
+    if (vec) {
+        const int st = up_tc(BACK, type, tab, ids, base, d, rows, h, ld, s);
+        if (st != TRC_CUDA_EUNSUPPORTED) return st;
+    }
     if (type == TRC_CUDA_TYPE_F32) return up_of<BACK, float>(tab, ids, rb, rd, vec, rows, n, h, ld, s);
     if (type == TRC_CUDA_TYPE_F16) return up_of<BACK, __half>(tab, ids, rb, rd, vec, rows, n, h, ld, s);
     return up_of<BACK, __nv_bfloat16>(tab, ids, rb, rd, vec, rows, n, h, ld, s);

@@ -1,0 +1,412 @@
+// lora_tc.cu -- the wide product of the low-rank adapters, d = base + h W^T, on tcgen05.
+//
+// It moves base and d once (8 bytes for each output) and computes 2 * rank flops for it in three TF32
+// products: at rank 64 that is 3 * 128 flops for 8 bytes, more than the mma.sync pipe gives beside the copy (93
+// TFLOP/s of split products), and a quarter of what tcgen05 does.
+//
+// A CTA takes 128 rows (the MMA's M) and walks over blocks of 32 columns (its N). The rows' h is the first
+// operand and stays in TMEM for the whole walk, as heads and tails; the factor's block is the second, built in shared
+// memory by four warps (heads and tails, K-major, 64-byte swizzle); the sums land in TMEM, double-buffered; four
+// warps, one row per lane, add them to base's block, which TMA has brought, in place, and TMA takes it to d. A tile whose rows
+// have several adapters goes through all of them for each block, each row keeping the sums of its own: base and d
+// still move once.
+#include <cuda.h>
+#include <cudaTypedefs.h>
+
+#include <algorithm>
+#include <mutex>
+
+#include "lora_common.cuh"
+
+namespace trc {
+namespace lora {
+
+namespace {
+
+constexpr int kTile = 128, kBlock = 32;           // rows and columns of a step
+constexpr int kSlots = 4;                          // blocks of base and d in shared memory
+constexpr int kSlotBytes = kTile * kBlock * 4;     // 16 KB
+constexpr int kTcThreads = 288;                    // 4 warps add and store, 4 build the factor's blocks, 1 issues
+
+template <typename W, int LD>
+struct TcSmem {
+    static constexpr int kPart = kBlock * LD * 4;                  // heads or tails of a block of the factor
+    static constexpr int kW = kPart * (sizeof(W) == 2 ? 1 : 2);    // half factors have no tails
+    static constexpr int kBytes = kSlots * kSlotBytes + 2 * kW + 1024;
+    static constexpr uint32_t kCols = 2 * LD + 2 * kBlock <= 128 ? 128 : 256;  // TMEM: heads, tails, two blocks of sums
+};
+
+// The MMA with its first operand in TMEM.
+__device__ __forceinline__ void umma_tf32_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::tf32 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
+        "r"(a_tmem), "l"(bdesc), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+
+__device__ __forceinline__ void tma_load_2d(uint32_t dst, const void* map, uint64_t* bar, int c0, int c1) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(smem_u32(bar))
+        : "memory");
+}
+
+__device__ __forceinline__ void tma_store_2d(const void* map, uint32_t src, int c0, int c1) {
+    asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%1, %2}], [%3];" ::"l"(reinterpret_cast<uint64_t>(map)),
+                 "r"(c0), "r"(c1), "r"(src)
+                 : "memory");
+}
+
+struct Bars {
+    uint64_t w_full[2];          // the factor's block is built (128 arrivals)
+    uint64_t d_full[2];          // the sums are complete, the factor's block is read (the MMA's commit)
+    uint64_t d_free[2];          // the sums are in registers (128 arrivals)
+    uint64_t slot_full[kSlots];  // base's block is there
+    uint64_t slot_free[kSlots];  // d's block has left
+};
+
+template <typename W, bool BACK, int LD>
+__global__ void __launch_bounds__(kTcThreads, 2) up_tc_kernel(const __grid_constant__ Adapters tab, const int32_t* ids,
+                                                           const __grid_constant__ CUtensorMap base_map,
+                                                           const __grid_constant__ CUtensorMap d_map, int add, int64_t rows,
+                                                           int n_len, const float* h, int ld, int blocks_per, int splits) {
+    constexpr bool HALF = sizeof(W) == 2;
+    using S = TcSmem<W, LD>;
+    extern __shared__ uint8_t tc_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(tc_raw) + 1023) & ~uintptr_t(1023));
+    uint8_t* wbuf = smem + kSlots * kSlotBytes;
+    __shared__ __align__(8) Bars bars;
+    __shared__ uint32_t tmem_slot;
+    __shared__ int      tile_id[kTile], list[kTile], counts[4];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int64_t row0 = static_cast<int64_t>(blockIdx.x / splits) * kTile;
+    const int block0 = static_cast<int>(blockIdx.x % splits) * blocks_per;
+    const int blocks = min(blocks_per, (n_len + kBlock - 1) / kBlock - block0);
+
+    if (threadIdx.x == 256) {
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&bars.w_full[i], 128);
+            mbar_init(&bars.d_full[i], 1);
+            mbar_init(&bars.d_free[i], 128);
+        }
+        for (int i = 0; i < kSlots; ++i) {
+            mbar_init(&bars.slot_full[i], 1);
+            mbar_init(&bars.slot_free[i], 1);
+        }
+        fence_barrier_init();
+    }
+    if (warp == 8) {
+        tmem_alloc(&tmem_slot, S::kCols);
+        tmem_relinquish();
+    }
+    if (threadIdx.x < kTile) {
+        const int64_t t = row0 + threadIdx.x;
+        tile_id[threadIdx.x] = t < rows ? adapter_of(ids, t, tab.n) : -1;
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = tmem_slot;
+    // the tile's adapters, in the order of their first rows
+    if (warp < 4) {
+        const int t = threadIdx.x, id = tile_id[t];
+        bool first = id >= 0 && (t == 0 || tile_id[t - 1] != id);
+        for (int u = 0; first && u < t; ++u) first = tile_id[u] != id;
+        const uint32_t firsts = __ballot_sync(0xFFFFFFFFu, first);
+        if (lane == 0) counts[warp] = __popc(firsts);
+        named_barrier_sync(1, 128);
+        int at = __popc(firsts & ((1u << lane) - 1u));
+        for (int v = 0; v < warp; ++v) at += counts[v];
+        if (first) list[at] = id;
+    }
+    __syncthreads();
+    const int n_ad = counts[0] + counts[1] + counts[2] + counts[3];
+    const int per = max(n_ad, 1);  // steps of a block; a tile without adapters only passes base through
+    const int steps = blocks * per;
+    bool ok = true;
+
+    if (warp < 4) {
+        // ---------------- one row per lane: sums + base -> d
+        const int  my_id = tile_id[threadIdx.x];
+        const bool leader = threadIdx.x == 0;
+        for (int b = 0; b < blocks && ok; ++b) {
+            const int slot = b % kSlots;
+            uint32_t  y[32];
+            for (int i = 0; i < n_ad; ++i) {
+                const int s = b * per + i, buf = s & 1;
+                ok = ok && mbar_wait(&bars.d_full[buf], (s >> 1) & 1, TRC_DEVERR_WAIT_ACCUM);
+                tc_fence_after();
+                uint32_t v[32];
+                tmem_ld_32x32b_x32(tmem + (static_cast<uint32_t>(warp * 32) << 16) + 2 * LD + buf * kBlock, v);
+                tmem_ld_wait();
+                tc_fence_before();
+                mbar_arrive(&bars.d_free[buf]);
+                if (my_id == list[i])
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) y[e] = v[e];
+            }
+            ok = ok && mbar_wait(&bars.slot_full[slot], (b / kSlots) & 1, TRC_DEVERR_WAIT_FULL);
+            // 16-byte unit u of row r lies at unit u ^ (r & 7) (128-byte swizzle)
+            uint8_t* row = smem + slot * kSlotBytes + threadIdx.x * 128;
+#pragma unroll
+            for (int u = 0; u < 8; ++u) {
+                float4* p = reinterpret_cast<float4*>(row + ((u ^ (threadIdx.x & 7)) << 4));
+                float4  o = add ? *p : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                if (my_id >= 0) {
+                    o.x += __uint_as_float(y[4 * u]);
+                    o.y += __uint_as_float(y[4 * u + 1]);
+                    o.z += __uint_as_float(y[4 * u + 2]);
+                    o.w += __uint_as_float(y[4 * u + 3]);
+                }
+                *p = o;
+            }
+            fence_proxy_async_smem();
+            ok = named_barrier_and(1, 128, ok);
+            if (leader && ok) {
+                tma_store_2d(&d_map, smem_u32(smem + slot * kSlotBytes), (block0 + b) * kBlock, static_cast<int>(row0));
+                bulk_commit_group();
+                bulk_wait_group_read<1>();  // the block before has left its slot
+                if (b > 0) mbar_arrive(&bars.slot_free[(b - 1) % kSlots]);
+            }
+        }
+        if (leader) bulk_wait_group_all();
+    } else if (warp < 8) {
+        // ---------------- the rows' h to TMEM, then the factor's blocks to shared memory
+        const int tid = threadIdx.x - 128;
+        grid_wait();  // h is written
+        if (n_ad > 0) {
+            const int64_t t = row0 + tid;
+            const uint32_t lane_base = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
+#pragma unroll
+            for (int g = 0; g < LD / 16; ++g) {
+                uint32_t head[16], tail[16];
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {
+                    float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                    if (t < rows && 16 * g < ld) v = *reinterpret_cast<const float4*>(h + t * ld + 16 * g + 4 * u);
+                    split(v.x, head[4 * u], tail[4 * u]);
+                    split(v.y, head[4 * u + 1], tail[4 * u + 1]);
+                    split(v.z, head[4 * u + 2], tail[4 * u + 2]);
+                    split(v.w, head[4 * u + 3], tail[4 * u + 3]);
+                }
+                tmem_st_32x32b_x16(lane_base + 16 * g, head);
+                tmem_st_32x32b_x16(lane_base + LD + 16 * g, tail);
+            }
+            tmem_st_wait();
+            tc_fence_before();
+        }
+        // Pieces of four values of a block: FWD column i / (LD / 4), ranks 4 (i % (LD / 4)) ..; BACK rank j, columns kq ..
+        // (8 ranks and 4 groups of columns to a warp, so that the transposing stores meet in two lanes a bank).
+        constexpr int kPieces = kBlock * LD / 4 / 128;
+        float v[kPieces][4];
+        auto place = [&](int p, int& n, int& j) {
+            const int i = tid + 128 * p;
+            if constexpr (!BACK) {
+                n = i / (LD / 4);
+                j = 4 * (i % (LD / 4));
+            } else {
+                j = (i & 7) + 8 * (i / 64);
+                n = 4 * ((i >> 3) & 7);
+            }
+        };
+        auto load = [&](int s) {
+            const Adapter& A = tab.ad[list[s % per]];
+            const int      r = A.rank, n0 = (block0 + s / per) * kBlock;
+            const W*       w = static_cast<const W*>(BACK ? A.a : A.b);
+            const bool     whole = (A.vec & (BACK ? 1 : 2)) != 0;
+#pragma unroll
+            for (int p = 0; p < kPieces; ++p) {
+                int n, j;
+                place(p, n, j);
+                const W* from = BACK ? w + (static_cast<int64_t>(j) * n_len + n0 + n) : w + (static_cast<int64_t>(n0 + n) * r + j);
+                const int have = BACK ? (j < r ? n_len - (n0 + n) : 0) : (n0 + n < n_len ? r - j : 0);
+                if (whole) load_w<W, 4, true>(from, have, v[p]);
+                else load_w<W, 4, false>(from, have, v[p]);
+            }
+        };
+        if (n_ad > 0) load(0);
+        for (int s = 0; n_ad > 0 && s < steps && ok; ++s) {
+            const int buf = s & 1;
+            if (s >= 2) ok = mbar_wait(&bars.d_full[buf], ((s >> 1) - 1) & 1, TRC_DEVERR_WAIT_EMPTY);
+            uint8_t* heads = wbuf + buf * S::kW;
+            uint8_t* tails = heads + S::kPart;
+#pragma unroll
+            for (int p = 0; p < kPieces; ++p) {
+                int n, j;
+                place(p, n, j);
+                uint32_t hd[4], tl[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    if constexpr (HALF) hd[e] = __float_as_uint(v[p][e]);
+                    else split(v[p][e], hd[e], tl[e]);
+                }
+                if constexpr (!BACK) {
+                    const int off = (j >> 4) * (kBlock * 64) + n * 64 + ((((j >> 2) & 3) ^ ((n >> 1) & 3)) << 4);
+                    *reinterpret_cast<uint4*>(heads + off) = make_uint4(hd[0], hd[1], hd[2], hd[3]);
+                    if constexpr (!HALF) *reinterpret_cast<uint4*>(tails + off) = make_uint4(tl[0], tl[1], tl[2], tl[3]);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const int m = n + e;
+                        const int off = (j >> 4) * (kBlock * 64) + m * 64 + ((((j >> 2) & 3) ^ ((m >> 1) & 3)) << 4) + 4 * (j & 3);
+                        *reinterpret_cast<uint32_t*>(heads + off) = hd[e];
+                        if constexpr (!HALF) *reinterpret_cast<uint32_t*>(tails + off) = tl[e];
+                    }
+                }
+            }
+            fence_proxy_async_smem();
+            mbar_arrive(&bars.w_full[buf]);
+            if (s + 1 < steps) load(s + 1);
+        }
+    } else if (lane == 0) {
+        // ---------------- base's blocks and the MMAs
+        const uint32_t idesc = make_idesc_tf32(kTile, kBlock, 0, 0);
+        const uint32_t wbase = smem_u32(wbuf);
+        int asked = 0, issued = 0;
+        auto ask = [&](int b) {  // base's block b into its slot
+            const int slot = b % kSlots;
+            if (b >= kSlots && !mbar_wait(&bars.slot_free[slot], (b / kSlots - 1) & 1, TRC_DEVERR_WAIT_EMPTY)) return false;
+            if (add) {
+                mbar_arrive_expect_tx(&bars.slot_full[slot], kSlotBytes);
+                tma_load_2d(smem_u32(smem + slot * kSlotBytes), &base_map, &bars.slot_full[slot], (block0 + b) * kBlock,
+                            static_cast<int>(row0));
+            } else {
+                mbar_arrive(&bars.slot_full[slot]);
+            }
+            ++asked;
+            return true;
+        };
+        for (int b = 0; b < min(blocks, kSlots - 1); ++b) ok = ok && ask(b);
+        for (int s = 0; s < steps && ok; ++s) {
+            const int b = s / per;
+            // the slot of the block before this one is free once that block has left
+            if (s % per == 0 && b > 0 && b + kSlots - 2 < blocks) ok = ask(b + kSlots - 2);
+            if (n_ad == 0) continue;
+            const int buf = s & 1;
+            ok = ok && mbar_wait(&bars.w_full[buf], (s >> 1) & 1, TRC_DEVERR_WAIT_XFORM);
+            if (s >= 2) ok = ok && mbar_wait(&bars.d_free[buf], ((s >> 1) - 1) & 1, TRC_DEVERR_WAIT_ACCFREE);
+            if (!ok) break;
+            tc_fence_after();
+            const uint32_t heads = wbase + buf * S::kW, tails = heads + S::kPart, dst = tmem + 2 * LD + buf * kBlock;
+            const int groups = min(LD / 16, (tab.ad[list[s % per]].rank + 15) / 16);
+            for (int g = 0; g < groups; ++g)
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    const uint64_t bh = make_smem_desc(heads + g * (kBlock * 64) + k * 32, 16, 512, 4);
+                    const uint32_t a = tmem + 16 * g + 8 * k;
+                    umma_tf32_ts(dst, a + LD, bh, idesc, g + k > 0);
+                    if constexpr (!HALF) umma_tf32_ts(dst, a, make_smem_desc(tails + g * (kBlock * 64) + k * 32, 16, 512, 4), idesc, 1);
+                    umma_tf32_ts(dst, a, bh, idesc, 1);
+                }
+            umma_commit(&bars.d_full[buf]);
+            issued = s + 1;
+        }
+        // nothing may still write to shared memory or TMEM when the CTA ends
+        for (int b = max(0, asked - kSlots); b < asked; ++b) mbar_wait_drain(&bars.slot_full[b % kSlots], (b / kSlots) & 1);
+        for (int s = max(0, issued - 2); s < issued; ++s) mbar_wait_drain(&bars.d_full[s & 1], (s >> 1) & 1);
+    }
+    __syncwarp();
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    if (warp == 8) tmem_dealloc(tmem, S::kCols);
+}
+
+PFN_cuTensorMapEncodeTiled_v12000 encoder() {
+    static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
+    static std::once_flag once;
+    std::call_once(once, [] {
+        void* ptr = nullptr;
+        cudaDriverEntryPointQueryResult q = cudaDriverEntryPointSymbolNotFound;
+        if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &ptr, 12000, cudaEnableDefault, &q) == cudaSuccess &&
+            q == cudaDriverEntryPointSuccess)
+            fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(ptr);
+    });
+    return fn;
+}
+
+// Evenly spaced rows of floats (the caller has checked them), in boxes of 128 rows by 32 columns.
+bool encode_rows(const trc_cuda_view& v, int64_t rows, CUtensorMap& map) {
+    auto enc = encoder();
+    if (enc == nullptr) return false;
+    // one stride for all rows, that of the first extent over 1
+    int64_t step = 4 * v.ne[0];
+    for (int i = 3; i >= 1; --i)
+        if (v.ne[i] > 1) step = v.nb[i];
+    if (step <= 0 || step % 16 != 0) return false;
+    const cuuint64_t dims[2] = {static_cast<cuuint64_t>(v.ne[0]), static_cast<cuuint64_t>(rows)};
+    const cuuint64_t strides[1] = {static_cast<cuuint64_t>(step)};
+    const cuuint32_t box[2] = {kBlock, kTile}, one[2] = {1, 1};
+    return enc(&map, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 2, v.data, dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+               CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <typename W, bool BACK, int LD>
+int run(const Adapters& tab, const int32_t* ids, const CUtensorMap& base_map, const CUtensorMap& d_map, int add, int64_t rows, int n,
+        const float* h, int ld, cudaStream_t s) {
+    auto kernel = &up_tc_kernel<W, BACK, LD>;
+    const int smem = TcSmem<W, LD>::kBytes;
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) return cuda_fail(e);
+    // two waves of two CTAs for each SM (tiles at the borders between requests take longer than others), at least 8
+    // blocks to a CTA
+    const int64_t tiles = (rows + kTile - 1) / kTile;
+    const int blocks = (n + kBlock - 1) / kBlock;
+    const int64_t want = std::max<int64_t>(1, 4 * static_cast<int64_t>(std::max(1, sm_count_current())) / tiles);
+    const int per = static_cast<int>(std::max<int64_t>(std::min(blocks, 8), (blocks + want - 1) / want));
+    const int splits = (blocks + per - 1) / per;
+    if (tiles * splits > INT32_MAX) return TRC_CUDA_EUNSUPPORTED;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(static_cast<unsigned>(tiles * splits));
+    cfg.blockDim = dim3(kTcThreads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;  // it waits for down's h itself
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    e = cudaLaunchKernelEx(&cfg, kernel, tab, ids, base_map, d_map, add, rows, n, h, ld, per, splits);
+    if (e != cudaSuccess) {
+        cudaGetLastError();
+        return cuda_fail(e);
+    }
+    note_launch();
+    return TRC_CUDA_OK;
+}
+
+template <typename W, bool BACK>
+int run_ld(const Adapters& tab, const int32_t* ids, const CUtensorMap& base_map, const CUtensorMap& d_map, int add, int64_t rows,
+           int n, const float* h, int ld, cudaStream_t s) {
+    if (ld == 16) return run<W, BACK, 16>(tab, ids, base_map, d_map, add, rows, n, h, ld, s);
+    if (ld == 32) return run<W, BACK, 32>(tab, ids, base_map, d_map, add, rows, n, h, ld, s);
+    return run<W, BACK, 64>(tab, ids, base_map, d_map, add, rows, n, h, ld, s);
+}
+
+template <typename W>
+int run_dir(bool back, const Adapters& tab, const int32_t* ids, const CUtensorMap& base_map, const CUtensorMap& d_map, int add,
+            int64_t rows, int n, const float* h, int ld, cudaStream_t s) {
+    return back ? run_ld<W, true>(tab, ids, base_map, d_map, add, rows, n, h, ld, s)
+                : run_ld<W, false>(tab, ids, base_map, d_map, add, rows, n, h, ld, s);
+}
+
+}  // namespace
+
+int up_tc(bool back, int type, const Adapters& tab, const int32_t* ids, const trc_cuda_view* base, const trc_cuda_view* d,
+          int64_t rows, const float* h, int ld, cudaStream_t s) {
+    // a tile of 128 rows has to be worth its own: below, the warp-level kernel's tiles of 32 rows fill more SMs
+    if (ld > 64 || rows < 128) return TRC_CUDA_EUNSUPPORTED;
+    CUtensorMap d_map, base_map;
+    if (!encode_rows(*d, rows, d_map)) return TRC_CUDA_EUNSUPPORTED;
+    base_map = d_map;
+    if (base != nullptr && !encode_rows(*base, rows, base_map)) return TRC_CUDA_EUNSUPPORTED;
+    const int add = base != nullptr, n = static_cast<int>(d->ne[0]);
+    if (type == TRC_CUDA_TYPE_F32) return run_dir<float>(back, tab, ids, base_map, d_map, add, rows, n, h, ld, s);
+    if (type == TRC_CUDA_TYPE_F16) return run_dir<__half>(back, tab, ids, base_map, d_map, add, rows, n, h, ld, s);
+    return run_dir<__nv_bfloat16>(back, tab, ids, base_map, d_map, add, rows, n, h, ld, s);
+}
+
+}  // namespace lora
+}  // namespace trc
