@@ -67,13 +67,14 @@ __device__ __forceinline__ void widen(const uint32_t (&raw)[N * sizeof(W) / 4], 
     }
 }
 
-// N consecutive factor values as floats, in one load (WHOLE) or one by one, as far as there are any: `have`
-// counts those from p on that are inside.
+// N consecutive factor values as they are, in one load (WHOLE) or one by one, as far as there are any: `have`
+// counts those from p on that are inside; the others are zero.
 template <typename W, int N, bool WHOLE>
-__device__ __forceinline__ void load_w(const W* p, int have, float (&w)[N]) {
+__device__ __forceinline__ void load_raw(const W* p, int have, uint32_t (&raw)[N * sizeof(W) / 4]) {
+    constexpr int kWords = N * static_cast<int>(sizeof(W)) / 4;
+#pragma unroll
+    for (int j = 0; j < kWords; ++j) raw[j] = 0;
     if constexpr (WHOLE) {
-        constexpr int kWords = N * static_cast<int>(sizeof(W)) / 4;
-        uint32_t raw[kWords] = {};
         if (have > 0) {
             if constexpr (kWords == 4) {
                 const uint4 t = __ldg(reinterpret_cast<const uint4*>(p));
@@ -85,11 +86,22 @@ __device__ __forceinline__ void load_w(const W* p, int have, float (&w)[N]) {
                 raw[0] = __ldg(reinterpret_cast<const uint32_t*>(p));
             }
         }
-        widen<W, N>(raw, w);
     } else {
 #pragma unroll
-        for (int j = 0; j < N; ++j) w[j] = j < have ? static_cast<float>(p[j]) : 0.0f;
+        for (int j = 0; j < N; ++j)
+            if (j < have) {
+                if constexpr (sizeof(W) == 4) raw[j] = *reinterpret_cast<const uint32_t*>(p + j);
+                else raw[j / 2] |= static_cast<uint32_t>(*reinterpret_cast<const uint16_t*>(p + j)) << (16 * (j % 2));
+            }
     }
+}
+
+// The same as floats.
+template <typename W, int N, bool WHOLE>
+__device__ __forceinline__ void load_w(const W* p, int have, float (&w)[N]) {
+    uint32_t raw[N * sizeof(W) / 4];
+    load_raw<W, N, WHOLE>(p, have, raw);
+    widen<W, N>(raw, w);
 }
 
 __device__ __forceinline__ void grid_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }

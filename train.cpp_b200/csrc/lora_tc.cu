@@ -24,7 +24,6 @@ namespace lora {
 namespace {
 
 constexpr int kTile = 128, kBlock = 32;           // rows and columns of a step
-constexpr int kSlots = 4;                          // blocks of base and d in shared memory
 constexpr int kSlotBytes = kTile * kBlock * 4;     // 16 KB
 constexpr int kTcThreads = 288;                    // 4 warps add and store, 4 build the factor's blocks, 1 issues
 
@@ -32,7 +31,10 @@ template <typename W, int LD>
 struct TcSmem {
     static constexpr int kPart = kBlock * LD * 4;                  // heads or tails of a block of the factor
     static constexpr int kW = kPart * (sizeof(W) == 2 ? 1 : 2);    // half factors have no tails
+    // blocks of base and d: as many as leave room for two CTAs on an SM
+    static constexpr int kSlots = 2 * kW <= 8 * 1024 ? 6 : 2 * kW <= 16 * 1024 ? 5 : 4;
     static constexpr int kBytes = kSlots * kSlotBytes + 2 * kW + 1024;
+    static_assert(kBytes <= 112 * 1024, "two CTAs on an SM");
     static constexpr uint32_t kCols = 2 * LD + 2 * kBlock <= 128 ? 128 : 256;  // TMEM: heads, tails, two blocks of sums
 };
 
@@ -59,6 +61,7 @@ __device__ __forceinline__ void tma_store_2d(const void* map, uint32_t src, int 
                  : "memory");
 }
 
+template <int kSlots>
 struct Bars {
     uint64_t w_full[2];          // the factor's block is built (128 arrivals)
     uint64_t d_full[2];          // the sums are complete, the factor's block is read (the MMA's commit)
@@ -74,10 +77,11 @@ __global__ void __launch_bounds__(kTcThreads, 2) up_tc_kernel(const __grid_const
                                                            int n_len, const float* h, int ld, int blocks_per, int splits) {
     constexpr bool HALF = sizeof(W) == 2;
     using S = TcSmem<W, LD>;
+    constexpr int kSlots = S::kSlots;
     extern __shared__ uint8_t tc_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(tc_raw) + 1023) & ~uintptr_t(1023));
     uint8_t* wbuf = smem + kSlots * kSlotBytes;
-    __shared__ __align__(8) Bars bars;
+    __shared__ __align__(8) Bars<kSlots> bars;
     __shared__ uint32_t tmem_slot;
     __shared__ int      tile_id[kTile], list[kTile], counts[4];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -199,8 +203,9 @@ __global__ void __launch_bounds__(kTcThreads, 2) up_tc_kernel(const __grid_const
         }
         // Pieces of four values of a block: FWD column i / (LD / 4), ranks 4 (i % (LD / 4)) ..; BACK rank j, columns kq ..
         // (8 ranks and 4 groups of columns to a warp, so that the transposing stores meet in two lanes a bank).
-        constexpr int kPieces = kBlock * LD / 4 / 128;
-        float v[kPieces][4];
+        // Loads run kAhead steps ahead: with one, a step took an L2 round trip (1.4 us at rank 16 against @@).
+        constexpr int kPieces = kBlock * LD / 4 / 128, kAhead = LD == 16 ? 4 : 2;
+        uint32_t raw[kAhead][kPieces][sizeof(W)];
         auto place = [&](int p, int& n, int& j) {
             const int i = tid + 128 * p;
             if constexpr (!BACK) {
@@ -211,7 +216,7 @@ __global__ void __launch_bounds__(kTcThreads, 2) up_tc_kernel(const __grid_const
                 n = 4 * ((i >> 3) & 7);
             }
         };
-        auto load = [&](int s) {
+        auto load = [&](int s, uint32_t (&to)[kPieces][sizeof(W)]) {
             const Adapter& A = tab.ad[list[s % per]];
             const int      r = A.rank, n0 = (block0 + s / per) * kBlock;
             const W*       w = static_cast<const W*>(BACK ? A.a : A.b);
@@ -222,43 +227,52 @@ __global__ void __launch_bounds__(kTcThreads, 2) up_tc_kernel(const __grid_const
                 place(p, n, j);
                 const W* from = BACK ? w + (static_cast<int64_t>(j) * n_len + n0 + n) : w + (static_cast<int64_t>(n0 + n) * r + j);
                 const int have = BACK ? (j < r ? n_len - (n0 + n) : 0) : (n0 + n < n_len ? r - j : 0);
-                if (whole) load_w<W, 4, true>(from, have, v[p]);
-                else load_w<W, 4, false>(from, have, v[p]);
+                if (whole) load_raw<W, 4, true>(from, have, to[p]);
+                else load_raw<W, 4, false>(from, have, to[p]);
             }
         };
-        if (n_ad > 0) load(0);
-        for (int s = 0; n_ad > 0 && s < steps && ok; ++s) {
-            const int buf = s & 1;
-            if (s >= 2) ok = mbar_wait(&bars.d_full[buf], ((s >> 1) - 1) & 1, TRC_DEVERR_WAIT_EMPTY);
-            uint8_t* heads = wbuf + buf * S::kW;
-            uint8_t* tails = heads + S::kPart;
+        const int my_steps = n_ad > 0 ? steps : 0;
 #pragma unroll
-            for (int p = 0; p < kPieces; ++p) {
-                int n, j;
-                place(p, n, j);
-                uint32_t hd[4], tl[4];
+        for (int u = 0; u < kAhead; ++u)
+            if (u < my_steps) load(u, raw[u]);
+        for (int s0 = 0; s0 < my_steps && ok; s0 += kAhead) {
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    if constexpr (HALF) hd[e] = __float_as_uint(v[p][e]);
-                    else split(v[p][e], hd[e], tl[e]);
-                }
-                if constexpr (!BACK) {
-                    const int off = (j >> 4) * (kBlock * 64) + n * 64 + ((((j >> 2) & 3) ^ ((n >> 1) & 3)) << 4);
-                    *reinterpret_cast<uint4*>(heads + off) = make_uint4(hd[0], hd[1], hd[2], hd[3]);
-                    if constexpr (!HALF) *reinterpret_cast<uint4*>(tails + off) = make_uint4(tl[0], tl[1], tl[2], tl[3]);
-                } else {
+            for (int u = 0; u < kAhead; ++u) {
+                const int s = s0 + u, buf = u & 1;  // kAhead is even
+                if (s >= my_steps || !ok) continue;
+                if (s >= 2) ok = mbar_wait(&bars.d_full[buf], ((s >> 1) - 1) & 1, TRC_DEVERR_WAIT_EMPTY);
+                uint8_t* heads = wbuf + buf * S::kW;
+                uint8_t* tails = heads + S::kPart;
+#pragma unroll
+                for (int p = 0; p < kPieces; ++p) {
+                    int n, j;
+                    place(p, n, j);
+                    float    v[4];
+                    uint32_t hd[4], tl[4];
+                    widen<W, 4>(raw[u][p], v);
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        const int m = n + e;
-                        const int off = (j >> 4) * (kBlock * 64) + m * 64 + ((((j >> 2) & 3) ^ ((m >> 1) & 3)) << 4) + 4 * (j & 3);
-                        *reinterpret_cast<uint32_t*>(heads + off) = hd[e];
-                        if constexpr (!HALF) *reinterpret_cast<uint32_t*>(tails + off) = tl[e];
+                        if constexpr (HALF) hd[e] = __float_as_uint(v[e]);
+                        else split(v[e], hd[e], tl[e]);
+                    }
+                    if constexpr (!BACK) {
+                        const int off = (j >> 4) * (kBlock * 64) + n * 64 + ((((j >> 2) & 3) ^ ((n >> 1) & 3)) << 4);
+                        *reinterpret_cast<uint4*>(heads + off) = make_uint4(hd[0], hd[1], hd[2], hd[3]);
+                        if constexpr (!HALF) *reinterpret_cast<uint4*>(tails + off) = make_uint4(tl[0], tl[1], tl[2], tl[3]);
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const int m = n + e;
+                            const int off = (j >> 4) * (kBlock * 64) + m * 64 + ((((j >> 2) & 3) ^ ((m >> 1) & 3)) << 4) + 4 * (j & 3);
+                            *reinterpret_cast<uint32_t*>(heads + off) = hd[e];
+                            if constexpr (!HALF) *reinterpret_cast<uint32_t*>(tails + off) = tl[e];
+                        }
                     }
                 }
+                fence_proxy_async_smem();
+                mbar_arrive(&bars.w_full[buf]);
+                if (s + kAhead < my_steps) load(s + kAhead, raw[u]);
             }
-            fence_proxy_async_smem();
-            mbar_arrive(&bars.w_full[buf]);
-            if (s + 1 < steps) load(s + 1);
         }
     } else if (lane == 0) {
         // ---------------- base's blocks and the MMAs
@@ -280,10 +294,16 @@ __global__ void __launch_bounds__(kTcThreads, 2) up_tc_kernel(const __grid_const
         };
         for (int b = 0; b < min(blocks, kSlots - 1); ++b) ok = ok && ask(b);
         for (int s = 0; s < steps && ok; ++s) {
+            // After a block's last MMAs, so that they run while d's block before it is still being added up: the slot of the
+            // block two before is free once that one has left.
             const int b = s / per;
-            // the slot of the block before this one is free once that block has left
-            if (s % per == 0 && b > 0 && b + kSlots - 2 < blocks) ok = ask(b + kSlots - 2);
-            if (n_ad == 0) continue;
+            auto ask_next = [&] {
+                if (s % per == per - 1 && b > 0 && b + kSlots - 2 < blocks) ok = ask(b + kSlots - 2);
+            };
+            if (n_ad == 0) {
+                ask_next();
+                continue;
+            }
             const int buf = s & 1;
             ok = ok && mbar_wait(&bars.w_full[buf], (s >> 1) & 1, TRC_DEVERR_WAIT_XFORM);
             if (s >= 2) ok = ok && mbar_wait(&bars.d_free[buf], ((s >> 1) - 1) & 1, TRC_DEVERR_WAIT_ACCFREE);
@@ -302,6 +322,7 @@ __global__ void __launch_bounds__(kTcThreads, 2) up_tc_kernel(const __grid_const
                 }
             umma_commit(&bars.d_full[buf]);
             issued = s + 1;
+            ask_next();
         }
         // nothing may still write to shared memory or TMEM when the CTA ends
         for (int b = max(0, asked - kSlots); b < asked; ++b) mbar_wait_drain(&bars.slot_full[b % kSlots], (b / kSlots) & 1);
@@ -350,12 +371,12 @@ int run(const Adapters& tab, const int32_t* ids, const CUtensorMap& base_map, co
     const int smem = TcSmem<W, LD>::kBytes;
     cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return cuda_fail(e);
-    // two waves of two CTAs for each SM (tiles at the borders between requests take longer than others), at least 8
+    // two waves of two CTAs for each SM (tiles at the borders between requests take longer than others), at least 2
     // blocks to a CTA
     const int64_t tiles = (rows + kTile - 1) / kTile;
     const int blocks = (n + kBlock - 1) / kBlock;
     const int64_t want = std::max<int64_t>(1, 4 * static_cast<int64_t>(std::max(1, sm_count_current())) / tiles);
-    const int per = static_cast<int>(std::max<int64_t>(std::min(blocks, 8), (blocks + want - 1) / want));
+    const int per = static_cast<int>(std::max<int64_t>(std::min(blocks, 2), (blocks + want - 1) / want));
     const int splits = (blocks + per - 1) / per;
     if (tiles * splits > INT32_MAX) return TRC_CUDA_EUNSUPPORTED;
     cudaLaunchConfig_t cfg{};
