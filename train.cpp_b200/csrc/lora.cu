@@ -137,18 +137,6 @@ struct TileIds {
     }
 };
 
-__device__ __forceinline__ float ld_cluster(uint32_t addr) {
-    float v;
-    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
-    return v;
-}
-
-__device__ __forceinline__ uint32_t cluster_nctarank() {
-    uint32_t r;
-    asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
-    return r;
-}
-
 constexpr int kWarps = 8, kThreads = 256;
 
 // Bytes of one stage of a warp's ring: the rows' part and the factor's (grad: h's), and the stages that keep two
@@ -166,13 +154,6 @@ struct UpRing {
     static constexpr int kCtas = JG <= 2 ? 2 : 1;
     static constexpr int kRoom = kCtas == 2 ? 112 * 1024 : 224 * 1024;
     static constexpr int kStages = kWarps * kStage * 4 <= kRoom ? 4 : kWarps * kStage * 3 <= kRoom ? 3 : 2;
-    static constexpr int kBytes = kWarps * kStages * kStage;
-};
-template <int MT>
-struct GradRing {
-    static constexpr int kX = 8 * 512, kH = 8 * 32 * 8 * MT, kStage = kX + kH;
-    static constexpr int kCtas = MT == 1 ? 2 : 1;
-    static constexpr int kStages = MT == 2 ? 3 : 2;
     static constexpr int kBytes = kWarps * kStages * kStage;
 };
 
@@ -809,171 +790,6 @@ __global__ void __launch_bounds__(kThreads, 2) few_kernel(const __grid_constant_
     }
 }
 
-// ------------------------------------------------------------------ gradients of the factors
-// out(j, k) (+)= sum over the adapter's rows t of h[t, j] x[t, k]; dA (h = g, x) is j-major, dB (h, x = dy)
-// k-major. The ranks are the 16-row side of the tensor core's tile, so a warp holds all ranks (up to 64)
-// of 32 columns and x is read once, straight into registers. Four warps of a CTA stand side by side in the
-// columns, two share the rows in turns of 32, and so do the CTAs of a cluster. Lane (c, q) takes the
-// columns 4c .. 4c + 3 (column 4c + i in tile i) and the ranks 2 MT c .. (the two halves of the MT tiles in turn).
-struct GradSide {
-    Rows         x;
-    const float* h;
-    int32_t      k_len;
-    int32_t      strips;  // of 128 columns
-};
-
-template <int MT, bool VEC>
-__global__ void __launch_bounds__(kThreads, GradRing<MT>::kCtas) grad_kernel(const __grid_constant__ Adapters tab, const int32_t* ids,
-                                                        const __grid_constant__ GradSide side_a,
-                                                        const __grid_constant__ GradSide side_b, int64_t rows, int ld,
-                                                        int accumulate) {
-    constexpr int kR = 16 * MT;
-    extern __shared__ __align__(16) char grad_smem[];  // the warps' rings, then sums of [kR][128 + 4]
-    const int  warp = threadIdx.x >> 5, lane = threadIdx.x & 31, c = lane >> 2, q = lane & 3;
-    const int  ranks = static_cast<int>(cluster_nctarank()), rank = static_cast<int>(cluster_ctarank());
-    int        strip = static_cast<int>(blockIdx.x) / ranks;
-    const bool is_b = strip >= side_a.strips;
-    const GradSide& S = is_b ? side_b : side_a;
-    if (is_b) strip -= side_a.strips;
-    const Adapter& A = tab.ad[blockIdx.z];
-    float* out = is_b ? A.db : A.da;
-    const int j0 = blockIdx.y * kR, r = A.rank;
-    grid_wait();
-    if (out == nullptr || j0 >= r) return;  // the whole cluster
-    const int col = strip * 128 + (warp & 3) * 32 + 4 * c;
-
-    // Steps of 32 rows t0 + q + 4 e; a step without a row of this adapter is passed over.
-    float acc[MT][4][4] = {};
-    const int64_t  steps = (rows + 31) / 32, hop = 2 * ranks;
-    using Ring = GradRing<MT>;
-    constexpr int  kStages = Ring::kStages, kPiece = MT == 1 ? 8 : 16, kPieces = MT == 4 ? 2 : 1;  // of a row's 2 MT ranks
-    const uint32_t ring = smem_u32(grad_smem) + warp * (kStages * Ring::kStage);
-    int64_t  ahead = rank + static_cast<int64_t>(warp >> 2) * ranks - hop;  // the step fetched last
-    uint32_t at_rows[kStages] = {};  // the rows of the steps in the ring, the oldest step first
-    auto fetch = [&](int stage) {
-        uint32_t mine = 0;
-        while (mine == 0 && ahead + hop < steps) {
-            ahead += hop;
-            const int64_t t = ahead * 32 + lane;
-            mine = __ballot_sync(0xFFFFFFFFu, t < rows && adapter_of(ids, t, tab.n) == static_cast<int>(blockIdx.z));
-        }
-        at_rows[kStages - 1] = mine;
-        if (mine != 0) {
-            const uint32_t place = ring + stage * Ring::kStage;
-            const int64_t  t = ahead * 32 + q;
-            const char*    xr = S.x.row<VEC>(t);
-            const float*   hr = S.h + t * ld + j0 + 2 * MT * c;
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const bool live = (mine >> (q + 4 * e)) & 1u;
-                if constexpr (!VEC) xr = live ? S.x.row<VEC>(t + 4 * e) : S.x.data;
-                ring_x4<VEC>(place + e * 512 + lane * 16, xr, live, S.x.nb0, col, S.k_len);
-                if constexpr (VEC) xr += 16ll * S.x.step;
-#pragma unroll
-                for (int i = 0; i < kPieces; ++i)
-                    ring_w<kPiece>(place + Ring::kX + ((e * kPieces + i) * 32 + lane) * kPiece, hr + 4 * i,
-                                   live && j0 + 2 * MT * c + 4 * i < ld);
-                hr += 4 * ld;
-            }
-        }
-        ring_commit();
-    };
-    auto shift = [&]() {
-#pragma unroll
-        for (int p = 0; p + 1 < kStages; ++p) at_rows[p] = at_rows[p + 1];
-    };
-#pragma unroll
-    for (int p = 0; p < kStages - 1; ++p) {
-        shift();
-        fetch(p);
-    }
-    for (int stage = 0;; stage = stage + 1 == kStages ? 0 : stage + 1) {
-        shift();
-        fetch(stage == 0 ? kStages - 1 : stage - 1);
-        if (at_rows[0] == 0) break;  // nothing follows
-        ring_wait<kStages - 1>();
-        const uint32_t place = ring + stage * Ring::kStage;
-        float d[MT][4][4] = {};
-#pragma unroll
-        for (int s = 0; s < 2; ++s) {
-            float hv[4][2 * MT];
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-#pragma unroll
-                for (int i = 0; i < kPieces; ++i) {
-                    float p[kPiece / 4];
-                    ring_take_w<float, kPiece / 4>(place + Ring::kX + (((4 * s + e) * kPieces + i) * 32 + lane) * kPiece, p);
-#pragma unroll
-                    for (int j = 0; j < kPiece / 4; ++j) hv[e][4 * i + j] = p[j];
-                }
-            uint32_t bh[2][4][2], bt[2][4][2];  // [8 rows][tile]
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                float xv[4];
-                ring_take(place + (4 * s + e) * 512 + lane * 16, xv);
-#pragma unroll
-                for (int n = 0; n < 4; ++n) split(xv[n], bh[e >> 1][n][e & 1], bt[e >> 1][n][e & 1]);
-            }
-#pragma unroll
-            for (int m = 0; m < MT; ++m) {
-                uint32_t ah[2][4], at[2][4];
-#pragma unroll
-                for (int u = 0; u < 2; ++u)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e)  // a[e]: half e & 1, row q + 4 (e >> 1) of the 8
-                        split(hv[2 * u + (e >> 1)][2 * m + (e & 1)], ah[u][e], at[u][e]);
-#pragma unroll
-                for (int n = 0; n < 4; ++n) {
-                    mma_split<false>(d[m][n], ah[0], at[0], bh[0][n], bt[0][n]);
-                    mma_split<false>(d[m][n], ah[1], at[1], bh[1][n], bt[1][n]);
-                }
-            }
-        }
-#pragma unroll
-        for (int m = 0; m < MT; ++m)
-#pragma unroll
-            for (int n = 0; n < 4; ++n)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) acc[m][n][e] += d[m][n][e];
-    }
-    ring_wait<0>();
-    __syncthreads();  // the sums take the rings' place
-    float (*sum)[128 + 4] = reinterpret_cast<float (*)[128 + 4]>(grad_smem);
-    // the two row halves of the CTA, then the cluster
-    const int col0 = (warp & 3) * 32;
-#pragma unroll
-    for (int half = 1; half >= 0; --half) {
-        if ((warp >> 2) == half) {
-#pragma unroll
-            for (int m = 0; m < MT; ++m)
-#pragma unroll
-                for (int n = 0; n < 4; ++n)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        float* s = &sum[2 * MT * c + 2 * m + (e >> 1)][col0 + 4 * (2 * q + (e & 1)) + n];
-                        *s = half == 1 ? acc[m][n][e] : *s + acc[m][n][e];
-                    }
-        }
-        __syncthreads();
-    }
-    if (ranks > 1) cluster_sync();
-    for (int i = rank * kThreads + threadIdx.x; i < kR * 128; i += kThreads * ranks) {
-        // neighbours in memory are neighbours in the lanes
-        const int j = is_b ? i % kR : i / 128, k = is_b ? i / kR : i % 128;
-        if (j0 + j >= r || strip * 128 + k >= S.k_len) continue;
-        float s = 0.0f;
-        if (ranks > 1) {
-            for (int v = 0; v < ranks; ++v) s += ld_cluster(mapa_shared(&sum[j][k], v));
-        } else {
-            s = sum[j][k];
-        }
-        const int64_t kk = strip * 128 + k;
-        float* o = out + (is_b ? kk * r + j0 + j : static_cast<int64_t>(j0 + j) * S.k_len + kk);
-        *o = accumulate ? *o + s : s;
-    }
-    if (ranks > 1) cluster_sync();
-}
-
 constexpr int64_t kMaxLen = int64_t(1) << 30;  // rows, K and N of a call
 
 // TRC_CUDA_OK if the adapters are valid for trc_cuda_lora*; *ld = the row length of h.
@@ -1240,35 +1056,6 @@ int up(int type, const Adapters& tab, const int32_t* ids, const trc_cuda_view* b
     return up_of<BACK, __nv_bfloat16>(tab, ids, rb, rd, vec, rows, n, h, ld, s);
 }
 
-// Both factors' gradients; the kernel before it on the stream has to be down's.
-int grad(const Adapters& tab, const int32_t* ids, const trc_cuda_view* x, const trc_cuda_view* dy, int64_t rows, const float* g,
-         const float* h, int ld, int accumulate, cudaStream_t s) {
-    bool any_a = false, any_b = false;
-    for (int i = 0; i < tab.n; ++i) {
-        any_a = any_a || tab.ad[i].da != nullptr;
-        any_b = any_b || tab.ad[i].db != nullptr;
-    }
-    if (!any_a && !any_b) return TRC_CUDA_OK;
-    GradSide a{rows_of(x), g, static_cast<int32_t>(x->ne[0]), 0};
-    GradSide b{rows_of(dy), h, static_cast<int32_t>(dy->ne[0]), 0};
-    if (any_a) a.strips = (a.k_len + 127) / 128;
-    if (any_b) b.strips = (b.k_len + 127) / 128;
-    const int mt = std::min(ld / 16, 3) == 3 ? 4 : ld / 16;
-    const unsigned chunks = static_cast<unsigned>((ld + 16 * mt - 1) / (16 * mt));
-    const int64_t strips = a.strips + b.strips;
-    const int cluster = std::min(power_for(strips * tab.n * chunks, full_grid() / (mt == 1 ? 1 : 2), 8), power_for(1, (rows + 63) / 64, 8));
-    const bool vec = vec_rows(x) && vec_rows(dy);
-    const void* kernel = mt == 1   ? (vec ? reinterpret_cast<const void*>(&grad_kernel<1, true>) : reinterpret_cast<const void*>(&grad_kernel<1, false>))
-                         : mt == 2 ? (vec ? reinterpret_cast<const void*>(&grad_kernel<2, true>) : reinterpret_cast<const void*>(&grad_kernel<2, false>))
-                                   : (vec ? reinterpret_cast<const void*>(&grad_kernel<4, true>) : reinterpret_cast<const void*>(&grad_kernel<4, false>));
-    const size_t smem = mt == 1 ? GradRing<1>::kBytes : mt == 2 ? GradRing<2>::kBytes : GradRing<4>::kBytes;
-    const int st = allow_smem(kernel, smem);
-    if (st != TRC_CUDA_OK) return st;
-    void* args[] = {const_cast<Adapters*>(&tab), &ids, &a, &b, &rows, &ld, &accumulate};
-    return launch(kernel, dim3(static_cast<unsigned>(strips * cluster), chunks, static_cast<unsigned>(tab.n)), cluster, smem,
-                  false, args, s);
-}
-
 }  // namespace
 
 }  // namespace trc
@@ -1355,7 +1142,7 @@ int trc_cuda_lora_back(int type, const trc_cuda_lora_adapter* adapters, int n_ad
         if ((st = down<true>(type, tab, ids, dy, rows, g, l, s)) != TRC_CUDA_OK) return st;
         if (dx != nullptr && (st = up<true>(type, tab, ids, base, dx, rows, g, l, s)) != TRC_CUDA_OK) return st;
     }
-    return grad(tab, ids, x, dy, rows, g, h, l, accumulate, s);
+    return grad_tc(tab, ids, *x, rows_of(x), *dy, rows_of(dy), rows, g, h, l, accumulate, s);
 }
 
 }  // extern "C"

@@ -107,6 +107,18 @@ __device__ __forceinline__ void load_w(const W* p, int have, float (&w)[N]) {
 __device__ __forceinline__ void grid_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ __forceinline__ void grid_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
+__device__ __forceinline__ float ld_cluster(uint32_t addr) {
+    float v;
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+    return v;
+}
+
+__device__ __forceinline__ uint32_t cluster_nctarank() {
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
+    return r;
+}
+
 inline bool aligned_to(const void* p, uint64_t bytes) { return (reinterpret_cast<uint64_t>(p) & (bytes - 1)) == 0; }
 
 inline int64_t item_bytes(int type) { return type == TRC_CUDA_TYPE_F32 ? 4 : 2; }
@@ -115,6 +127,10 @@ inline int64_t item_bytes(int type) { return type == TRC_CUDA_TYPE_F32 ? 4 : 2; 
 // 64. TRC_CUDA_EUNSUPPORTED, with nothing launched, where it does not apply. back: W is A^T, else B.
 int up_tc(bool back, int type, const Adapters& tab, const int32_t* ids, const trc_cuda_view* base, const trc_cuda_view* d,
           int64_t rows, const float* h, int ld, cudaStream_t s);
+
+// dA (from x and g) and dB (from dy and h) of every adapter that wants them (lora_tc.cu).
+int grad_tc(const Adapters& tab, const int32_t* ids, const trc_cuda_view& x, const Rows& x_rows, const trc_cuda_view& dy,
+            const Rows& dy_rows, int64_t rows, const float* g, const float* h, int ld, int accumulate, cudaStream_t s);
 
 }  // namespace lora
 }  // namespace trc

@@ -143,6 +143,7 @@ __global__ void __launch_bounds__(kTcThreads, 2) up_tc_kernel(const __grid_const
                 ok = ok && mbar_wait(&bars.d_full[buf], (s >> 1) & 1, TRC_DEVERR_WAIT_ACCUM);
                 tc_fence_after();
                 uint32_t v[32];
+                __syncwarp();
                 tmem_ld_32x32b_x32(tmem + (static_cast<uint32_t>(warp * 32) << 16) + 2 * LD + buf * kBlock, v);
                 tmem_ld_wait();
                 tc_fence_before();
@@ -195,6 +196,7 @@ __global__ void __launch_bounds__(kTcThreads, 2) up_tc_kernel(const __grid_const
                     split(v.z, head[4 * u + 2], tail[4 * u + 2]);
                     split(v.w, head[4 * u + 3], tail[4 * u + 3]);
                 }
+                __syncwarp();
                 tmem_st_32x32b_x16(lane_base + 16 * g, head);
                 tmem_st_32x32b_x16(lane_base + LD + 16 * g, tail);
             }
@@ -335,6 +337,305 @@ __global__ void __launch_bounds__(kTcThreads, 2) up_tc_kernel(const __grid_const
     if (warp == 8) tmem_dealloc(tmem, S::kCols);
 }
 
+// ------------------------------------------------------------------ gradients of the factors
+// out(j, k) (+)= sum over the adapter's rows t of h[t, j] x[t, k]; dA (h = g, x) is j-major, dB (h, x = dy)
+// k-major. The MMA's M are 128 columns of x, its N the ranks (up to 64 at a time), its K the rows. A thread of four
+// warps owns a column: it loads 32 rows of it (a warp reads whole lines, whatever the strides between rows), splits them and puts
+// them into its lane of TMEM, the first operand, so x is read once and never staged. Four other warps build the
+// ranks' rows in shared memory (transposed, K-major, 64-byte swizzle) and add the sums of every 64 rows up in
+// fp32, because the tensor core's own sums lose a little at every product (7e-8 of the result for 8 rows in a chain).
+// The CTAs of a cluster share the steps of 32 rows in turns and join their sums in order.
+constexpr int kGradRows = 32, kGradPromote = 2;  // rows of a step, steps between two additions in fp32
+
+struct GradSide {
+    Rows         x;
+    const float* h;
+    int32_t      k_len;
+    int32_t      strips;  // of 128 columns
+};
+
+struct GradBars {
+    uint64_t a_full[2], b_full[2];  // a step's operands are there (128 arrivals each)
+    uint64_t ab_free[2];            // and read (commit)
+    uint64_t d_full[2];             // the sums of some steps are complete (commit)
+    uint64_t d_free[2];             // and in registers (128 arrivals)
+};
+
+template <int LD>
+struct GradSmem {
+    static constexpr int kPart = LD * kGradRows * 4, kBuf = 2 * kPart;  // heads, tails
+    static constexpr int kSum = LD * (kTile + 4) * 4;
+    static constexpr int kBytes = (2 * kBuf > kSum ? 2 * kBuf : kSum) + 1024;
+    static constexpr uint32_t kD = 4 * kGradRows, kCols = 4 * kGradRows + 2 * LD <= 128 ? 128 : 256;
+};
+
+template <int LD>
+__global__ void __launch_bounds__(kTcThreads, 2) grad_tc_kernel(const __grid_constant__ Adapters tab, const int32_t* ids,
+                                                                const __grid_constant__ GradSide side_a,
+                                                                const __grid_constant__ GradSide side_b, int64_t rows, int ld,
+                                                                int accumulate) {
+    using S = GradSmem<LD>;
+    extern __shared__ uint8_t tc_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(tc_raw) + 1023) & ~uintptr_t(1023));
+    __shared__ __align__(8) GradBars bars;
+    __shared__ uint32_t tmem_slot;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int ranks = static_cast<int>(cluster_nctarank()), rank = static_cast<int>(cluster_ctarank());
+    int        strip = static_cast<int>(blockIdx.x) / ranks;
+    const bool is_b = strip >= side_a.strips;
+    const GradSide& G = is_b ? side_b : side_a;
+    if (is_b) strip -= side_a.strips;
+    const int      ad = static_cast<int>(blockIdx.z);
+    const Adapter& A = tab.ad[ad];
+    float*         out = is_b ? A.db : A.da;
+    const int      j0 = blockIdx.y * LD, r = A.rank;
+    if (out == nullptr || j0 >= r) return;  // the whole cluster
+
+    if (threadIdx.x == 256) {
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&bars.a_full[i], 128);
+            mbar_init(&bars.b_full[i], 128);
+            mbar_init(&bars.ab_free[i], 1);
+            mbar_init(&bars.d_full[i], 1);
+            mbar_init(&bars.d_free[i], 128);
+        }
+        fence_barrier_init();
+    }
+    if (warp == 8) {
+        tmem_alloc(&tmem_slot, S::kCols);
+        tmem_relinquish();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = tmem_slot;
+
+    // This CTA's steps: those of its turn that have a row of the adapter. Every warp goes through them for itself.
+    const int64_t all = (rows + kGradRows - 1) / kGradRows;
+    int64_t  at = rank - ranks;
+    auto next = [&](uint32_t& mine) {  // the next step's number, its rows in `mine`; mine = 0: there is none
+        mine = 0;
+        while (mine == 0 && at + ranks < all) {
+            at += ranks;
+            const int64_t t = at * kGradRows + lane;
+            mine = __ballot_sync(0xFFFFFFFFu, t < rows && adapter_of(ids, t, tab.n) == ad);
+        }
+        return at;
+    };
+    bool ok = true;
+    float (*sum)[kTile + 4] = reinterpret_cast<float (*)[kTile + 4]>(smem);  // in the place of the ranks' rows
+
+    if (warp < 4) {
+        const int  col = strip * kTile + static_cast<int>(threadIdx.x);
+        const bool inside = col < G.k_len;
+        const uint32_t lane_base = tmem + (static_cast<uint32_t>(warp * 32) << 16);
+        float    x[kGradRows];
+        uint32_t mine;
+        auto load = [&](int64_t step, uint32_t mine) {
+            if (G.x.step >= 0) {
+                const char* p = G.x.data + 4 * (step * kGradRows * G.x.step) + col * G.x.nb0;
+#pragma unroll
+                for (int e = 0; e < kGradRows; ++e) {
+                    x[e] = inside && ((mine >> e) & 1u) ? *reinterpret_cast<const float*>(p) : 0.0f;
+                    p += 4ll * G.x.step;
+                }
+            } else {
+#pragma unroll
+                for (int e = 0; e < kGradRows; ++e)
+                    x[e] = inside && ((mine >> e) & 1u)
+                               ? *reinterpret_cast<const float*>(G.x.row<false>(step * kGradRows + e) + col * G.x.nb0) : 0.0f;
+            }
+        };
+        int64_t step = next(mine);
+        if (mine != 0) load(step, mine);
+        for (int s = 0; mine != 0 && ok; ++s) {
+            const int buf = s & 1;
+            if (s >= 2) ok = mbar_wait(&bars.ab_free[buf], ((s >> 1) - 1) & 1, TRC_DEVERR_WAIT_EMPTY);
+            tc_fence_after();
+            const uint32_t heads = lane_base + buf * 2 * kGradRows;
+#pragma unroll
+            for (int g = 0; g < 2; ++g) {
+                uint32_t hd[16], tl[16];
+#pragma unroll
+                for (int e = 0; e < 16; ++e) split(x[16 * g + e], hd[e], tl[e]);
+                __syncwarp();
+                tmem_st_32x32b_x16(heads + 16 * g, hd);
+                tmem_st_32x32b_x16(heads + kGradRows + 16 * g, tl);
+            }
+            step = next(mine);
+            if (mine != 0) load(step, mine);
+            __syncwarp();
+            tmem_st_wait();
+            tc_fence_before();
+            mbar_arrive(&bars.a_full[buf]);
+        }
+    } else if (warp < 8) {
+        const int tid = threadIdx.x - 128;
+        float acc[LD];  // this lane's column, all ranks
+#pragma unroll
+        for (int j = 0; j < LD; ++j) acc[j] = 0.0f;
+        constexpr int kPieces = kGradRows * LD / 4 / 128;  // four ranks of a row each
+        float4   v[kPieces];
+        uint32_t mine;
+        auto place = [&](int p, int& t, int& j) {
+            const int i = tid + 128 * p;
+            t = (i & 7) + 8 * (i / (2 * LD));
+            j = 4 * ((i >> 3) % (LD / 4));
+        };
+        auto load = [&](int64_t step, uint32_t mine) {
+#pragma unroll
+            for (int p = 0; p < kPieces; ++p) {
+                int t, j;
+                place(p, t, j);
+                v[p] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                if (((mine >> t) & 1u) && j0 + j < ld) v[p] = *reinterpret_cast<const float4*>(G.h + (step * kGradRows + t) * ld + j0 + j);
+            }
+        };
+        auto add = [&](int q) {  // the sums of steps kGradPromote * q ..
+            const int buf = q & 1;
+            ok = ok && mbar_wait(&bars.d_full[buf], (q >> 1) & 1, TRC_DEVERR_WAIT_ACCUM);
+            tc_fence_after();
+            __syncwarp();
+#pragma unroll
+            for (int g = 0; g < LD / 16; ++g) {
+                uint32_t d[16];
+                tmem_ld_32x32b_x16(tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16) + S::kD + buf * LD + 16 * g, d);
+                tmem_ld_wait();
+#pragma unroll
+                for (int e = 0; e < 16; ++e) acc[16 * g + e] += __uint_as_float(d[e]);
+            }
+            tc_fence_before();
+            mbar_arrive(&bars.d_free[buf]);
+        };
+        int64_t step = next(mine);
+        if (mine != 0) load(step, mine);
+        int s = 0;
+        for (; mine != 0 && ok; ++s) {
+            const int buf = s & 1;
+            if (s >= 2) ok = mbar_wait(&bars.ab_free[buf], ((s >> 1) - 1) & 1, TRC_DEVERR_WAIT_EMPTY);
+            uint8_t* heads = smem + buf * S::kBuf;
+#pragma unroll
+            for (int p = 0; p < kPieces; ++p) {
+                int t, j;
+                place(p, t, j);
+                const float w[4] = {v[p].x, v[p].y, v[p].z, v[p].w};
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    uint32_t hd, tl;
+                    split(w[e], hd, tl);
+                    const int m = j + e;
+                    const int off = (t >> 4) * (LD * 64) + m * 64 + ((((t >> 2) & 3) ^ ((m >> 1) & 3)) << 4) + 4 * (t & 3);
+                    *reinterpret_cast<uint32_t*>(heads + off) = hd;
+                    *reinterpret_cast<uint32_t*>(heads + S::kPart + off) = tl;
+                }
+            }
+            fence_proxy_async_smem();
+            mbar_arrive(&bars.b_full[buf]);
+            step = next(mine);
+            if (mine != 0) load(step, mine);
+            // while this group of steps runs, the one before
+            if (s % kGradPromote == kGradPromote - 1 && s >= kGradPromote) add(s / kGradPromote - 1);
+        }
+        // the groups that are left: the loop has added group q when it built the last step of group q + 1
+        const int groups = (s + kGradPromote - 1) / kGradPromote, added = s >= 2 * kGradPromote ? s / kGradPromote - 1 : 0;
+        for (int q = added; q < groups && ok; ++q) add(q);
+        // every MMA of this CTA is complete: nothing reads the ranks' rows any more
+#pragma unroll
+        for (int j = 0; j < LD; ++j) sum[j][tid] = acc[j];
+    } else {
+        const uint32_t idesc = make_idesc_tf32(kTile, LD, 0, 0);
+        const uint32_t base = smem_u32(smem);
+        uint32_t mine;
+        next(mine);
+        int s = 0;
+        for (; mine != 0 && ok; ++s) {
+            uint32_t following;
+            next(following);
+            const int buf = s & 1, q = s / kGradPromote, part = s % kGradPromote;
+            if (lane == 0) {
+                ok = mbar_wait(&bars.a_full[buf], (s >> 1) & 1, TRC_DEVERR_WAIT_XFORM) &&
+                     mbar_wait(&bars.b_full[buf], (s >> 1) & 1, TRC_DEVERR_WAIT_XFORM);
+                if (part == 0 && q >= 2) ok = ok && mbar_wait(&bars.d_free[q & 1], ((q >> 1) - 1) & 1, TRC_DEVERR_WAIT_ACCFREE);
+                if (ok) {
+                    tc_fence_after();
+                    const uint32_t dst = tmem + S::kD + (q & 1) * LD, a0 = tmem + buf * 2 * kGradRows, b0 = base + buf * S::kBuf;
+#pragma unroll
+                    for (int k = 0; k < kGradRows / 8; ++k) {
+                        const uint32_t off = (k >> 1) * (LD * 64) + (k & 1) * 32;
+                        const uint64_t bh = make_smem_desc(b0 + off, 16, 512, 4), bt = make_smem_desc(b0 + S::kPart + off, 16, 512, 4);
+                        umma_tf32_ts(dst, a0 + kGradRows + 8 * k, bh, idesc, part + k > 0);
+                        umma_tf32_ts(dst, a0 + 8 * k, bt, idesc, 1);
+                        umma_tf32_ts(dst, a0 + 8 * k, bh, idesc, 1);
+                    }
+                    umma_commit(&bars.ab_free[buf]);
+                    if (part == kGradPromote - 1 || following == 0) umma_commit(&bars.d_full[q & 1]);
+                }
+            }
+            ok = __shfl_sync(0xFFFFFFFFu, ok ? 1 : 0, 0) != 0;
+            mine = following;
+        }
+        // nothing may still read shared memory or TMEM when they are used anew
+        if (lane == 0)
+            for (int p = max(0, s - 2); p < (ok ? s : s - 1); ++p) mbar_wait_drain(&bars.ab_free[p & 1], (p >> 1) & 1);
+    }
+    __syncwarp();
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    if (warp == 8) tmem_dealloc(tmem, S::kCols);
+
+    // this CTA's sums, then the cluster's
+    if (ranks > 1) cluster_sync();
+    for (int i = rank * kTcThreads + threadIdx.x; i < LD * kTile; i += kTcThreads * ranks) {
+        // neighbours in memory are neighbours in the lanes
+        const int j = is_b ? i % LD : i / kTile, k = is_b ? i / LD : i % kTile;
+        if (j0 + j >= r || strip * kTile + k >= G.k_len) continue;
+        float total = 0.0f;
+        if (ranks > 1) {
+            for (int v = 0; v < ranks; ++v) total += ld_cluster(mapa_shared(&sum[j][k], v));
+        } else {
+            total = sum[j][k];
+        }
+        const int64_t kk = strip * kTile + k;
+        float* o = out + (is_b ? kk * r + j0 + j : static_cast<int64_t>(j0 + j) * G.k_len + kk);
+        *o = accumulate ? *o + total : total;
+    }
+    if (ranks > 1) cluster_sync();
+}
+
+template <int LD>
+int run_grad(const Adapters& tab, const int32_t* ids, const GradSide& a, const GradSide& b, int64_t rows, int ld, int accumulate,
+             cudaStream_t s) {
+    auto kernel = &grad_tc_kernel<LD>;
+    const int smem = GradSmem<LD>::kBytes;
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) return cuda_fail(e);
+    const int64_t chunks = (ld + LD - 1) / LD, units = (a.strips + b.strips) * chunks * tab.n;
+    // the rows of a strip go to 1 - 8 CTAs: one wave of two CTAs for each SM, at least four steps for each
+    const int64_t room = 2 * static_cast<int64_t>(std::max(1, sm_count_current())), steps = (rows + kGradRows - 1) / kGradRows;
+    unsigned cluster = 1;
+    while (cluster < 8 && 2 * cluster * units <= room && 8 * cluster <= steps) cluster *= 2;
+    if ((a.strips + b.strips) * static_cast<int64_t>(cluster) > INT32_MAX) return TRC_CUDA_EUNSUPPORTED;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(static_cast<unsigned>((a.strips + b.strips) * cluster), static_cast<unsigned>(chunks), static_cast<unsigned>(tab.n));
+    cfg.blockDim = dim3(kTcThreads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = cluster;
+    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    e = cudaLaunchKernelEx(&cfg, kernel, tab, ids, a, b, rows, ld, accumulate);
+    if (e != cudaSuccess) {
+        cudaGetLastError();
+        return cuda_fail(e);
+    }
+    note_launch();
+    return TRC_CUDA_OK;
+}
+
 PFN_cuTensorMapEncodeTiled_v12000 encoder() {
     static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
     static std::once_flag once;
@@ -427,6 +728,21 @@ int up_tc(bool back, int type, const Adapters& tab, const int32_t* ids, const tr
     if (type == TRC_CUDA_TYPE_F32) return run_dir<float>(back, tab, ids, base_map, d_map, add, rows, n, h, ld, s);
     if (type == TRC_CUDA_TYPE_F16) return run_dir<__half>(back, tab, ids, base_map, d_map, add, rows, n, h, ld, s);
     return run_dir<__nv_bfloat16>(back, tab, ids, base_map, d_map, add, rows, n, h, ld, s);
+}
+
+int grad_tc(const Adapters& tab, const int32_t* ids, const trc_cuda_view& x, const Rows& x_rows, const trc_cuda_view& dy,
+            const Rows& dy_rows, int64_t rows, const float* g, const float* h, int ld, int accumulate, cudaStream_t s) {
+    bool any_a = false, any_b = false;
+    for (int i = 0; i < tab.n; ++i) {
+        any_a = any_a || tab.ad[i].da != nullptr;
+        any_b = any_b || tab.ad[i].db != nullptr;
+    }
+    if (!any_a && !any_b) return TRC_CUDA_OK;
+    const GradSide a{x_rows, g, static_cast<int32_t>(x.ne[0]), any_a ? static_cast<int32_t>((x.ne[0] + kTile - 1) / kTile) : 0};
+    const GradSide b{dy_rows, h, static_cast<int32_t>(dy.ne[0]), any_b ? static_cast<int32_t>((dy.ne[0] + kTile - 1) / kTile) : 0};
+    if (ld == 16) return run_grad<16>(tab, ids, a, b, rows, ld, accumulate, s);
+    if (ld == 32) return run_grad<32>(tab, ids, a, b, rows, ld, accumulate, s);
+    return run_grad<64>(tab, ids, a, b, rows, ld, accumulate, s);
 }
 
 }  // namespace lora
