@@ -1142,7 +1142,7 @@ int trc_cuda_lora_back(int type, const trc_cuda_lora_adapter* adapters, int n_ad
         if ((st = down<true>(type, tab, ids, dy, rows, g, l, s)) != TRC_CUDA_OK) return st;
         if (dx != nullptr && (st = up<true>(type, tab, ids, base, dx, rows, g, l, s)) != TRC_CUDA_OK) return st;
     }
-    return grad_tc(tab, ids, *x, rows_of(x), *dy, rows_of(dy), rows, g, h, l, accumulate, s);
+    return grad_tc(tab, ids, *x, rows_of(x), *dy, rows_of(dy), vec_rows(x) && vec_rows(dy), rows, g, h, l, accumulate, s);
 }
 
 }  // extern "C"

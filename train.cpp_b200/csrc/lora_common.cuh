@@ -128,9 +128,10 @@ inline int64_t item_bytes(int type) { return type == TRC_CUDA_TYPE_F32 ? 4 : 2; 
 int up_tc(bool back, int type, const Adapters& tab, const int32_t* ids, const trc_cuda_view* base, const trc_cuda_view* d,
           int64_t rows, const float* h, int ld, cudaStream_t s);
 
-// dA (from x and g) and dB (from dy and h) of every adapter that wants them (lora_tc.cu).
+// dA (from x and g) and dB (from dy and h) of every adapter that wants them (lora_tc.cu). vec: rows of floats in whole
+// 16-byte pieces on both sides.
 int grad_tc(const Adapters& tab, const int32_t* ids, const trc_cuda_view& x, const Rows& x_rows, const trc_cuda_view& dy,
-            const Rows& dy_rows, int64_t rows, const float* g, const float* h, int ld, int accumulate, cudaStream_t s);
+            const Rows& dy_rows, bool vec, int64_t rows, const float* g, const float* h, int ld, int accumulate, cudaStream_t s);
 
 }  // namespace lora
 }  // namespace trc

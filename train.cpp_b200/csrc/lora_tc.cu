@@ -340,10 +340,11 @@ __global__ void __launch_bounds__(kTcThreads, 2) up_tc_kernel(const __grid_const
 // ------------------------------------------------------------------ gradients of the factors
 // out(j, k) (+)= sum over the adapter's rows t of h[t, j] x[t, k]; dA (h = g, x) is j-major, dB (h, x = dy)
 // k-major. The MMA's M are 128 columns of x, its N the ranks (up to 64 at a time), its K the rows. A thread of four
-// warps owns a column: it loads 32 rows of it (a warp reads whole lines, whatever the strides between rows), splits them and puts
-// them into its lane of TMEM, the first operand, so x is read once and never staged. Four other warps build the
-// ranks' rows in shared memory (transposed, K-major, 64-byte swizzle) and add the sums of every 64 rows up in
-// fp32, because the tensor core's own sums lose a little at every product (7e-8 of the result for 8 rows in a chain).
+// warps owns a column: it takes 32 rows of it, splits them and puts them into its lane of TMEM, the first operand. Four
+// other warps build the ranks' rows in shared memory (transposed, K-major, 64-byte swizzle) and add the sums of every 64
+// rows up in fp32, because the tensor core's own sums lose a little at every product (7e-8 of the result for 8 rows in a chain).
+// What a warp takes (its 32 columns of x, its pieces of h) runs through a ring of asynchronous copies of its own, two to
+// three steps ahead: with loads one step ahead, in registers, a step took a DRAM round trip, 1.9 us.
 // The CTAs of a cluster share the steps of 32 rows in turns and join their sums in order.
 constexpr int kGradRows = 32, kGradPromote = 2;  // rows of a step, steps between two additions in fp32
 
@@ -364,12 +365,28 @@ struct GradBars {
 template <int LD>
 struct GradSmem {
     static constexpr int kPart = LD * kGradRows * 4, kBuf = 2 * kPart;  // heads, tails
+    static constexpr int kStages = LD == 64 ? 3 : 4;
+    static constexpr int kX = kGradRows * kTile * 4, kH = kGradRows * LD * 4;  // a stage of the rings
+    static constexpr int kXAt = 2 * kBuf, kHAt = kXAt + kStages * kX, kAll = kHAt + kStages * kH;
     static constexpr int kSum = LD * (kTile + 4) * 4;
-    static constexpr int kBytes = (2 * kBuf > kSum ? 2 * kBuf : kSum) + 1024;
+    static constexpr int kBytes = (kAll > kSum ? kAll : kSum) + 1024;
+    static_assert(kBytes <= 112 * 1024, "two CTAs on an SM");
     static constexpr uint32_t kD = 4 * kGradRows, kCols = 4 * kGradRows + 2 * LD <= 128 ? 128 : 256;
 };
 
-template <int LD>
+template <int BYTES>
+__device__ __forceinline__ void copy_async(uint32_t place, const void* from, bool live) {
+    if constexpr (BYTES == 16)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(place), "l"(from), "r"(live ? 16 : 0) : "memory");
+    else
+        asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(place), "l"(from), "n"(BYTES), "r"(live ? BYTES : 0) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+// VEC: both sides' rows are evenly spaced, whole in 16-byte pieces and start at multiples of 16 bytes.
+template <int LD, bool VEC>
 __global__ void __launch_bounds__(kTcThreads, 2) grad_tc_kernel(const __grid_constant__ Adapters tab, const int32_t* ids,
                                                                 const __grid_constant__ GradSide side_a,
                                                                 const __grid_constant__ GradSide side_b, int64_t rows, int ld,
@@ -423,72 +440,89 @@ __global__ void __launch_bounds__(kTcThreads, 2) grad_tc_kernel(const __grid_con
         return at;
     };
     bool ok = true;
-    float (*sum)[kTile + 4] = reinterpret_cast<float (*)[kTile + 4]>(smem);  // in the place of the ranks' rows
+    float (*sum)[kTile + 4] = reinterpret_cast<float (*)[kTile + 4]>(smem);  // in the place of all that
+    constexpr int kStages = S::kStages;
+    uint32_t ahead[kStages] = {};  // the rows of the steps in a warp's ring, the oldest step first
+    auto turn = [&](auto&& fetch, int stage) {  // one more step into the ring
+        uint32_t mine;
+        const int64_t step = next(mine);
+#pragma unroll
+        for (int p = 0; p + 1 < kStages; ++p) ahead[p] = ahead[p + 1];
+        ahead[kStages - 1] = mine;
+        if (mine != 0) fetch(step, mine, stage);
+        copy_commit();
+    };
 
     if (warp < 4) {
-        const int  col = strip * kTile + static_cast<int>(threadIdx.x);
-        const bool inside = col < G.k_len;
+        const int col0 = strip * kTile + warp * 32;  // this warp's columns: [32 rows][32] floats in each stage
         const uint32_t lane_base = tmem + (static_cast<uint32_t>(warp * 32) << 16);
-        float    x[kGradRows];
-        uint32_t mine;
-        auto load = [&](int64_t step, uint32_t mine) {
-            if (G.x.step >= 0) {
-                const char* p = G.x.data + 4 * (step * kGradRows * G.x.step) + col * G.x.nb0;
+        const uint8_t* mine_at = smem + S::kXAt + warp * 4096;
+        auto fetch = [&](int64_t step, uint32_t mine, int stage) {
+            const uint32_t place = smem_u32(mine_at + stage * S::kX);
+            if constexpr (VEC) {  // 4 rows at a time
+                const int   sub = lane >> 3, col = col0 + 4 * (lane & 7);
+                const char* p = G.x.row<true>(step * kGradRows + sub) + 4ll * col;
 #pragma unroll
-                for (int e = 0; e < kGradRows; ++e) {
-                    x[e] = inside && ((mine >> e) & 1u) ? *reinterpret_cast<const float*>(p) : 0.0f;
-                    p += 4ll * G.x.step;
+                for (int e = 0; e < 8; ++e) {
+                    copy_async<16>(place + (4 * e + sub) * 128 + (lane & 7) * 16, p, ((mine >> (4 * e + sub)) & 1u) && col < G.k_len);
+                    p += 16ll * G.x.step;
                 }
             } else {
-#pragma unroll
-                for (int e = 0; e < kGradRows; ++e)
-                    x[e] = inside && ((mine >> e) & 1u)
-                               ? *reinterpret_cast<const float*>(G.x.row<false>(step * kGradRows + e) + col * G.x.nb0) : 0.0f;
+                const bool inside = col0 + lane < G.k_len;
+                for (int e = 0; e < kGradRows; ++e) {
+                    const bool live = inside && ((mine >> e) & 1u);
+                    copy_async<4>(place + e * 128 + lane * 4,
+                                  live ? G.x.row<false>(step * kGradRows + e) + (col0 + lane) * G.x.nb0 : G.x.data, live);
+                }
             }
         };
-        int64_t step = next(mine);
-        if (mine != 0) load(step, mine);
-        for (int s = 0; mine != 0 && ok; ++s) {
+#pragma unroll
+        for (int p = 0; p < kStages - 1; ++p) turn(fetch, p);
+        for (int s = 0, stage = 0; ok; ++s, stage = stage + 1 == kStages ? 0 : stage + 1) {
+            __syncwarp();  // all lanes have read the stage that is filled now
+            turn(fetch, stage == 0 ? kStages - 1 : stage - 1);
+            if (ahead[0] == 0) break;
             const int buf = s & 1;
             if (s >= 2) ok = mbar_wait(&bars.ab_free[buf], ((s >> 1) - 1) & 1, TRC_DEVERR_WAIT_EMPTY);
             tc_fence_after();
+            copy_wait<kStages - 1>();
+            __syncwarp();  // every lane's copies are there
+            const float* x = reinterpret_cast<const float*>(mine_at + stage * S::kX) + lane;
             const uint32_t heads = lane_base + buf * 2 * kGradRows;
 #pragma unroll
             for (int g = 0; g < 2; ++g) {
                 uint32_t hd[16], tl[16];
 #pragma unroll
-                for (int e = 0; e < 16; ++e) split(x[16 * g + e], hd[e], tl[e]);
+                for (int e = 0; e < 16; ++e) split(x[32 * (16 * g + e)], hd[e], tl[e]);
                 __syncwarp();
                 tmem_st_32x32b_x16(heads + 16 * g, hd);
                 tmem_st_32x32b_x16(heads + kGradRows + 16 * g, tl);
             }
-            step = next(mine);
-            if (mine != 0) load(step, mine);
-            __syncwarp();
             tmem_st_wait();
             tc_fence_before();
             mbar_arrive(&bars.a_full[buf]);
         }
+        copy_wait<0>();
+        named_barrier_sync(1, 256);
     } else if (warp < 8) {
         const int tid = threadIdx.x - 128;
         float acc[LD];  // this lane's column, all ranks
 #pragma unroll
         for (int j = 0; j < LD; ++j) acc[j] = 0.0f;
         constexpr int kPieces = kGradRows * LD / 4 / 128;  // four ranks of a row each
-        float4   v[kPieces];
-        uint32_t mine;
         auto place = [&](int p, int& t, int& j) {
             const int i = tid + 128 * p;
             t = (i & 7) + 8 * (i / (2 * LD));
             j = 4 * ((i >> 3) % (LD / 4));
         };
-        auto load = [&](int64_t step, uint32_t mine) {
+        const uint8_t* mine_at = smem + S::kHAt + tid * 16;  // this lane's own pieces
+        auto fetch = [&](int64_t step, uint32_t mine, int stage) {
 #pragma unroll
             for (int p = 0; p < kPieces; ++p) {
                 int t, j;
                 place(p, t, j);
-                v[p] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                if (((mine >> t) & 1u) && j0 + j < ld) v[p] = *reinterpret_cast<const float4*>(G.h + (step * kGradRows + t) * ld + j0 + j);
+                copy_async<16>(smem_u32(mine_at + stage * S::kH + p * 2048), G.h + (step * kGradRows + t) * ld + j0 + j,
+                               ((mine >> t) & 1u) && j0 + j < ld);
             }
         };
         auto add = [&](int q) {  // the sums of steps kGradPromote * q ..
@@ -507,18 +541,22 @@ __global__ void __launch_bounds__(kTcThreads, 2) grad_tc_kernel(const __grid_con
             tc_fence_before();
             mbar_arrive(&bars.d_free[buf]);
         };
-        int64_t step = next(mine);
-        if (mine != 0) load(step, mine);
+#pragma unroll
+        for (int p = 0; p < kStages - 1; ++p) turn(fetch, p);
         int s = 0;
-        for (; mine != 0 && ok; ++s) {
+        for (int stage = 0; ok; ++s, stage = stage + 1 == kStages ? 0 : stage + 1) {
+            turn(fetch, stage == 0 ? kStages - 1 : stage - 1);
+            if (ahead[0] == 0) break;
             const int buf = s & 1;
             if (s >= 2) ok = mbar_wait(&bars.ab_free[buf], ((s >> 1) - 1) & 1, TRC_DEVERR_WAIT_EMPTY);
+            copy_wait<kStages - 1>();
             uint8_t* heads = smem + buf * S::kBuf;
 #pragma unroll
             for (int p = 0; p < kPieces; ++p) {
                 int t, j;
                 place(p, t, j);
-                const float w[4] = {v[p].x, v[p].y, v[p].z, v[p].w};
+                const float4 v = *reinterpret_cast<const float4*>(mine_at + stage * S::kH + p * 2048);
+                const float w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     uint32_t hd, tl;
@@ -531,15 +569,15 @@ __global__ void __launch_bounds__(kTcThreads, 2) grad_tc_kernel(const __grid_con
             }
             fence_proxy_async_smem();
             mbar_arrive(&bars.b_full[buf]);
-            step = next(mine);
-            if (mine != 0) load(step, mine);
             // while this group of steps runs, the one before
             if (s % kGradPromote == kGradPromote - 1 && s >= kGradPromote) add(s / kGradPromote - 1);
         }
+        copy_wait<0>();
         // the groups that are left: the loop has added group q when it built the last step of group q + 1
         const int groups = (s + kGradPromote - 1) / kGradPromote, added = s >= 2 * kGradPromote ? s / kGradPromote - 1 : 0;
         for (int q = added; q < groups && ok; ++q) add(q);
-        // every MMA of this CTA is complete: nothing reads the ranks' rows any more
+        // every MMA of this CTA is complete, and so are all copies once the other warps are through
+        named_barrier_sync(1, 256);
 #pragma unroll
         for (int j = 0; j < LD; ++j) sum[j][tid] = acc[j];
     } else {
@@ -604,9 +642,9 @@ __global__ void __launch_bounds__(kTcThreads, 2) grad_tc_kernel(const __grid_con
 }
 
 template <int LD>
-int run_grad(const Adapters& tab, const int32_t* ids, const GradSide& a, const GradSide& b, int64_t rows, int ld, int accumulate,
-             cudaStream_t s) {
-    auto kernel = &grad_tc_kernel<LD>;
+int run_grad(const Adapters& tab, const int32_t* ids, const GradSide& a, const GradSide& b, bool vec, int64_t rows, int ld,
+             int accumulate, cudaStream_t s) {
+    auto kernel = vec ? &grad_tc_kernel<LD, true> : &grad_tc_kernel<LD, false>;
     const int smem = GradSmem<LD>::kBytes;
     cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return cuda_fail(e);
@@ -731,7 +769,7 @@ int up_tc(bool back, int type, const Adapters& tab, const int32_t* ids, const tr
 }
 
 int grad_tc(const Adapters& tab, const int32_t* ids, const trc_cuda_view& x, const Rows& x_rows, const trc_cuda_view& dy,
-            const Rows& dy_rows, int64_t rows, const float* g, const float* h, int ld, int accumulate, cudaStream_t s) {
+            const Rows& dy_rows, bool vec, int64_t rows, const float* g, const float* h, int ld, int accumulate, cudaStream_t s) {
     bool any_a = false, any_b = false;
     for (int i = 0; i < tab.n; ++i) {
         any_a = any_a || tab.ad[i].da != nullptr;
@@ -740,9 +778,9 @@ int grad_tc(const Adapters& tab, const int32_t* ids, const trc_cuda_view& x, con
     if (!any_a && !any_b) return TRC_CUDA_OK;
     const GradSide a{x_rows, g, static_cast<int32_t>(x.ne[0]), any_a ? static_cast<int32_t>((x.ne[0] + kTile - 1) / kTile) : 0};
     const GradSide b{dy_rows, h, static_cast<int32_t>(dy.ne[0]), any_b ? static_cast<int32_t>((dy.ne[0] + kTile - 1) / kTile) : 0};
-    if (ld == 16) return run_grad<16>(tab, ids, a, b, rows, ld, accumulate, s);
-    if (ld == 32) return run_grad<32>(tab, ids, a, b, rows, ld, accumulate, s);
-    return run_grad<64>(tab, ids, a, b, rows, ld, accumulate, s);
+    if (ld == 16) return run_grad<16>(tab, ids, a, b, vec, rows, ld, accumulate, s);
+    if (ld == 32) return run_grad<32>(tab, ids, a, b, vec, rows, ld, accumulate, s);
+    return run_grad<64>(tab, ids, a, b, vec, rows, ld, accumulate, s);
 }
 
 }  // namespace lora
