@@ -396,6 +396,7 @@ __global__ void __launch_bounds__(kTcThreads, 2) grad_tc_kernel(const __grid_con
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(tc_raw) + 1023) & ~uintptr_t(1023));
     __shared__ __align__(8) GradBars bars;
     __shared__ uint32_t tmem_slot;
+    __shared__ int      is_last[2];  // of a step's operands: no step follows
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int ranks = static_cast<int>(cluster_nctarank()), rank = static_cast<int>(cluster_ctarank());
     int        strip = static_cast<int>(blockIdx.x) / ranks;
@@ -500,6 +501,7 @@ __global__ void __launch_bounds__(kTcThreads, 2) grad_tc_kernel(const __grid_con
             }
             tmem_st_wait();
             tc_fence_before();
+            if (threadIdx.x == 0) is_last[buf] = ahead[1] == 0;
             mbar_arrive(&bars.a_full[buf]);
         }
         copy_wait<0>();
@@ -584,37 +586,32 @@ __global__ void __launch_bounds__(kTcThreads, 2) grad_tc_kernel(const __grid_con
         const uint32_t idesc = make_idesc_tf32(kTile, LD, 0, 0);
         const uint32_t base = smem_u32(smem);
         uint32_t mine;
-        next(mine);
+        next(mine);  // is there a step at all?
         int s = 0;
-        for (; mine != 0 && ok; ++s) {
-            uint32_t following;
-            next(following);
-            const int buf = s & 1, q = s / kGradPromote, part = s % kGradPromote;
-            if (lane == 0) {
+        if (lane == 0 && mine != 0)
+            for (bool last = false; !last && ok; ++s) {
+                const int buf = s & 1, q = s / kGradPromote, part = s % kGradPromote;
                 ok = mbar_wait(&bars.a_full[buf], (s >> 1) & 1, TRC_DEVERR_WAIT_XFORM) &&
                      mbar_wait(&bars.b_full[buf], (s >> 1) & 1, TRC_DEVERR_WAIT_XFORM);
                 if (part == 0 && q >= 2) ok = ok && mbar_wait(&bars.d_free[q & 1], ((q >> 1) - 1) & 1, TRC_DEVERR_WAIT_ACCFREE);
-                if (ok) {
-                    tc_fence_after();
-                    const uint32_t dst = tmem + S::kD + (q & 1) * LD, a0 = tmem + buf * 2 * kGradRows, b0 = base + buf * S::kBuf;
+                if (!ok) break;
+                last = is_last[buf] != 0;
+                tc_fence_after();
+                const uint32_t dst = tmem + S::kD + (q & 1) * LD, a0 = tmem + buf * 2 * kGradRows, b0 = base + buf * S::kBuf;
 #pragma unroll
-                    for (int k = 0; k < kGradRows / 8; ++k) {
-                        const uint32_t off = (k >> 1) * (LD * 64) + (k & 1) * 32;
-                        const uint64_t bh = make_smem_desc(b0 + off, 16, 512, 4), bt = make_smem_desc(b0 + S::kPart + off, 16, 512, 4);
-                        umma_tf32_ts(dst, a0 + kGradRows + 8 * k, bh, idesc, part + k > 0);
-                        umma_tf32_ts(dst, a0 + 8 * k, bt, idesc, 1);
-                        umma_tf32_ts(dst, a0 + 8 * k, bh, idesc, 1);
-                    }
-                    umma_commit(&bars.ab_free[buf]);
-                    if (part == kGradPromote - 1 || following == 0) umma_commit(&bars.d_full[q & 1]);
+                for (int k = 0; k < kGradRows / 8; ++k) {
+                    const uint32_t off = (k >> 1) * (LD * 64) + (k & 1) * 32;
+                    const uint64_t bh = make_smem_desc(b0 + off, 16, 512, 4), bt = make_smem_desc(b0 + S::kPart + off, 16, 512, 4);
+                    umma_tf32_ts(dst, a0 + kGradRows + 8 * k, bh, idesc, part + k > 0);
+                    umma_tf32_ts(dst, a0 + 8 * k, bt, idesc, 1);
+                    umma_tf32_ts(dst, a0 + 8 * k, bh, idesc, 1);
                 }
+                umma_commit(&bars.ab_free[buf]);
+                if (part == kGradPromote - 1 || last) umma_commit(&bars.d_full[q & 1]);
             }
-            ok = __shfl_sync(0xFFFFFFFFu, ok ? 1 : 0, 0) != 0;
-            mine = following;
-        }
         // nothing may still read shared memory or TMEM when they are used anew
         if (lane == 0)
-            for (int p = max(0, s - 2); p < (ok ? s : s - 1); ++p) mbar_wait_drain(&bars.ab_free[p & 1], (p >> 1) & 1);
+            for (int p = max(0, s - 2); p < s; ++p) mbar_wait_drain(&bars.ab_free[p & 1], (p >> 1) & 1);
     }
     __syncwarp();
     tc_fence_before();
