@@ -364,14 +364,19 @@ struct GradBars {
 
 template <int LD>
 struct GradSmem {
-    static constexpr int kPart = LD * kGradRows * 4, kBuf = 2 * kPart;  // heads, tails
+    // The ranks' heads and, as further columns of the same operand, their tails: up to 32 ranks one MMA multiplies both
+    // with x's heads, which leaves two for 8 rows instead of three (an MMA takes 46 clocks to issue whatever its N up to 64).
+    // 64 ranks would need all of TMEM for it.
+    static constexpr bool kJoint = LD <= 32;
+    static constexpr int  kChunk = 2 * LD * 64, kBuf = 2 * kChunk;  // 16 rows each
+    static constexpr int  kSums = kJoint ? 2 * LD : LD;             // columns of sums
     static constexpr int kStages = LD == 64 ? 3 : 4;
     static constexpr int kX = kGradRows * kTile * 4, kH = kGradRows * LD * 4;  // a stage of the rings
     static constexpr int kXAt = 2 * kBuf, kHAt = kXAt + kStages * kX, kAll = kHAt + kStages * kH;
     static constexpr int kSum = LD * (kTile + 4) * 4;
     static constexpr int kBytes = (kAll > kSum ? kAll : kSum) + 1024;
     static_assert(kBytes <= 112 * 1024, "two CTAs on an SM");
-    static constexpr uint32_t kD = 4 * kGradRows, kCols = 4 * kGradRows + 2 * LD <= 128 ? 128 : 256;
+    static constexpr uint32_t kD = 4 * kGradRows, kCols = 4 * kGradRows + 2 * kSums <= 128 ? 128 : 256;
 };
 
 template <int BYTES>
@@ -430,13 +435,19 @@ __global__ void __launch_bounds__(kTcThreads, 2) grad_tc_kernel(const __grid_con
 
     // This CTA's steps: those of its turn that have a row of the adapter. Every warp goes through them for itself.
     const int64_t all = (rows + kGradRows - 1) / kGradRows;
-    int64_t  at = rank - ranks;
+    // The ids of the step after are loaded before they are needed (without it every step waited for them: 0.3 us).
+    int64_t at = rank - ranks;
+    auto hit = [&](int64_t step) {
+        const int64_t t = step * kGradRows + lane;
+        return step < all && t < rows && adapter_of(ids, t, tab.n) == ad;
+    };
+    bool coming = hit(at + ranks);
     auto next = [&](uint32_t& mine) {  // the next step's number, its rows in `mine`; mine = 0: there is none
         mine = 0;
         while (mine == 0 && at + ranks < all) {
             at += ranks;
-            const int64_t t = at * kGradRows + lane;
-            mine = __ballot_sync(0xFFFFFFFFu, t < rows && adapter_of(ids, t, tab.n) == ad);
+            mine = __ballot_sync(0xFFFFFFFFu, coming);
+            coming = hit(at + ranks);
         }
         return at;
     };
@@ -533,12 +544,12 @@ __global__ void __launch_bounds__(kTcThreads, 2) grad_tc_kernel(const __grid_con
             tc_fence_after();
             __syncwarp();
 #pragma unroll
-            for (int g = 0; g < LD / 16; ++g) {
+            for (int g = 0; g < S::kSums / 16; ++g) {
                 uint32_t d[16];
-                tmem_ld_32x32b_x16(tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16) + S::kD + buf * LD + 16 * g, d);
+                tmem_ld_32x32b_x16(tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16) + S::kD + buf * S::kSums + 16 * g, d);
                 tmem_ld_wait();
 #pragma unroll
-                for (int e = 0; e < 16; ++e) acc[16 * g + e] += __uint_as_float(d[e]);
+                for (int e = 0; e < 16; ++e) acc[(16 * g + e) % LD] += __uint_as_float(d[e]);
             }
             tc_fence_before();
             mbar_arrive(&bars.d_free[buf]);
@@ -564,9 +575,10 @@ __global__ void __launch_bounds__(kTcThreads, 2) grad_tc_kernel(const __grid_con
                     uint32_t hd, tl;
                     split(w[e], hd, tl);
                     const int m = j + e;
-                    const int off = (t >> 4) * (LD * 64) + m * 64 + ((((t >> 2) & 3) ^ ((m >> 1) & 3)) << 4) + 4 * (t & 3);
+                    // row LD + m is row m of another 8-row group of the swizzle: LD is a multiple of 8
+                    const int off = (t >> 4) * S::kChunk + m * 64 + ((((t >> 2) & 3) ^ ((m >> 1) & 3)) << 4) + 4 * (t & 3);
                     *reinterpret_cast<uint32_t*>(heads + off) = hd;
-                    *reinterpret_cast<uint32_t*>(heads + S::kPart + off) = tl;
+                    *reinterpret_cast<uint32_t*>(heads + LD * 64 + off) = tl;
                 }
             }
             fence_proxy_async_smem();
@@ -583,7 +595,7 @@ __global__ void __launch_bounds__(kTcThreads, 2) grad_tc_kernel(const __grid_con
 #pragma unroll
         for (int j = 0; j < LD; ++j) sum[j][tid] = acc[j];
     } else {
-        const uint32_t idesc = make_idesc_tf32(kTile, LD, 0, 0);
+        const uint32_t idesc = make_idesc_tf32(kTile, LD, 0, 0), joint = make_idesc_tf32(kTile, 2 * LD, 0, 0);
         const uint32_t base = smem_u32(smem);
         uint32_t mine;
         next(mine);  // is there a step at all?
@@ -597,14 +609,19 @@ __global__ void __launch_bounds__(kTcThreads, 2) grad_tc_kernel(const __grid_con
                 if (!ok) break;
                 last = is_last[buf] != 0;
                 tc_fence_after();
-                const uint32_t dst = tmem + S::kD + (q & 1) * LD, a0 = tmem + buf * 2 * kGradRows, b0 = base + buf * S::kBuf;
+                const uint32_t dst = tmem + S::kD + (q & 1) * S::kSums, a0 = tmem + buf * 2 * kGradRows, b0 = base + buf * S::kBuf;
 #pragma unroll
                 for (int k = 0; k < kGradRows / 8; ++k) {
-                    const uint32_t off = (k >> 1) * (LD * 64) + (k & 1) * 32;
-                    const uint64_t bh = make_smem_desc(b0 + off, 16, 512, 4), bt = make_smem_desc(b0 + S::kPart + off, 16, 512, 4);
-                    umma_tf32_ts(dst, a0 + kGradRows + 8 * k, bh, idesc, part + k > 0);
-                    umma_tf32_ts(dst, a0 + 8 * k, bt, idesc, 1);
-                    umma_tf32_ts(dst, a0 + 8 * k, bh, idesc, 1);
+                    const uint64_t bh = make_smem_desc(b0 + (k >> 1) * S::kChunk + (k & 1) * 32, 16, 512, 4);
+                    if constexpr (S::kJoint) {
+                        umma_tf32_ts(dst, a0 + 8 * k, bh, joint, part + k > 0);
+                        umma_tf32_ts(dst, a0 + kGradRows + 8 * k, bh, idesc, 1);
+                    } else {
+                        const uint64_t bt = make_smem_desc(b0 + LD * 64 + (k >> 1) * S::kChunk + (k & 1) * 32, 16, 512, 4);
+                        umma_tf32_ts(dst, a0 + kGradRows + 8 * k, bh, idesc, part + k > 0);
+                        umma_tf32_ts(dst, a0 + 8 * k, bt, idesc, 1);
+                        umma_tf32_ts(dst, a0 + 8 * k, bh, idesc, 1);
+                    }
                 }
                 umma_commit(&bars.ab_free[buf]);
                 if (part == kGradPromote - 1 || last) umma_commit(&bars.d_full[q & 1]);
