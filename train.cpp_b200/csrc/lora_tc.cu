@@ -15,6 +15,7 @@
 
 #include <algorithm>
 #include <mutex>
+#include <type_traits>
 
 #include "lora_common.cuh"
 
@@ -341,11 +342,13 @@ __global__ void __launch_bounds__(kTcThreads, 2) up_tc_kernel(const __grid_const
 // out(j, k) (+)= sum over the adapter's rows t of h[t, j] x[t, k]; dA (h = g, x) is j-major, dB (h, x = dy)
 // k-major. The MMA's M are 128 columns of x, its N the ranks (up to 64 at a time), its K the rows. A thread of four
 // warps owns a column: it takes 32 rows of it, splits them and puts them into its lane of TMEM, the first operand. Four
-// other warps build the ranks' rows in shared memory (transposed, K-major, 64-byte swizzle) and add the sums of every 64
+// other warps build the ranks' rows in shared memory (heads and tails, MN-major as they come) and add the sums of every 64
 // rows up in fp32, because the tensor core's own sums lose a little at every product (7e-8 of the result for 8 rows in a chain).
-// What a warp takes (its 32 columns of x, its pieces of h) runs through a ring of asynchronous copies of its own, two to
-// three steps ahead: with loads one step ahead, in registers, a step took a DRAM round trip, 1.9 us.
+// x comes through TMA, three to four steps ahead (rows that TMA cannot address: through asynchronous copies of each warp's
+// own columns), h through copies of each lane's own pieces. With loads one step ahead, in registers, a step took a DRAM
+// round trip, 1.9 us; with the four warps of x copying for themselves 0.9 us, most of it their copies' instructions.
 // The CTAs of a cluster share the steps of 32 rows in turns and join their sums in order.
+constexpr int kGradThreads = 320;  // 4 warps for x, 4 for the ranks, 1 issues, 1 loads
 constexpr int kGradRows = 32, kGradPromote = 2;  // rows of a step, steps between two additions in fp32
 
 struct GradSide {
@@ -360,6 +363,7 @@ struct GradBars {
     uint64_t ab_free[2];            // and read (commit)
     uint64_t d_full[2];             // the sums of some steps are complete (commit)
     uint64_t d_free[2];             // and in registers (128 arrivals)
+    uint64_t x_full[4], x_free[4];  // x's stages: landed, taken (128 arrivals)
 };
 
 template <int LD>
@@ -368,7 +372,8 @@ struct GradSmem {
     // with x's heads, which leaves two for 8 rows instead of three (an MMA takes 46 clocks to issue whatever its N up to 64).
     // 64 ranks would need all of TMEM for it.
     static constexpr bool kJoint = LD <= 32;
-    static constexpr int  kChunk = 2 * LD * 64, kBuf = 2 * kChunk;  // 16 rows each
+    // MN-major: 2 KB for 16 rows of 32 columns (heads, then tails), 128-byte swizzle in 32-byte units
+    static constexpr int  kChunk = 2 * LD / 32 * 2048, kBuf = 2 * kChunk;  // 16 rows each
     static constexpr int  kSums = kJoint ? 2 * LD : LD;             // columns of sums
     static constexpr int kStages = LD == 64 ? 3 : 4;
     static constexpr int kX = kGradRows * kTile * 4, kH = kGradRows * LD * 4;  // a stage of the rings
@@ -392,7 +397,9 @@ __device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group 
 
 // VEC: both sides' rows are evenly spaced, whole in 16-byte pieces and start at multiples of 16 bytes.
 template <int LD, bool VEC>
-__global__ void __launch_bounds__(kTcThreads, 2) grad_tc_kernel(const __grid_constant__ Adapters tab, const int32_t* ids,
+__global__ void __launch_bounds__(kGradThreads, 2) grad_tc_kernel(const __grid_constant__ Adapters tab, const int32_t* ids,
+                                                                const __grid_constant__ CUtensorMap map_a,
+                                                                const __grid_constant__ CUtensorMap map_b,
                                                                 const __grid_constant__ GradSide side_a,
                                                                 const __grid_constant__ GradSide side_b, int64_t rows, int ld,
                                                                 int accumulate) {
@@ -402,6 +409,8 @@ __global__ void __launch_bounds__(kTcThreads, 2) grad_tc_kernel(const __grid_con
     __shared__ __align__(8) GradBars bars;
     __shared__ uint32_t tmem_slot;
     __shared__ int      is_last[2];  // of a step's operands: no step follows
+    __shared__ uint32_t stage_rows[4];
+    __shared__ int      stage_last[4];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int ranks = static_cast<int>(cluster_nctarank()), rank = static_cast<int>(cluster_ctarank());
     int        strip = static_cast<int>(blockIdx.x) / ranks;
@@ -421,6 +430,10 @@ __global__ void __launch_bounds__(kTcThreads, 2) grad_tc_kernel(const __grid_con
             mbar_init(&bars.ab_free[i], 1);
             mbar_init(&bars.d_full[i], 1);
             mbar_init(&bars.d_free[i], 128);
+        }
+        for (int i = 0; i < S::kStages; ++i) {
+            mbar_init(&bars.x_full[i], 1);
+            mbar_init(&bars.x_free[i], 128);
         }
         fence_barrier_init();
     }
@@ -466,56 +479,69 @@ __global__ void __launch_bounds__(kTcThreads, 2) grad_tc_kernel(const __grid_con
     };
 
     if (warp < 4) {
-        const int col0 = strip * kTile + warp * 32;  // this warp's columns: [32 rows][32] floats in each stage
         const uint32_t lane_base = tmem + (static_cast<uint32_t>(warp * 32) << 16);
-        const uint8_t* mine_at = smem + S::kXAt + warp * 4096;
-        auto fetch = [&](int64_t step, uint32_t mine, int stage) {
-            const uint32_t place = smem_u32(mine_at + stage * S::kX);
-            if constexpr (VEC) {  // 4 rows at a time
-                const int   sub = lane >> 3, col = col0 + 4 * (lane & 7);
-                const char* p = G.x.row<true>(step * kGradRows + sub) + 4ll * col;
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    copy_async<16>(place + (4 * e + sub) * 128 + (lane & 7) * 16, p, ((mine >> (4 * e + sub)) & 1u) && col < G.k_len);
-                    p += 16ll * G.x.step;
-                }
-            } else {
-                const bool inside = col0 + lane < G.k_len;
-                for (int e = 0; e < kGradRows; ++e) {
-                    const bool live = inside && ((mine >> e) & 1u);
-                    copy_async<4>(place + e * 128 + lane * 4,
-                                  live ? G.x.row<false>(step * kGradRows + e) + (col0 + lane) * G.x.nb0 : G.x.data, live);
-                }
-            }
-        };
-#pragma unroll
-        for (int p = 0; p < kStages - 1; ++p) turn(fetch, p);
-        for (int s = 0, stage = 0; ok; ++s, stage = stage + 1 == kStages ? 0 : stage + 1) {
-            __syncwarp();  // all lanes have read the stage that is filled now
-            turn(fetch, stage == 0 ? kStages - 1 : stage - 1);
-            if (ahead[0] == 0) break;
+        // 32 rows of this lane's column, `pitch` floats apart, into TMEM; rows that are not the adapter's as zeros
+        auto put = [&](int s, const float* x, auto pitch, uint32_t mine, bool last) {
+            constexpr int kPitch = decltype(pitch)::value;
             const int buf = s & 1;
-            if (s >= 2) ok = mbar_wait(&bars.ab_free[buf], ((s >> 1) - 1) & 1, TRC_DEVERR_WAIT_EMPTY);
+            if (s >= 2) ok = ok && mbar_wait(&bars.ab_free[buf], ((s >> 1) - 1) & 1, TRC_DEVERR_WAIT_EMPTY);
             tc_fence_after();
-            copy_wait<kStages - 1>();
-            __syncwarp();  // every lane's copies are there
-            const float* x = reinterpret_cast<const float*>(mine_at + stage * S::kX) + lane;
             const uint32_t heads = lane_base + buf * 2 * kGradRows;
 #pragma unroll
             for (int g = 0; g < 2; ++g) {
+                float    v[16];
                 uint32_t hd[16], tl[16];
 #pragma unroll
-                for (int e = 0; e < 16; ++e) split(x[32 * (16 * g + e)], hd[e], tl[e]);
+                for (int e = 0; e < 16; ++e) v[e] = x[kPitch * (16 * g + e)];
+                if (mine != 0xFFFFFFFFu)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) v[e] = (mine >> (16 * g + e)) & 1u ? v[e] : 0.0f;
+#pragma unroll
+                for (int e = 0; e < 16; ++e) split(v[e], hd[e], tl[e]);
                 __syncwarp();
                 tmem_st_32x32b_x16(heads + 16 * g, hd);
                 tmem_st_32x32b_x16(heads + kGradRows + 16 * g, tl);
             }
             tmem_st_wait();
             tc_fence_before();
-            if (threadIdx.x == 0) is_last[buf] = ahead[1] == 0;
+            if (threadIdx.x == 0) is_last[buf] = last;
             mbar_arrive(&bars.a_full[buf]);
+        };
+        if constexpr (VEC) {
+            bool last = false;
+            for (int s = 0, stage = 0; !last && ok; ++s) {
+                ok = mbar_wait(&bars.x_full[stage], (s / kStages) & 1, TRC_DEVERR_WAIT_FULL);
+                const uint32_t mine = stage_rows[stage];
+                last = stage_last[stage] != 0;
+                if (!ok || mine == 0) break;  // no step at all
+                put(s, reinterpret_cast<const float*>(smem + S::kXAt + stage * S::kX) + threadIdx.x,
+                    std::integral_constant<int, kTile>(), mine, last);
+                mbar_arrive(&bars.x_free[stage]);
+                stage = stage + 1 == kStages ? 0 : stage + 1;
+            }
+        } else {
+            const int col0 = strip * kTile + warp * 32;  // this warp's columns: [32 rows][32] floats in each stage
+            const uint8_t* mine_at = smem + S::kXAt + warp * 4096;
+            auto fetch = [&](int64_t step, uint32_t mine, int stage) {
+                const uint32_t place = smem_u32(mine_at + stage * S::kX);
+                const bool inside = col0 + lane < G.k_len;
+                for (int e = 0; e < kGradRows; ++e) {
+                    const bool live = inside && ((mine >> e) & 1u);
+                    copy_async<4>(place + e * 128 + lane * 4,
+                                  live ? G.x.row<false>(step * kGradRows + e) + (col0 + lane) * G.x.nb0 : G.x.data, live);
+                }
+            };
+#pragma unroll
+            for (int p = 0; p < kStages - 1; ++p) turn(fetch, p);
+            for (int s = 0, stage = 0; ok; ++s, stage = stage + 1 == kStages ? 0 : stage + 1) {
+                turn(fetch, stage == 0 ? kStages - 1 : stage - 1);
+                if (ahead[0] == 0) break;
+                copy_wait<kStages - 1>();
+                put(s, reinterpret_cast<const float*>(mine_at + stage * S::kX) + lane, std::integral_constant<int, 32>(), 0xFFFFFFFFu,
+                    ahead[1] == 0);
+            }
+            copy_wait<0>();
         }
-        copy_wait<0>();
         named_barrier_sync(1, 256);
     } else if (warp < 8) {
         const int tid = threadIdx.x - 128;
@@ -524,9 +550,9 @@ __global__ void __launch_bounds__(kTcThreads, 2) grad_tc_kernel(const __grid_con
         for (int j = 0; j < LD; ++j) acc[j] = 0.0f;
         constexpr int kPieces = kGradRows * LD / 4 / 128;  // four ranks of a row each
         auto place = [&](int p, int& t, int& j) {
-            const int i = tid + 128 * p;
-            t = (i & 7) + 8 * (i / (2 * LD));
-            j = 4 * ((i >> 3) % (LD / 4));
+            const int i = tid + 128 * p;  // a row's pieces side by side
+            t = i / (LD / 4);
+            j = 4 * (i % (LD / 4));
         };
         const uint8_t* mine_at = smem + S::kHAt + tid * 16;  // this lane's own pieces
         auto fetch = [&](int64_t step, uint32_t mine, int stage) {
@@ -569,17 +595,17 @@ __global__ void __launch_bounds__(kTcThreads, 2) grad_tc_kernel(const __grid_con
                 int t, j;
                 place(p, t, j);
                 const float4 v = *reinterpret_cast<const float4*>(mine_at + stage * S::kH + p * 2048);
-                const float w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    uint32_t hd, tl;
-                    split(w[e], hd, tl);
-                    const int m = j + e;
-                    // row LD + m is row m of another 8-row group of the swizzle: LD is a multiple of 8
-                    const int off = (t >> 4) * S::kChunk + m * 64 + ((((t >> 2) & 3) ^ ((m >> 1) & 3)) << 4) + 4 * (t & 3);
-                    *reinterpret_cast<uint32_t*>(heads + off) = hd;
-                    *reinterpret_cast<uint32_t*>(heads + LD * 64 + off) = tl;
-                }
+                uint32_t hd[4], tl[4];
+                split(v.x, hd[0], tl[0]);
+                split(v.y, hd[1], tl[1]);
+                split(v.z, hd[2], tl[2]);
+                split(v.w, hd[3], tl[3]);
+                // columns m .. m + 3 of row t: chunk m / 32, 32-byte unit (m % 32) / 8 exchanged by the row
+                auto at_column = [&](int m) {
+                    return (t >> 4) * S::kChunk + (m >> 5) * 2048 + (t & 15) * 128 + ((((m & 31) >> 3) ^ (t & 3)) << 5) + ((m & 4) << 2);
+                };
+                *reinterpret_cast<uint4*>(heads + at_column(j)) = make_uint4(hd[0], hd[1], hd[2], hd[3]);
+                *reinterpret_cast<uint4*>(heads + at_column(LD + j)) = make_uint4(tl[0], tl[1], tl[2], tl[3]);
             }
             fence_proxy_async_smem();
             mbar_arrive(&bars.b_full[buf]);
@@ -594,8 +620,8 @@ __global__ void __launch_bounds__(kTcThreads, 2) grad_tc_kernel(const __grid_con
         named_barrier_sync(1, 256);
 #pragma unroll
         for (int j = 0; j < LD; ++j) sum[j][tid] = acc[j];
-    } else {
-        const uint32_t idesc = make_idesc_tf32(kTile, LD, 0, 0), joint = make_idesc_tf32(kTile, 2 * LD, 0, 0);
+    } else if (warp == 8) {
+        const uint32_t idesc = make_idesc_tf32(kTile, LD, 0, 1), joint = make_idesc_tf32(kTile, 2 * LD, 0, 1);
         const uint32_t base = smem_u32(smem);
         uint32_t mine;
         next(mine);  // is there a step at all?
@@ -612,12 +638,12 @@ __global__ void __launch_bounds__(kTcThreads, 2) grad_tc_kernel(const __grid_con
                 const uint32_t dst = tmem + S::kD + (q & 1) * S::kSums, a0 = tmem + buf * 2 * kGradRows, b0 = base + buf * S::kBuf;
 #pragma unroll
                 for (int k = 0; k < kGradRows / 8; ++k) {
-                    const uint64_t bh = make_smem_desc(b0 + (k >> 1) * S::kChunk + (k & 1) * 32, 16, 512, 4);
+                    const uint64_t bh = make_smem_desc(b0 + (k >> 1) * S::kChunk + (k & 1) * 1024, 2048, 512, 1);
                     if constexpr (S::kJoint) {
                         umma_tf32_ts(dst, a0 + 8 * k, bh, joint, part + k > 0);
                         umma_tf32_ts(dst, a0 + kGradRows + 8 * k, bh, idesc, 1);
                     } else {
-                        const uint64_t bt = make_smem_desc(b0 + LD * 64 + (k >> 1) * S::kChunk + (k & 1) * 32, 16, 512, 4);
+                        const uint64_t bt = make_smem_desc(b0 + LD / 32 * 2048 + (k >> 1) * S::kChunk + (k & 1) * 1024, 2048, 512, 1);
                         umma_tf32_ts(dst, a0 + kGradRows + 8 * k, bh, idesc, part + k > 0);
                         umma_tf32_ts(dst, a0 + 8 * k, bt, idesc, 1);
                         umma_tf32_ts(dst, a0 + 8 * k, bh, idesc, 1);
@@ -629,6 +655,35 @@ __global__ void __launch_bounds__(kTcThreads, 2) grad_tc_kernel(const __grid_con
         // nothing may still read shared memory or TMEM when they are used anew
         if (lane == 0)
             for (int p = max(0, s - 2); p < s; ++p) mbar_wait_drain(&bars.ab_free[p & 1], (p >> 1) & 1);
+    } else if constexpr (VEC) {
+        // x's tiles: 32 rows of 128 columns, whoever's they are; `stage_rows` says which of them count
+        uint32_t mine, following;
+        int64_t  step = next(mine);
+        int s = 0;
+        for (bool go = true; go && ok; ++s) {
+            const int     stage = s % kStages;
+            const int64_t after = next(following);
+            if (lane == 0) {
+                if (s >= kStages) ok = mbar_wait(&bars.x_free[stage], (s / kStages - 1) & 1, TRC_DEVERR_WAIT_EMPTY);
+                if (ok) {
+                    stage_rows[stage] = mine;
+                    stage_last[stage] = following == 0;
+                    if (mine != 0) {
+                        mbar_arrive_expect_tx(&bars.x_full[stage], S::kX);
+                        tma_load_2d(smem_u32(smem + S::kXAt + stage * S::kX), is_b ? &map_b : &map_a, &bars.x_full[stage],
+                                    strip * kTile, static_cast<int>(step * kGradRows));
+                    } else {
+                        mbar_arrive(&bars.x_full[stage]);
+                    }
+                }
+            }
+            ok = __shfl_sync(0xFFFFFFFFu, ok ? 1 : 0, 0) != 0;
+            go = following != 0;
+            mine = following;
+            step = after;
+        }
+        if (lane == 0)
+            for (int p = max(0, s - kStages); p < s; ++p) mbar_wait_drain(&bars.x_full[p % kStages], (p / kStages) & 1);
     }
     __syncwarp();
     tc_fence_before();
@@ -638,7 +693,7 @@ __global__ void __launch_bounds__(kTcThreads, 2) grad_tc_kernel(const __grid_con
 
     // this CTA's sums, then the cluster's
     if (ranks > 1) cluster_sync();
-    for (int i = rank * kTcThreads + threadIdx.x; i < LD * kTile; i += kTcThreads * ranks) {
+    for (int i = rank * kGradThreads + threadIdx.x; i < LD * kTile; i += kGradThreads * ranks) {
         // neighbours in memory are neighbours in the lanes
         const int j = is_b ? i % LD : i / kTile, k = is_b ? i / LD : i % kTile;
         if (j0 + j >= r || strip * kTile + k >= G.k_len) continue;
@@ -655,39 +710,6 @@ __global__ void __launch_bounds__(kTcThreads, 2) grad_tc_kernel(const __grid_con
     if (ranks > 1) cluster_sync();
 }
 
-template <int LD>
-int run_grad(const Adapters& tab, const int32_t* ids, const GradSide& a, const GradSide& b, bool vec, int64_t rows, int ld,
-             int accumulate, cudaStream_t s) {
-    auto kernel = vec ? &grad_tc_kernel<LD, true> : &grad_tc_kernel<LD, false>;
-    const int smem = GradSmem<LD>::kBytes;
-    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-    if (e != cudaSuccess) return cuda_fail(e);
-    const int64_t chunks = (ld + LD - 1) / LD, units = (a.strips + b.strips) * chunks * tab.n;
-    // the rows of a strip go to 1 - 8 CTAs: one wave of two CTAs for each SM, at least four steps for each
-    const int64_t room = 2 * static_cast<int64_t>(std::max(1, sm_count_current())), steps = (rows + kGradRows - 1) / kGradRows;
-    unsigned cluster = 1;
-    while (cluster < 8 && 2 * cluster * units <= room && 8 * cluster <= steps) cluster *= 2;
-    if ((a.strips + b.strips) * static_cast<int64_t>(cluster) > INT32_MAX) return TRC_CUDA_EUNSUPPORTED;
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(static_cast<unsigned>((a.strips + b.strips) * cluster), static_cast<unsigned>(chunks), static_cast<unsigned>(tab.n));
-    cfg.blockDim = dim3(kTcThreads);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = s;
-    cudaLaunchAttribute at[1];
-    at[0].id = cudaLaunchAttributeClusterDimension;
-    at[0].val.clusterDim.x = cluster;
-    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
-    cfg.attrs = at;
-    cfg.numAttrs = 1;
-    e = cudaLaunchKernelEx(&cfg, kernel, tab, ids, a, b, rows, ld, accumulate);
-    if (e != cudaSuccess) {
-        cudaGetLastError();
-        return cuda_fail(e);
-    }
-    note_launch();
-    return TRC_CUDA_OK;
-}
-
 PFN_cuTensorMapEncodeTiled_v12000 encoder() {
     static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
     static std::once_flag once;
@@ -701,8 +723,8 @@ PFN_cuTensorMapEncodeTiled_v12000 encoder() {
     return fn;
 }
 
-// Evenly spaced rows of floats (the caller has checked them), in boxes of 128 rows by 32 columns.
-bool encode_rows(const trc_cuda_view& v, int64_t rows, CUtensorMap& map) {
+// Evenly spaced rows of floats (the caller has checked them), in boxes of box_rows by box_cols.
+bool encode_rows(const trc_cuda_view& v, int64_t rows, CUtensorMap& map, int box_rows, int box_cols, CUtensorMapSwizzle swizzle) {
     auto enc = encoder();
     if (enc == nullptr) return false;
     // one stride for all rows, that of the first extent over 1
@@ -712,9 +734,42 @@ bool encode_rows(const trc_cuda_view& v, int64_t rows, CUtensorMap& map) {
     if (step <= 0 || step % 16 != 0) return false;
     const cuuint64_t dims[2] = {static_cast<cuuint64_t>(v.ne[0]), static_cast<cuuint64_t>(rows)};
     const cuuint64_t strides[1] = {static_cast<cuuint64_t>(step)};
-    const cuuint32_t box[2] = {kBlock, kTile}, one[2] = {1, 1};
+    const cuuint32_t box[2] = {static_cast<cuuint32_t>(box_cols), static_cast<cuuint32_t>(box_rows)}, one[2] = {1, 1};
     return enc(&map, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 2, v.data, dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
-               CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+               swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <int LD>
+int run_grad(const Adapters& tab, const int32_t* ids, const CUtensorMap& map_a, const CUtensorMap& map_b, const GradSide& a,
+             const GradSide& b, bool vec, int64_t rows, int ld, int accumulate, cudaStream_t s) {
+    auto kernel = vec ? &grad_tc_kernel<LD, true> : &grad_tc_kernel<LD, false>;
+    const int smem = GradSmem<LD>::kBytes;
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) return cuda_fail(e);
+    const int64_t chunks = (ld + LD - 1) / LD, units = (a.strips + b.strips) * chunks * tab.n;
+    // the rows of a strip go to 1 - 8 CTAs: one wave of two CTAs for each SM, at least four steps for each
+    const int64_t room = 2 * static_cast<int64_t>(std::max(1, sm_count_current())), steps = (rows + kGradRows - 1) / kGradRows;
+    unsigned cluster = 1;
+    while (cluster < 8 && 2 * cluster * units <= room && 8 * cluster <= steps) cluster *= 2;
+    if ((a.strips + b.strips) * static_cast<int64_t>(cluster) > INT32_MAX) return TRC_CUDA_EUNSUPPORTED;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(static_cast<unsigned>((a.strips + b.strips) * cluster), static_cast<unsigned>(chunks), static_cast<unsigned>(tab.n));
+    cfg.blockDim = dim3(kGradThreads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = cluster;
+    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    e = cudaLaunchKernelEx(&cfg, kernel, tab, ids, map_a, map_b, a, b, rows, ld, accumulate);
+    if (e != cudaSuccess) {
+        cudaGetLastError();
+        return cuda_fail(e);
+    }
+    note_launch();
+    return TRC_CUDA_OK;
 }
 
 template <typename W, bool BACK, int LD>
@@ -773,9 +828,9 @@ int up_tc(bool back, int type, const Adapters& tab, const int32_t* ids, const tr
     // a tile of 128 rows has to be worth its own: below, the warp-level kernel's tiles of 32 rows fill more SMs
     if (ld > 64 || rows < 128) return TRC_CUDA_EUNSUPPORTED;
     CUtensorMap d_map, base_map;
-    if (!encode_rows(*d, rows, d_map)) return TRC_CUDA_EUNSUPPORTED;
+    if (!encode_rows(*d, rows, d_map, kTile, kBlock, CU_TENSOR_MAP_SWIZZLE_128B)) return TRC_CUDA_EUNSUPPORTED;
     base_map = d_map;
-    if (base != nullptr && !encode_rows(*base, rows, base_map)) return TRC_CUDA_EUNSUPPORTED;
+    if (base != nullptr && !encode_rows(*base, rows, base_map, kTile, kBlock, CU_TENSOR_MAP_SWIZZLE_128B)) return TRC_CUDA_EUNSUPPORTED;
     const int add = base != nullptr, n = static_cast<int>(d->ne[0]);
     if (type == TRC_CUDA_TYPE_F32) return run_dir<float>(back, tab, ids, base_map, d_map, add, rows, n, h, ld, s);
     if (type == TRC_CUDA_TYPE_F16) return run_dir<__half>(back, tab, ids, base_map, d_map, add, rows, n, h, ld, s);
@@ -792,9 +847,13 @@ int grad_tc(const Adapters& tab, const int32_t* ids, const trc_cuda_view& x, con
     if (!any_a && !any_b) return TRC_CUDA_OK;
     const GradSide a{x_rows, g, static_cast<int32_t>(x.ne[0]), any_a ? static_cast<int32_t>((x.ne[0] + kTile - 1) / kTile) : 0};
     const GradSide b{dy_rows, h, static_cast<int32_t>(dy.ne[0]), any_b ? static_cast<int32_t>((dy.ne[0] + kTile - 1) / kTile) : 0};
-    if (ld == 16) return run_grad<16>(tab, ids, a, b, vec, rows, ld, accumulate, s);
-    if (ld == 32) return run_grad<32>(tab, ids, a, b, vec, rows, ld, accumulate, s);
-    return run_grad<64>(tab, ids, a, b, vec, rows, ld, accumulate, s);
+    CUtensorMap map_a{}, map_b{};
+    if (vec && rows > 0)
+        vec = encode_rows(x, rows, map_a, kGradRows, kTile, CU_TENSOR_MAP_SWIZZLE_NONE) &&
+              encode_rows(dy, rows, map_b, kGradRows, kTile, CU_TENSOR_MAP_SWIZZLE_NONE);
+    if (ld == 16) return run_grad<16>(tab, ids, map_a, map_b, a, b, vec, rows, ld, accumulate, s);
+    if (ld == 32) return run_grad<32>(tab, ids, map_a, map_b, a, b, vec, rows, ld, accumulate, s);
+    return run_grad<64>(tab, ids, map_a, map_b, a, b, vec, rows, ld, accumulate, s);
 }
 
 }  // namespace lora
