@@ -349,6 +349,7 @@ __global__ void __launch_bounds__(kTcThreads, 2) up_tc_kernel(const __grid_const
 // round trip, 1.9 us; with the four warps of x copying for themselves 0.9 us, most of it their copies' instructions.
 // The CTAs of a cluster share the steps of 32 rows in turns and join their sums in order.
 constexpr int kGradThreads = 320;  // 4 warps for x, 4 for the ranks, 1 issues, 1 loads
+constexpr int kGradMasks = 768;
 constexpr int kGradRows = 32, kGradPromote = 2;  // rows of a step, steps between two additions in fp32
 
 struct GradSide {
@@ -409,7 +410,7 @@ __global__ void __launch_bounds__(kGradThreads, 2) grad_tc_kernel(const __grid_c
     __shared__ __align__(8) GradBars bars;
     __shared__ uint32_t tmem_slot;
     __shared__ int      is_last[2];  // of a step's operands: no step follows
-    __shared__ uint32_t stage_rows[4];
+    __shared__ uint32_t stage_rows[4], masks[kGradMasks];
     __shared__ int      stage_last[4];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int ranks = static_cast<int>(cluster_nctarank()), rank = static_cast<int>(cluster_ctarank());
@@ -446,23 +447,29 @@ __global__ void __launch_bounds__(kGradThreads, 2) grad_tc_kernel(const __grid_c
     tc_fence_after();
     const uint32_t tmem = tmem_slot;
 
-    // This CTA's steps: those of its turn that have a row of the adapter. Every warp goes through them for itself.
-    const int64_t all = (rows + kGradRows - 1) / kGradRows;
-    // The ids of the step after are loaded before they are needed (without it every step waited for them: 0.3 us).
-    int64_t at = rank - ranks;
-    auto hit = [&](int64_t step) {
-        const int64_t t = step * kGradRows + lane;
-        return step < all && t < rows && adapter_of(ids, t, tab.n) == ad;
+    // This CTA's steps are those of its turn that have a row of the adapter. Which rows: looked up for all of them at once,
+    // at the start (step by step every one waited for its ids, and an adapter's first step for all those before it: 25 us
+    // with three adapters and 2048 rows); beyond kGradMasks steps, as they come.
+    const int64_t all = (rows + kGradRows - 1) / kGradRows, my = all > rank ? (all - rank + ranks - 1) / ranks : 0;
+    auto rows_of_step = [&](int64_t i) {  // of the i-th step of this CTA's turn
+        const int64_t t = (rank + i * ranks) * kGradRows + lane;
+        return __ballot_sync(0xFFFFFFFFu, t < rows && adapter_of(ids, t, tab.n) == ad);
     };
-    bool coming = hit(at + ranks);
+    const int known = static_cast<int>(min(my, static_cast<int64_t>(kGradMasks)));
+#pragma unroll 4
+    for (int i = warp; i < known; i += kGradThreads / 32) {
+        const uint32_t m = rows_of_step(i);
+        if (lane == 0) masks[i] = m;
+    }
+    __syncthreads();
+    int64_t at = -1;
     auto next = [&](uint32_t& mine) {  // the next step's number, its rows in `mine`; mine = 0: there is none
         mine = 0;
-        while (mine == 0 && at + ranks < all) {
-            at += ranks;
-            mine = __ballot_sync(0xFFFFFFFFu, coming);
-            coming = hit(at + ranks);
+        while (mine == 0 && at + 1 < my) {
+            ++at;
+            mine = at < known ? masks[at] : rows_of_step(at);
         }
-        return at;
+        return rank + at * ranks;
     };
     bool ok = true;
     float (*sum)[kTile + 4] = reinterpret_cast<float (*)[kTile + 4]>(smem);  // in the place of all that
