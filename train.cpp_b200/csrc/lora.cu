@@ -178,8 +178,9 @@ __global__ void __launch_bounds__(kThreads, DownRing<W, NT>::kCtas) down_kernel(
     const uint32_t ring = smem_u32(red) + warp * (kStages * Ring::kStage);
     const int      ranks = static_cast<int>(cluster_nctarank()), rank = static_cast<int>(cluster_ctarank());
     const int64_t  row0 = static_cast<int64_t>(blockIdx.x / ranks) * kRows;
-    const TileIds  tile(ids, row0, kRows, rows, tab.n);
+    grid_wait();
     grid_dependents();
+    const TileIds  tile(ids, row0, kRows, rows, tab.n);
 
     if (blockIdx.y == 0 && rank == 0) {  // rows without an adapter
         for (int r = warp; r < kRows; r += kWarps) {
@@ -371,6 +372,7 @@ __global__ void __launch_bounds__(kThreads, UpRing<W, BACK, JG>::kCtas) up_kerne
     const int      last = min(n_len, first + stride * iters);
     const TileIds  tile(ids, row0, kRows, rows, tab.n);
     grid_wait();  // h is written
+    grid_dependents();
     if (row0 >= rows || first >= n_len) return;
 
     float hv[JG][4][4];  // the first 16 * JG ranks of rows c, c + 8, ...: values 4q .. 4q + 3 of each 16
@@ -579,6 +581,8 @@ __global__ void __launch_bounds__(kThreads, 2) few_kernel(const __grid_constant_
     const int rank = static_cast<int>(cluster_ctarank());
     const int a = static_cast<int>(blockIdx.y);
     const bool none = a == tab.n;
+    grid_wait();
+    grid_dependents();
     // clusters of this adapter: `share` for each 16 of its ranks
     const int clusters = min(static_cast<int>(gridDim.x) / kFewCtas, none ? 1 : share * ((tab.ad[a].rank + 15) / 16));
     if (static_cast<int>(blockIdx.x) >= clusters * kFewCtas) return;
@@ -727,20 +731,21 @@ __global__ void __launch_bounds__(kThreads, 2) few_kernel(const __grid_constant_
             for (int e = 0; e < 4; ++e)
                 part[kwarp * Ring::kPart + (c + 8 * (e >> 1)) * kCols + 8 * (tile0 + n) + 2 * q + (e & 1)] = acc[n][e];
         __syncthreads();
-        for (int i = threadIdx.x; i < Ring::kPart; i += kThreads) {
+        const int n_sums = min(16, total - at) * kCols;  // of the rows that are there
+        for (int i = threadIdx.x; i < n_sums; i += kThreads) {
             float s = part[i];
 #pragma unroll
             for (int v = 1; v < Ring::kKWarps; ++v) s += part[v * Ring::kPart + i];
             part[i] = s;
         }
         cluster_sync();
-        for (int i = threadIdx.x; i < Ring::kPart; i += kThreads) {
+        for (int i = threadIdx.x; i < n_sums; i += kThreads) {
             float s = 0.0f;
 #pragma unroll
             for (int v = 0; v < kFewCtas; ++v) s += ld_cluster(mapa_shared(part + i, v));
             s = i % kCols < r ? s * A.scale : 0.0f;
             hs[i] = s;
-            if (h != nullptr && blockIdx.x == 0 && at + i / kCols < total && i % kCols < ld)
+            if (h != nullptr && blockIdx.x == 0 && i % kCols < ld)
                 h[static_cast<int64_t>(list[at + i / kCols]) * ld + i % kCols] = s;
         }
         cluster_sync();  // every CTA has read the partial sums, and this one's h is complete
@@ -749,6 +754,7 @@ __global__ void __launch_bounds__(kThreads, 2) few_kernel(const __grid_constant_
         for (int g = 0; g < JG; ++g)
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
+                // (rows that are not there hold anything: their sums are not written)
                 const float4 v = *reinterpret_cast<const float4*>(hs + (c + 8 * i) * kCols + 16 * g + 4 * q);
                 split(v.x, hh[g][0][i], ht[g][0][i]);
                 split(v.y, hh[g][0][i + 2], ht[g][0][i + 2]);
@@ -877,25 +883,20 @@ bool vec_rows(const trc_cuda_view* v) {
     return true;
 }
 
-int launch(const void* kernel, dim3 grid, unsigned cluster, size_t smem, bool after, void** args, cudaStream_t s) {
+int launch(const void* kernel, dim3 grid, unsigned cluster, size_t smem, void** args, cudaStream_t s) {
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = grid;
     cfg.blockDim = dim3(kThreads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = s;
     cudaLaunchAttribute at[2];
-    unsigned n = 0;
-    at[n].id = cudaLaunchAttributeClusterDimension;
-    at[n].val.clusterDim.x = cluster;
-    at[n].val.clusterDim.y = at[n].val.clusterDim.z = 1;
-    ++n;
-    if (after) {  // may be set up while the kernel before it drains; it waits for that kernel's results itself
-        at[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-        at[n].val.programmaticStreamSerializationAllowed = 1;
-        ++n;
-    }
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = cluster;
+    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = at;
-    cfg.numAttrs = n;
+    cfg.numAttrs = 2;
     const cudaError_t e = cudaLaunchKernelExC(&cfg, kernel, args);
     if (e != cudaSuccess) {
         cudaGetLastError();
@@ -942,7 +943,7 @@ int run_down(const Adapters& tab, const int32_t* ids, const Rows& x, bool vec, i
     const int st = allow_smem(kernel, smem);
     if (st != TRC_CUDA_OK) return st;
     void* args[] = {const_cast<Adapters*>(&tab), &ids, const_cast<Rows*>(&x), &rows, &k, &h, &ld};
-    return launch(kernel, dim3(static_cast<unsigned>(tiles * cluster), static_cast<unsigned>(slices)), cluster, smem, false, args, s);
+    return launch(kernel, dim3(static_cast<unsigned>(tiles * cluster), static_cast<unsigned>(slices)), cluster, smem, args, s);
 }
 
 template <bool BACK, typename W>
@@ -975,7 +976,7 @@ int run_up(const Adapters& tab, const int32_t* ids, const Rows& base, const Rows
     int cols = static_cast<int>(col_blocks);
     void* args[] = {const_cast<Adapters*>(&tab), &ids, const_cast<Rows*>(&base), const_cast<Rows*>(&d), &rows, &n, &h, &ld, &wr,
                     &iters, &cols};
-    return launch(kernel, grid, 1, smem, true, args, s);
+    return launch(kernel, grid, 1, smem, args, s);
 }
 
 template <bool BACK, typename W>
@@ -1004,7 +1005,7 @@ int run_few(const Adapters& tab, const int32_t* ids, const Rows& x, const Rows& 
     const int64_t parts = std::min<int64_t>(most, static_cast<int64_t>(share) * (ld / 16));
     void* args[] = {const_cast<Adapters*>(&tab), &ids, const_cast<Rows*>(&x), const_cast<Rows*>(&base), const_cast<Rows*>(&d), &rows, &k, &n, &h, &ld,
                     &share};
-    return launch(kernel, dim3(static_cast<unsigned>(parts * kFewCtas), static_cast<unsigned>(tab.n + 1)), kFewCtas, smem, false, args, s);
+    return launch(kernel, dim3(static_cast<unsigned>(parts * kFewCtas), static_cast<unsigned>(tab.n + 1)), kFewCtas, smem, args, s);
 }
 
 template <typename W>

@@ -104,9 +104,6 @@ __device__ __forceinline__ void load_w(const W* p, int have, float (&w)[N]) {
     widen<W, N>(raw, w);
 }
 
-__device__ __forceinline__ void grid_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
-__device__ __forceinline__ void grid_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
-
 __device__ __forceinline__ float ld_cluster(uint32_t addr) {
     float v;
     asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");

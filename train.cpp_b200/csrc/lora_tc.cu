@@ -422,7 +422,10 @@ __global__ void __launch_bounds__(kGradThreads, 2) grad_tc_kernel(const __grid_c
     const Adapter& A = tab.ad[ad];
     float*         out = is_b ? A.db : A.da;
     const int      j0 = blockIdx.y * LD, r = A.rank;
-    if (out == nullptr || j0 >= r) return;  // the whole cluster
+    if (out == nullptr || j0 >= r) {  // the whole cluster
+        grid_wait();
+        return;
+    }
 
     if (threadIdx.x == 256) {
         for (int i = 0; i < 2; ++i) {
@@ -446,6 +449,8 @@ __global__ void __launch_bounds__(kGradThreads, 2) grad_tc_kernel(const __grid_c
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = tmem_slot;
+    grid_wait();
+    grid_dependents();
 
     // This CTA's steps are those of its turn that have a row of the adapter. Which rows: looked up for all of them at once,
     // at the start (step by step every one waited for its ids, and an adapter's first step for all those before it: 25 us
@@ -754,22 +759,28 @@ int run_grad(const Adapters& tab, const int32_t* ids, const CUtensorMap& map_a, 
     cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return cuda_fail(e);
     const int64_t chunks = (ld + LD - 1) / LD, units = (a.strips + b.strips) * chunks * tab.n;
-    // the rows of a strip go to 1 - 8 CTAs: one wave of two CTAs for each SM, at least four steps for each
+    // The rows of a strip go to 1 - 8 CTAs, at least four steps for each, as the least time asks: waves of two CTAs for each
+    // SM, each as long as a CTA's steps (its share of an adapter's rows) and some 20 more for its start and end.
     const int64_t room = 2 * static_cast<int64_t>(std::max(1, sm_count_current())), steps = (rows + kGradRows - 1) / kGradRows;
+    const int64_t share = steps / std::max(1, tab.n) + 1;
+    auto time = [&](unsigned c) { return (units * c + room - 1) / room * (share / c + 20); };
     unsigned cluster = 1;
-    while (cluster < 8 && 2 * cluster * units <= room && 8 * cluster <= steps) cluster *= 2;
+    for (unsigned c = 2; c <= 8 && 4 * static_cast<int64_t>(c) <= steps; c *= 2)
+        if (time(c) < time(cluster)) cluster = c;
     if ((a.strips + b.strips) * static_cast<int64_t>(cluster) > INT32_MAX) return TRC_CUDA_EUNSUPPORTED;
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(static_cast<unsigned>((a.strips + b.strips) * cluster), static_cast<unsigned>(chunks), static_cast<unsigned>(tab.n));
     cfg.blockDim = dim3(kGradThreads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = s;
-    cudaLaunchAttribute at[1];
+    cudaLaunchAttribute at[2];
     at[0].id = cudaLaunchAttributeClusterDimension;
     at[0].val.clusterDim.x = cluster;
     at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = at;
-    cfg.numAttrs = 1;
+    cfg.numAttrs = 2;
     e = cudaLaunchKernelEx(&cfg, kernel, tab, ids, map_a, map_b, a, b, rows, ld, accumulate);
     if (e != cudaSuccess) {
         cudaGetLastError();
@@ -800,7 +811,9 @@ int run(const Adapters& tab, const int32_t* ids, const CUtensorMap& base_map, co
     cfg.dynamicSmemBytes = smem;
     cfg.stream = s;
     cudaLaunchAttribute at[1];
-    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;  // it waits for down's h itself
+    // It waits for down's h itself. It does not let its own successor start early: that one's CTAs, waiting with most of an
+    // SM's shared memory, took 6 % off the step's time at 2048 rows of ranks 64 and 32 in the wrong direction.
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     at[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = at;
     cfg.numAttrs = 1;

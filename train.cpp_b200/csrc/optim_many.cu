@@ -20,6 +20,7 @@
 #include <cstdint>
 
 #include "trc_internal.h"
+#include "trc_ptx.cuh"
 
 namespace trc {
 
@@ -28,7 +29,7 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kRun     = 2048;  // elements that a CTA takes at a time: 8 per thread, 8 blocks of an 8-bit state
 constexpr int kBlock   = TRC_CUDA_STATE8_BLOCK;
-constexpr int kMaxJobs = 480;   // tensors of one launch (31 KB of kernel parameters)
+constexpr int kFewJobs = 32, kMaxJobs = 480;  // tensors of one launch (2 or 31 KB of kernel parameters)
 static_assert(kRun == kThreads * 8 && kBlock == 256, "a warp takes one block of 256, 8 elements per lane");
 
 // 1 / 127^2 and 1 / 255^2: the units of the two square laws.
@@ -51,14 +52,17 @@ struct StepJob {
     int32_t      aligned;    // its vectors may be loaded whole
 };
 
+// Two sizes of table: a launch copies all of its parameters.
+template <int JOBS>
 struct StepBatch {
-    StepJob      job[kMaxJobs];
+    static constexpr int kJobs = JOBS;
     const float* norm;
     AdamwParams  a;
     int32_t      n_jobs;
     int32_t      per;  // a run is kRun * per elements
+    StepJob      job[JOBS];
 };
-static_assert(sizeof(StepBatch) <= 32764, "kernel parameter limit");
+static_assert(sizeof(StepBatch<kMaxJobs>) <= 32764, "kernel parameter limit");
 
 // The tensor that run `run` belongs to (run_begin ascends).
 template <class JOB>
@@ -303,8 +307,10 @@ __device__ __forceinline__ void step_block(const StepJob& J, int64_t b0, const A
     }
 }
 
-template <int BITS>
-__global__ void __launch_bounds__(kThreads, 4) adamw_many_kernel(const __grid_constant__ StepBatch batch) {
+template <int BITS, int JOBS>
+__global__ void __launch_bounds__(kThreads, 4) adamw_many_kernel(const __grid_constant__ StepBatch<JOBS> batch) {
+    grid_wait();
+    grid_dependents();
     // From the last run to the first: the norm's pass read the gradients from the first to the last, so
     // those that are still in L2 come first.
     const int      run = static_cast<int>(gridDim.x - 1 - blockIdx.x);
@@ -392,12 +398,20 @@ struct Span {
     int32_t      aligned;
 };
 
+template <int JOBS>
 struct SpanBatch {
-    Span    job[kMaxSpans];
+    static constexpr int kJobs = JOBS;
     double* partials;
     int32_t n_jobs;
+    Span    job[JOBS];
 };
-static_assert(sizeof(SpanBatch) <= 32764, "kernel parameter limit");
+static_assert(sizeof(SpanBatch<kMaxSpans>) <= 32764, "kernel parameter limit");
+
+struct SumBatch {
+    const double* partials;
+    int64_t       n;
+    float*        out;
+};
 
 __device__ __forceinline__ double block_sum(double s) {
     __shared__ double sh[kThreads / 32];
@@ -410,7 +424,10 @@ __device__ __forceinline__ double block_sum(double s) {
     return s;
 }
 
-__global__ void __launch_bounds__(kThreads) sum_sqr_many_kernel(const __grid_constant__ SpanBatch batch) {
+template <int JOBS>
+__global__ void __launch_bounds__(kThreads) sum_sqr_many_kernel(const __grid_constant__ SpanBatch<JOBS> batch) {
+    grid_wait();
+    grid_dependents();
     const int     run = static_cast<int>(blockIdx.x);
     const Span&   J   = batch.job[job_of(batch.job, batch.n_jobs, run)];
     const int64_t lo = static_cast<int64_t>(run - J.run_begin) * kChunk, hi = min(J.n, lo + kChunk);
@@ -433,11 +450,13 @@ __global__ void __launch_bounds__(kThreads) sum_sqr_many_kernel(const __grid_con
     if (threadIdx.x == 0) batch.partials[run] = s;
 }
 
-__global__ void __launch_bounds__(kThreads) sum_sqr_many_final_kernel(const double* partials, int64_t n, float* out) {
+__global__ void __launch_bounds__(kThreads) sum_sqr_many_final_kernel(const __grid_constant__ SumBatch b) {
+    grid_wait();
+    grid_dependents();
     double s = 0.0;
-    for (int64_t i = threadIdx.x; i < n; i += kThreads) s = __dadd_rn(s, partials[i]);
+    for (int64_t i = threadIdx.x; i < b.n; i += kThreads) s = __dadd_rn(s, b.partials[i]);
     s = block_sum(s);
-    if (threadIdx.x == 0) out[0] = __double2float_rn(s);
+    if (threadIdx.x == 0) b.out[0] = __double2float_rn(s);
 }
 
 bool aligned_to(const void* p, uint64_t bytes) { return (reinterpret_cast<uint64_t>(p) & (bytes - 1)) == 0; }
@@ -448,7 +467,102 @@ int64_t chunks_of(const trc_cuda_span* spans, int n_spans) {
     return c;
 }
 
+// Launches a kernel that may be set up while the one before it on the stream drains: it begins with grid_wait().
+template <class ARGS>
+int launch(void (*kernel)(ARGS), int64_t grid, const ARGS& args, cudaStream_t s) {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(static_cast<unsigned>(grid));
+    cfg.blockDim = dim3(kThreads);
+    cfg.stream = s;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    void* list[] = {const_cast<ARGS*>(&args)};
+    const cudaError_t e = cudaLaunchKernelExC(&cfg, reinterpret_cast<const void*>(kernel), list);
+    if (e != cudaSuccess) {
+        cudaGetLastError();
+        return cuda_fail(e);
+    }
+    note_launch();
+    return TRC_CUDA_OK;
+}
+
 constexpr int64_t kMaxElems = int64_t(1) << 40;  // of one tensor: its runs and chunks fit a grid
+
+template <int JOBS>
+int step_many(const trc_cuda_adamw_job* jobs, int n_jobs, int state_bits, const AdamwParams& a, const float* norm, cudaStream_t s) {
+    const uint64_t state_bytes = state_bits == 32 ? 4 : 1;
+    StepBatch<JOBS> batch;
+    batch.norm = norm;
+    // Long runs share the search for their tensor; runs stay short where there are few: 1 - 4 blocks for each warp, as long as
+    // every SM has 8 runs (202 M elements of 8-bit state, 1 / 2 / 4 blocks: @@).
+    int64_t total = 0;
+    for (int i = 0; i < n_jobs; ++i) total += jobs[i].n;
+    const int64_t wave = 8 * static_cast<int64_t>(std::max(1, sm_count_current())) * kRun;
+    batch.per = total >= 4 * wave ? 4 : total >= 2 * wave ? 2 : 1;
+    const int64_t run_len = static_cast<int64_t>(kRun) * batch.per;
+    batch.a = a;
+    // Batches from the last tensor to the first, as the runs inside a launch.
+    for (int last = n_jobs; last > 0;) {
+        int64_t runs = 0;
+        int first = last;
+        batch.n_jobs = 0;
+        while (first > 0 && last - first < JOBS) {
+            const int64_t r = (jobs[first - 1].n + run_len - 1) / run_len;
+            if (runs + r > INT32_MAX) break;
+            runs += r;
+            --first;
+        }
+        runs = 0;
+        for (int i = first; i < last; ++i) {
+            const trc_cuda_adamw_job& in = jobs[i];
+            if (in.n == 0) continue;
+            StepJob& J  = batch.job[batch.n_jobs++];
+            J.p         = in.param;
+            J.g         = in.grad;
+            J.m         = in.m;
+            J.v         = in.v;
+            J.m_scale   = in.m_scale;
+            J.v_scale   = in.v_scale;
+            J.n         = in.n;
+            J.run_begin = static_cast<int32_t>(runs);
+            J.aligned   = aligned_to(in.param, 16) && aligned_to(in.grad, 16) && aligned_to(in.m, 4 * state_bytes) &&
+                        aligned_to(in.v, 4 * state_bytes);
+            runs += (in.n + run_len - 1) / run_len;
+        }
+        last = first;
+        if (runs == 0) continue;
+        const int st = state_bits == 32 ? launch(&adamw_many_kernel<32, JOBS>, runs, batch, s) : launch(&adamw_many_kernel<8, JOBS>, runs, batch, s);
+        if (st != TRC_CUDA_OK) return st;
+    }
+    return TRC_CUDA_OK;
+}
+
+template <int JOBS>
+int sum_many(const trc_cuda_span* spans, int n_spans, float* out, double* partials, cudaStream_t s) {
+    int64_t done = 0;
+    SpanBatch<JOBS> batch;
+    for (int i = 0; i < n_spans;) {
+        int64_t runs = 0;
+        batch.n_jobs = 0;
+        batch.partials = partials + done;
+        for (; i < n_spans && batch.n_jobs < JOBS; ++i) {
+            const int64_t r = (spans[i].n + kChunk - 1) / kChunk;
+            if (r == 0) continue;
+            if (runs + r > INT32_MAX) break;
+            batch.job[batch.n_jobs++] = Span{spans[i].data, spans[i].n, static_cast<int32_t>(runs),
+                                             aligned_to(spans[i].data, 16) ? 1 : 0};
+            runs += r;
+        }
+        if (runs == 0) continue;
+        const int st = launch(&sum_sqr_many_kernel<JOBS>, runs, batch, s);
+        if (st != TRC_CUDA_OK) return st;
+        done += runs;
+    }
+    return launch(&sum_sqr_many_final_kernel, 1, SumBatch{partials, done, out}, s);
+}
 
 }  // namespace
 
@@ -476,54 +590,10 @@ int trc_cuda_opt_step_adamw_many(const trc_cuda_adamw_job* jobs, int n_jobs, int
                                 !aligned_to(in.v_scale, 4)))
             return TRC_CUDA_EINVAL;
     }
+    const AdamwParams a{params6[0], params6[1], params6[2], params6[3], params6[4], params6[5], max_norm, clip_eps};
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    StepBatch batch;
-    batch.norm = norm;
-    // Long runs share the search for their tensor; runs stay short where there are few: 1 - 4 blocks for each warp, as long as
-    // every SM has 8 runs (202 M elements of 8-bit state, 1 / 2 / 4 blocks: @@).
-    int64_t total = 0;
-    for (int i = 0; i < n_jobs; ++i) total += jobs[i].n;
-    const int64_t wave = 8 * static_cast<int64_t>(std::max(1, sm_count_current())) * kRun;
-    batch.per = total >= 4 * wave ? 4 : total >= 2 * wave ? 2 : 1;
-    const int64_t run_len = static_cast<int64_t>(kRun) * batch.per;
-    batch.a = AdamwParams{params6[0], params6[1], params6[2], params6[3], params6[4], params6[5], max_norm, clip_eps};
-    // Batches from the last tensor to the first, as the runs inside a launch.
-    for (int last = n_jobs; last > 0;) {
-        int64_t runs = 0;
-        int first = last;
-        batch.n_jobs = 0;
-        while (first > 0 && last - first < kMaxJobs) {
-            const int64_t r = (jobs[first - 1].n + run_len - 1) / run_len;
-            if (runs + r > INT32_MAX) break;
-            runs += r;
-            --first;
-        }
-        runs = 0;
-        for (int i = first; i < last; ++i) {
-            const trc_cuda_adamw_job& in = jobs[i];
-            if (in.n == 0) continue;
-            StepJob& J  = batch.job[batch.n_jobs++];
-            J.p         = in.param;
-            J.g         = in.grad;
-            J.m         = in.m;
-            J.v         = in.v;
-            J.m_scale   = in.m_scale;
-            J.v_scale   = in.v_scale;
-            J.n         = in.n;
-            J.run_begin = static_cast<int32_t>(runs);
-            J.aligned   = aligned_to(in.param, 16) && aligned_to(in.grad, 16) && aligned_to(in.m, 4 * state_bytes) &&
-                        aligned_to(in.v, 4 * state_bytes);
-            runs += (in.n + run_len - 1) / run_len;
-        }
-        last = first;
-        if (runs == 0) continue;
-        if (state_bits == 32) adamw_many_kernel<32><<<static_cast<unsigned>(runs), kThreads, 0, s>>>(batch);
-        else adamw_many_kernel<8><<<static_cast<unsigned>(runs), kThreads, 0, s>>>(batch);
-        note_launch();
-        const int st = check_launch();
-        if (st != TRC_CUDA_OK) return st;
-    }
-    return TRC_CUDA_OK;
+    return n_jobs <= kFewJobs ? step_many<kFewJobs>(jobs, n_jobs, state_bits, a, norm, s)
+                              : step_many<kMaxJobs>(jobs, n_jobs, state_bits, a, norm, s);
 }
 
 int trc_cuda_state8_to_f32(int which, const void* codes, const float* scales, float* values, int64_t n, void* stream) {
@@ -575,30 +645,8 @@ int trc_cuda_sum_sqr_many(const trc_cuda_span* spans, int n_spans, float* out, v
         return TRC_CUDA_EINVAL;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     double* partials = static_cast<double*>(workspace);
-    int64_t done = 0;
-    SpanBatch batch;
-    for (int i = 0; i < n_spans;) {
-        int64_t runs = 0;
-        batch.n_jobs = 0;
-        batch.partials = partials + done;
-        for (; i < n_spans && batch.n_jobs < kMaxSpans; ++i) {
-            const int64_t r = (spans[i].n + kChunk - 1) / kChunk;
-            if (r == 0) continue;
-            if (runs + r > INT32_MAX) break;
-            batch.job[batch.n_jobs++] = Span{spans[i].data, spans[i].n, static_cast<int32_t>(runs),
-                                             aligned_to(spans[i].data, 16) ? 1 : 0};
-            runs += r;
-        }
-        if (runs == 0) continue;
-        sum_sqr_many_kernel<<<static_cast<unsigned>(runs), kThreads, 0, s>>>(batch);
-        note_launch();
-        const int st = check_launch();
-        if (st != TRC_CUDA_OK) return st;
-        done += runs;
-    }
-    sum_sqr_many_final_kernel<<<1, kThreads, 0, s>>>(partials, done, out);
-    note_launch();
-    return check_launch();
+    return n_spans <= kFewJobs ? sum_many<kFewJobs>(spans, n_spans, out, partials, s)
+                               : sum_many<kMaxSpans>(spans, n_spans, out, partials, s);
 }
 
 }  // extern "C"

@@ -177,6 +177,13 @@ __device__ __forceinline__ bool mbar_wait_drain(uint64_t* bar, uint32_t parity) 
     }
 }
 
+// A kernel launched with programmatic stream serialization may be set up while the kernel before it on the stream
+// drains; grid_wait() returns once that one has ended and its writes are visible. Until then it touches nothing that
+// another kernel reads or writes. (The adapters' second product, which always follows their first, reads its ids, base
+// and factors before: the first lets it start, grid_dependents(), only after its own wait.)
+__device__ __forceinline__ void grid_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void grid_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
 // ------------------------------------------------------------------ TMA / bulk copies
 __device__ __forceinline__ void tma_load_4d(uint32_t smem_dst, const void* tmap, uint64_t* bar, int c0, int c1,
                                             int c2, int c3) {
