@@ -3,7 +3,11 @@
 //
 // A low-rank adapter gives two small tensors for every projection, hundreds for a model, so one launch
 // per tensor costs more than its work. Here the tensors of a call are a table in the kernel's parameters,
-// cut into runs of 2048 - 8192 elements; one CTA takes one run.
+// cut into runs of 1024 elements; one CTA of four warps takes
+// one run. Many short CTAs overlap one another's loads, roots and stores best (202 M elements, norm and step / 8-bit step and
+// states read back: 128 threads 942 / 915 us, 256 threads 935 / 928, 256 threads that take 2 blocks for each warp in turn 946 /
+// 1103, 4 blocks 977 / 1065; 8 warps on an SM fewer for 80 registers 934 / 1027, more for 48 1155 for the 8-bit form; the next block's
+// loads through a ring of asynchronous copies 1110).
 //
 // 32-bit states: every fp32 operation is rounded by itself, in the order of train_ops.cu's adamw_kernel, so the
 // step is bit-exact with the one-tensor step. 28 bytes for each element leave room for its two divisions and square
@@ -27,10 +31,10 @@ namespace trc {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kRun     = 2048;  // elements that a CTA takes at a time: 8 per thread, 8 blocks of an 8-bit state
+constexpr int kStepThreads = 128, kRun = 1024;  // a CTA of the step: 8 elements per thread, 4 blocks of an 8-bit state
 constexpr int kBlock   = TRC_CUDA_STATE8_BLOCK;
 constexpr int kFewJobs = 32, kMaxJobs = 480;  // tensors of one launch (2 or 31 KB of kernel parameters)
-static_assert(kRun == kThreads * 8 && kBlock == 256, "a warp takes one block of 256, 8 elements per lane");
+static_assert(kRun == kStepThreads * 8 && kBlock == 256, "a warp takes one block of 256, 8 elements per lane");
 
 // 1 / 127^2 and 1 / 255^2: the units of the two square laws.
 constexpr float kUnitM = 1.0f / 16129.0f, kUnitV = 1.0f / 65025.0f;
@@ -59,7 +63,6 @@ struct StepBatch {
     const float* norm;
     AdamwParams  a;
     int32_t      n_jobs;
-    int32_t      per;  // a run is kRun * per elements
     StepJob      job[JOBS];
 };
 static_assert(sizeof(StepBatch<kMaxJobs>) <= 32764, "kernel parameter limit");
@@ -308,7 +311,7 @@ __device__ __forceinline__ void step_block(const StepJob& J, int64_t b0, const A
 }
 
 template <int BITS, int JOBS>
-__global__ void __launch_bounds__(kThreads, 4) adamw_many_kernel(const __grid_constant__ StepBatch<JOBS> batch) {
+__global__ void __launch_bounds__(kStepThreads, 8) adamw_many_kernel(const __grid_constant__ StepBatch<JOBS> batch) {
     grid_wait();
     grid_dependents();
     // From the last run to the first: the norm's pass read the gradients from the first to the last, so
@@ -321,14 +324,10 @@ __global__ void __launch_bounds__(kThreads, 4) adamw_many_kernel(const __grid_co
         clip = __fdiv_rn(batch.a.max_norm, __fadd_rn(__fsqrt_rn(batch.norm[0]), batch.a.clip_eps));
         if (clip > 1.0f) clip = 1.0f;
     }
-    // batch.per blocks for each warp
-    int64_t b0 = static_cast<int64_t>(run - J.run_begin) * (kRun / kBlock) * batch.per + (threadIdx.x >> 5);
-#pragma unroll 1
-    for (int k = 0; k < batch.per; ++k, b0 += kRun / kBlock) {
-        if (b0 * kBlock >= J.n) return;
-        if (J.aligned && (b0 + 1) * kBlock <= J.n) step_block<BITS, true>(J, b0, batch.a, clipped, clip);
-        else step_block<BITS, false>(J, b0, batch.a, clipped, clip);
-    }
+    const int64_t b0 = static_cast<int64_t>(run - J.run_begin) * (kRun / kBlock) + (threadIdx.x >> 5);
+    if (b0 * kBlock >= J.n) return;
+    if (J.aligned && (b0 + 1) * kBlock <= J.n) step_block<BITS, true>(J, b0, batch.a, clipped, clip);
+    else step_block<BITS, false>(J, b0, batch.a, clipped, clip);
 }
 
 // ------------------------------------------------------------------ 8-bit states <-> values
@@ -469,10 +468,10 @@ int64_t chunks_of(const trc_cuda_span* spans, int n_spans) {
 
 // Launches a kernel that may be set up while the one before it on the stream drains: it begins with grid_wait().
 template <class ARGS>
-int launch(void (*kernel)(ARGS), int64_t grid, const ARGS& args, cudaStream_t s) {
+int launch(void (*kernel)(ARGS), int64_t grid, int threads, const ARGS& args, cudaStream_t s) {
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(static_cast<unsigned>(grid));
-    cfg.blockDim = dim3(kThreads);
+    cfg.blockDim = dim3(static_cast<unsigned>(threads));
     cfg.stream = s;
     cudaLaunchAttribute at[1];
     at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -496,13 +495,6 @@ int step_many(const trc_cuda_adamw_job* jobs, int n_jobs, int state_bits, const 
     const uint64_t state_bytes = state_bits == 32 ? 4 : 1;
     StepBatch<JOBS> batch;
     batch.norm = norm;
-    // Long runs share the search for their tensor; runs stay short where there are few: 1 - 4 blocks for each warp, as long as
-    // every SM has 8 runs (202 M elements of 8-bit state, 1 / 2 / 4 blocks: @@).
-    int64_t total = 0;
-    for (int i = 0; i < n_jobs; ++i) total += jobs[i].n;
-    const int64_t wave = 8 * static_cast<int64_t>(std::max(1, sm_count_current())) * kRun;
-    batch.per = total >= 4 * wave ? 4 : total >= 2 * wave ? 2 : 1;
-    const int64_t run_len = static_cast<int64_t>(kRun) * batch.per;
     batch.a = a;
     // Batches from the last tensor to the first, as the runs inside a launch.
     for (int last = n_jobs; last > 0;) {
@@ -510,7 +502,7 @@ int step_many(const trc_cuda_adamw_job* jobs, int n_jobs, int state_bits, const 
         int first = last;
         batch.n_jobs = 0;
         while (first > 0 && last - first < JOBS) {
-            const int64_t r = (jobs[first - 1].n + run_len - 1) / run_len;
+            const int64_t r = (jobs[first - 1].n + kRun - 1) / kRun;
             if (runs + r > INT32_MAX) break;
             runs += r;
             --first;
@@ -530,11 +522,12 @@ int step_many(const trc_cuda_adamw_job* jobs, int n_jobs, int state_bits, const 
             J.run_begin = static_cast<int32_t>(runs);
             J.aligned   = aligned_to(in.param, 16) && aligned_to(in.grad, 16) && aligned_to(in.m, 4 * state_bytes) &&
                         aligned_to(in.v, 4 * state_bytes);
-            runs += (in.n + run_len - 1) / run_len;
+            runs += (in.n + kRun - 1) / kRun;
         }
         last = first;
         if (runs == 0) continue;
-        const int st = state_bits == 32 ? launch(&adamw_many_kernel<32, JOBS>, runs, batch, s) : launch(&adamw_many_kernel<8, JOBS>, runs, batch, s);
+        const int st = state_bits == 32 ? launch(&adamw_many_kernel<32, JOBS>, runs, kStepThreads, batch, s)
+                                          : launch(&adamw_many_kernel<8, JOBS>, runs, kStepThreads, batch, s);
         if (st != TRC_CUDA_OK) return st;
     }
     return TRC_CUDA_OK;
@@ -557,11 +550,11 @@ int sum_many(const trc_cuda_span* spans, int n_spans, float* out, double* partia
             runs += r;
         }
         if (runs == 0) continue;
-        const int st = launch(&sum_sqr_many_kernel<JOBS>, runs, batch, s);
+        const int st = launch(&sum_sqr_many_kernel<JOBS>, runs, kThreads, batch, s);
         if (st != TRC_CUDA_OK) return st;
         done += runs;
     }
-    return launch(&sum_sqr_many_final_kernel, 1, SumBatch{partials, done, out}, s);
+    return launch(&sum_sqr_many_final_kernel, 1, kThreads, SumBatch{partials, done, out}, s);
 }
 
 }  // namespace
@@ -602,7 +595,7 @@ int trc_cuda_state8_to_f32(int which, const void* codes, const float* scales, fl
     if (n == 0) return TRC_CUDA_OK;
     if (codes == nullptr || scales == nullptr || values == nullptr || !aligned_to(scales, 4) || !aligned_to(values, 4))
         return TRC_CUDA_EINVAL;
-    const unsigned grid = static_cast<unsigned>((n + kRun * kToF32 - 1) / (kRun * kToF32));
+    const unsigned grid = static_cast<unsigned>((n + kThreads * 8 * kToF32 - 1) / (kThreads * 8 * kToF32));
     const bool whole = aligned_to(codes, 4) && aligned_to(values, 16);
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     const uint8_t* c = static_cast<const uint8_t*>(codes);
@@ -618,7 +611,7 @@ int trc_cuda_state8_from_f32(int which, const float* values, void* codes, float*
     if (n == 0) return TRC_CUDA_OK;
     if (codes == nullptr || scales == nullptr || values == nullptr || !aligned_to(scales, 4) || !aligned_to(values, 4))
         return TRC_CUDA_EINVAL;
-    const unsigned grid = static_cast<unsigned>((n + kRun - 1) / kRun);
+    const unsigned grid = static_cast<unsigned>((n + kThreads * 8 - 1) / (kThreads * 8));
     const bool whole = aligned_to(codes, 4) && aligned_to(values, 16);
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     uint8_t* c = static_cast<uint8_t*>(codes);
