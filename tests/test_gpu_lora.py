@@ -356,6 +356,79 @@ def test_streams_and_two_calls_at_once(tc):
         near(grads[1][1], wdb[1])
 
 
+def test_calls_follow_what_wrote_their_inputs(tc):
+    """Kernels are set up while the one before drains: they must not read what it still writes. Inputs change
+    between calls on one stream without a wait, and every result is that of its own inputs."""
+    for rows, n, ranks in ((8, 96, (4, 8)), (100, 512, (16, 8)), (700, 2048, (16, 32)), (1500, 1024, (64,))):
+        sets = [make(rows, 512, n, ranks, seed=s) for s in (1, 40, 80)]
+        ad = [(a.clone(), b.clone(), c) for a, b, c in sets[0][0]]
+        ids, x, base, dy = (t.clone() for t in sets[0][1:])
+        grads = grads_of(ad)
+        handle = tc.LoraAdapters(ad, grads)
+        want, got = [], []
+        for wait in (True, False):
+            out = want if wait else got
+            for _ in range(4):
+                for s in sets:
+                    for t, u in zip((ids, x, base, dy), s[1:]):
+                        t.copy_(u)
+                    for (a, b, _), (a2, b2, _) in zip(ad, s[0]):
+                        a.copy_(a2)
+                        b.copy_(b2)
+                    if wait:
+                        torch.cuda.synchronize()
+                    h = tc.lora_h(handle, x)
+                    y = tc.lora(handle, x, ids, base=base, h=h)
+                    if wait:
+                        torch.cuda.synchronize()
+                    dx = tc.lora_back(handle, x, ids, dy, h, base=x)
+                    if wait:
+                        torch.cuda.synchronize()
+                    out.append([y.clone(), dx.clone()] + [g.clone() for pair in grads for g in pair])
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for u, v in zip(want, got) for a, b in zip(u, v))
+        for (y, dx, *_), s in zip(want[:3], sets):
+            wy, wdx, _, _ = formula(s[0], s[1], s[2], s[3], s[4], s[2])
+            near(y, wy)
+            near(dx, wdx)
+
+
+def test_many_rows_of_many_adapters(tc):
+    """More steps of rows than a gradient's CTA looks up at once, and more than one tile for every adapter."""
+    rows, k, n, count = 26_000, 48, 40, 200
+    ad, ids, x, base, dy = make(rows, k, n, (2, 3) * (count // 2), order="runs", none=70)
+    grads = grads_of(ad)
+    handle = tc.LoraAdapters(ad, grads)
+    h = tc.lora_h(handle, x)
+    y = tc.lora(handle, x, ids, base=base, h=h)
+    dx = tc.lora_back(handle, x, ids, dy, h)
+    wy, wdx, wda, wdb = formula(ad, ids, x, base, dy)
+    near(y, wy)
+    near(dx, wdx)
+    for i in range(0, count, 13):
+        near(grads[i][0], wda[i])
+        near(grads[i][1], wdb[i])
+    ids.copy_(ids[torch.randperm(rows, device="cuda")])  # mixed: every step has rows of many adapters
+    tc.lora(handle, x, ids, h=h)
+    tc.lora_back(handle, x, ids, dy, h, need_dx=False)
+    _, _, wda, wdb = formula(ad, ids, x, None, dy)
+    for i in range(0, count, 13):
+        near(grads[i][0], wda[i])
+        near(grads[i][1], wdb[i])
+
+
+def test_one_adapter_without_ids_on_a_long_batch(tc):
+    ad, _, x, base, dy = make(1000, 256, 384, (32,))
+    grads = grads_of(ad)
+    handle = tc.LoraAdapters(ad, grads)
+    h = tc.lora_h(handle, x)
+    y = tc.lora(handle, x, base=base, h=h)
+    dx = tc.lora_back(handle, x, None, dy, h)
+    wy, wdx, wda, wdb = formula(ad, torch.zeros(1000), x, base, dy)
+    for got, want in ((y, wy), (dx, wdx), (grads[0][0], wda[0]), (grads[0][1], wdb[0])):
+        near(got, want)
+
+
 def test_captured_step_follows_its_inputs(tc):
     """A captured forward and backward: replayed after x, ids and the adapters changed in place."""
     rows, k, n = 130, 256, 192

@@ -5,6 +5,15 @@
 //   g[t]  = scale * B^T dy[t]          (down, with B in A's place)
 //   dx[t] = base[t] + A^T g[t]         (up, with A in B's place)
 //   dA    = sum g[t] x[t]^T,  dB = sum dy[t] h[t]^T   (over the adapter's rows)
+//
+// F32 accuracy: every product is three TF32 products of heads and tails (two with a half-precision factor), sums leave the
+// tensor core for fp32 every 16 - 64 terms. The whole is bound by memory up to rank 16 (4 K + 8 N bytes and 2 r (K + N)
+// flops for each row); at rank 64 the narrow product, on mma.sync, is bound by that pipe (278 TFLOP/s of TF32 measured, 93 of
+// split products).
+// Which kernel runs: decode batches the one-launch form (few); else down, then up. up and the gradients run on tcgen05
+// (lora_tc.cu), up from 128 rows on with rows that TMA can address and ranks up to 64, else on the kernel here. down stays on
+// mma.sync: the same scheme on tcgen05 (x to TMEM, clusters over the columns) took 25 us against 24 at 4096 rows of rank 16 and
+// a third more at ranks 64: its CTA's 1400 clocks for a step of 128 rows by 32 columns go into the operand's way to TMEM.
 #include <algorithm>
 #include <cstdint>
 #include <type_traits>
@@ -166,6 +175,9 @@ using False = std::false_type;
 // shared memory and then across the cluster, always in the same order. BACK: x is dy and W is B^T, whose
 // values for one rank are `rank` apart: a lane loads V ranks of one column at once and tile i of a group of V takes
 // rank V * c + i.
+// Measured (rank 16, 4096 rows of 4096: 67 MB): 24 us, 2.8 TB/s; 2048 rows of 14336 (117 MB): 36 us, 3.3 TB/s; at
+// ranks 64 and 32 37 us for 2048 rows of 4096, 71 us for 11008, 45 % of the pipe's cycles. Latency of 16 (rank 16) or 8
+// warps on an SM bounds it.
 template <typename W, bool BACK, int NT, bool VEC>
 __global__ void __launch_bounds__(kThreads, DownRing<W, NT>::kCtas) down_kernel(const __grid_constant__ Adapters tab,
                                                                                    const int32_t* ids, Rows x, int64_t rows, int k_len, float* h, int ld) {
@@ -544,7 +556,8 @@ __global__ void __launch_bounds__(kThreads, UpRing<W, BACK, JG>::kCtas) up_kerne
 // of x shared among its 64 warps; every CTA then adds the 8 CTAs' partial sums up for itself and goes on with its share of
 // the output's columns, whose factor values are already on their way. The last slice of the grid takes the rows without an
 // adapter. Against the two launches of down and up: 64 rows of 16 adapters (ranks 8 - 64, 4096 -> 11008, bf16)
-// @@, one row of one adapter (rank 16, 4096 -> 4096, f16) @@.
+// 23 us against 73, one row of one adapter (rank 16, 4096 -> 4096, f16) 6.7 us against 9.7. What is left is a chain of latencies:
+// ids, the first columns of x and A (3 - 5 us), the sums across the cluster (3 us), the walk over the columns of B.
 constexpr int kFewRows = 256, kFewCtas = 8;
 
 // Two CTAs fit an SM (registers and shared memory). With more than 16 ranks two groups of warps take half of them each in the
@@ -925,7 +938,7 @@ int allow_smem(const void* kernel, size_t smem) {
 
 // Into how many slices the adapters of a tile go, with `most` of them there and `room` for slices in a full grid:
 // at least 4, so that the tiles at the borders between requests, which have two adapters or three, do not take two or three
-// times as long as the rest (2048 rows, ranks 64, 32, 64: @@); a slice without work ends at once.
+// times as long as the rest (2048 rows, ranks 64, 32, 64: 66 -> 37 us for h, 127 -> 70 us for g); a slice without work ends at once.
 int64_t slices_for(int64_t most, int64_t room) { return std::max<int64_t>(1, std::min(most, std::max<int64_t>(room, 4))); }
 
 template <typename W, bool BACK, int NT>
