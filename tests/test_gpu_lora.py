@@ -154,9 +154,10 @@ def test_small_batches_with_all_rows_on_one_adapter(tc, rows, kind):
 
 
 @pytest.mark.parametrize("layout", ["offset", "transposed", "batched", "padded"])
-def test_strides_and_unaligned_rows(tc, layout):
+@pytest.mark.parametrize("rows", [60, 192])
+def test_strides_and_unaligned_rows(tc, layout, rows):
     """x, base and the outputs as parts of larger tensors; what lies between their elements stays."""
-    rows, k, n = 60, 132, 136
+    k, n = 132, 136
     ad, ids, x, base, dy = make(rows, k, n, (16, 12), none=5, order="mixed")
     dx_base = randn(9, rows, k, std=1e-2)
 
@@ -195,6 +196,44 @@ def test_strides_and_unaligned_rows(tc, layout):
     for whole, part in ((out_whole, out), (dx_whole, dx)):
         part.fill_(7.0)
         assert bool((whole == 7.0).all())
+
+
+@pytest.mark.parametrize("rows", [20, 200])
+def test_broadcast_inputs_and_shared_factors(tc, rows):
+    """One row of x, base and dy for all rows (stride 0); two adapters of the same factors with gradients of their own."""
+    ad, ids, x, base, dy = make(rows, 128, 64, (16, 16))
+    ad[1] = (ad[0][0], ad[0][1], 2.0)
+    one = [t[:1].expand(rows, -1) for t in (x, base, dy)]
+    grads = grads_of(ad)
+    handle = tc.LoraAdapters(ad, grads)
+    h = tc.lora_h(handle, one[0])
+    y = tc.lora(handle, one[0], ids, base=one[1], h=h)
+    dx = tc.lora_back(handle, one[0], ids, one[2], h, base=one[0])
+    wy, wdx, wda, wdb = formula(ad, ids, *one, one[0])
+    for got, want in ((y, wy), (dx, wdx), (grads[0][0], wda[0]), (grads[1][0], wda[1]), (grads[0][1], wdb[0]), (grads[1][1], wdb[1])):
+        near(got, want)
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+def test_factors_at_odd_addresses(tc, kind):
+    """Factors that start between 16-byte boundaries, as parts of one buffer, and widths of every remainder."""
+    for rows, k, n in ((9, 128, 64), (50, 131, 66), (150, 128, 64), (150, 132, 68)):
+        ad, ids, x, base, dy = make(rows, k, n, (16, 12), kind)
+        moved = []
+        for a, b, c in ad:
+            flat = torch.zeros(a.numel() + b.numel() + 4, dtype=a.dtype, device="cuda")
+            pa, pb = flat[1:1 + a.numel()].view(a.shape), flat[3 + a.numel():3 + a.numel() + b.numel()].view(b.shape)
+            pa.copy_(a)
+            pb.copy_(b)
+            moved.append((pa, pb, c))
+        grads = grads_of(ad)
+        handle = tc.LoraAdapters(moved, grads)
+        h = tc.lora_h(handle, x)
+        wy, wdx, wda, wdb = formula(ad, ids, x, base, dy)
+        near(tc.lora(handle, x, ids, base=base, h=h), wy)
+        near(tc.lora_back(handle, x, ids, dy, h), wdx)
+        near(grads[1][0], wda[1])
+        near(grads[0][1], wdb[0])
 
 
 def test_without_base_in_place_and_without_ids(tc):
