@@ -141,7 +141,16 @@ __global__ void __launch_bounds__(kTcThreads, 2) up_tc_kernel(const __grid_const
         grid_wait();  // nothing comes before; the bounded waits below start their clocks after it
         for (int b = 0; b < blocks && ok; ++b) {
             const int slot = b % kSlots;
-            uint32_t  y[32];
+            // base first: its way from shared memory overlaps the wait for the sums. 16-byte unit u of row r lies at unit
+            // u ^ (r & 7) (128-byte swizzle).
+            ok = ok && mbar_wait(&bars.slot_full[slot], (b / kSlots) & 1, TRC_DEVERR_WAIT_FULL);
+            uint8_t* row = smem + slot * kSlotBytes + threadIdx.x * 128;
+            float    o[32];
+#pragma unroll
+            for (int u = 0; u < 8; ++u) {
+                const float4 t = add ? *reinterpret_cast<const float4*>(row + ((u ^ (threadIdx.x & 7)) << 4)) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                o[4 * u] = t.x; o[4 * u + 1] = t.y; o[4 * u + 2] = t.z; o[4 * u + 3] = t.w;
+            }
             for (int i = 0; i < n_ad; ++i) {
                 const int s = b * per + i, buf = s & 1;
                 ok = ok && mbar_wait(&bars.d_full[buf], (s >> 1) & 1, TRC_DEVERR_WAIT_ACCUM);
@@ -154,23 +163,11 @@ __global__ void __launch_bounds__(kTcThreads, 2) up_tc_kernel(const __grid_const
                 mbar_arrive(&bars.d_free[buf]);
                 if (my_id == list[i])
 #pragma unroll
-                    for (int e = 0; e < 32; ++e) y[e] = v[e];
+                    for (int e = 0; e < 32; ++e) o[e] += __uint_as_float(v[e]);
             }
-            ok = ok && mbar_wait(&bars.slot_full[slot], (b / kSlots) & 1, TRC_DEVERR_WAIT_FULL);
-            // 16-byte unit u of row r lies at unit u ^ (r & 7) (128-byte swizzle)
-            uint8_t* row = smem + slot * kSlotBytes + threadIdx.x * 128;
 #pragma unroll
-            for (int u = 0; u < 8; ++u) {
-                float4* p = reinterpret_cast<float4*>(row + ((u ^ (threadIdx.x & 7)) << 4));
-                float4  o = add ? *p : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                if (my_id >= 0) {
-                    o.x += __uint_as_float(y[4 * u]);
-                    o.y += __uint_as_float(y[4 * u + 1]);
-                    o.z += __uint_as_float(y[4 * u + 2]);
-                    o.w += __uint_as_float(y[4 * u + 3]);
-                }
-                *p = o;
-            }
+            for (int u = 0; u < 8; ++u)
+                *reinterpret_cast<float4*>(row + ((u ^ (threadIdx.x & 7)) << 4)) = make_float4(o[4 * u], o[4 * u + 1], o[4 * u + 2], o[4 * u + 3]);
             fence_proxy_async_smem();
             ok = named_barrier_and(1, 128, ok);
             if (leader && ok) {
@@ -817,8 +814,8 @@ int run(const Adapters& tab, const int32_t* ids, const CUtensorMap& base_map, co
     cfg.dynamicSmemBytes = smem;
     cfg.stream = s;
     cudaLaunchAttribute at[1];
-    // It waits for down's h itself. It does not let its own successor start early: that one's CTAs, waiting with most of an
-    // SM's shared memory, took 6 % off the step's time at 2048 rows of ranks 64 and 32 in the wrong direction.
+    // It waits for down's h itself. It does not let its own successor start early: that one's CTAs would wait with most of
+    // an SM's shared memory, which made the step of 2048 rows of ranks 64 and 32 6 % slower.
     at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     at[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = at;
