@@ -148,7 +148,7 @@ struct TileIds {
 
 constexpr int kWarps = 8, kThreads = 256;
 
-// Bytes of one stage of a warp's ring: the rows' part and the factor's (grad: h's), and the stages that keep two
+// Bytes of one stage of a warp's ring: the rows' part and the factor's, and the stages that keep two
 // CTAs on an SM where the registers allow it (else one).
 template <typename W, int NT>
 struct DownRing {

@@ -3,11 +3,12 @@
 //
 // A low-rank adapter gives two small tensors for every projection, hundreds for a model, so one launch
 // per tensor costs more than its work. Here the tensors of a call are a table in the kernel's parameters,
-// cut into runs of 1024 elements; one CTA of four warps takes
-// one run. Many short CTAs overlap one another's loads, roots and stores best (202 M elements, norm and step / 8-bit step and
-// states read back: 128 threads 942 / 915 us, 256 threads 935 / 928, 256 threads that take 2 blocks for each warp in turn 946 /
-// 1103, 4 blocks 977 / 1065; 8 warps on an SM fewer for 80 registers 934 / 1027, more for 48 1155 for the 8-bit form; the next block's
-// loads through a ring of asynchronous copies 1110).
+// cut into runs of 1024 elements; one CTA of four warps takes one run. Many short CTAs overlap one another's
+// loads, roots and stores best. 202 M elements, clipped 32-bit step / 8-bit step with the states read back, in us:
+//   four warps, one block of 256 for each         937 /  886
+//   eight warps, one, two or four blocks in turn   935 /  928, 946 / 1103, 977 / 1065
+//   eight warps, one block, 24 warps on an SM (80 registers instead of 64)  934 / 1027
+//   eight warps, eight blocks in turn, the next one's loads through a ring of asynchronous copies  - / 1110
 //
 // 32-bit states: every fp32 operation is rounded by itself, in the order of train_ops.cu's adamw_kernel, so the
 // step is bit-exact with the one-tensor step. 28 bytes for each element leave room for its two divisions and square
