@@ -25,20 +25,13 @@ BLOCK = 256  # elements that share a scale in an 8-bit state
 UNIT_M, UNIT_V = float(np.float32(1 / 127 ** 2)), float(np.float32(1 / 255 ** 2))
 
 
-_module = None
-
-
 def _tc():
-    """The framework's Python module, imported once."""
-    global _module
-    if _module is None:
-        pkg = str(Path(__file__).resolve().parent.parent / "train.cpp_b200")
-        if pkg not in sys.path:
-            sys.path.insert(0, pkg)
-        import trc_cuda
+    pkg = str(Path(__file__).resolve().parent.parent / "train.cpp_b200")
+    if pkg not in sys.path:
+        sys.path.insert(0, pkg)
+    import trc_cuda
 
-        _module = trc_cuda
-    return _module
+    return trc_cuda
 
 
 # ------------------------------------------------------------------ the cases
