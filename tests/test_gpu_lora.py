@@ -395,6 +395,30 @@ def test_streams_and_two_calls_at_once(tc):
         near(grads[1][1], wdb[1])
 
 
+def test_h_on_the_stream_of_its_calls(tc):
+    """h for calls on another stream: its memory is that stream's, so that dropping h while those calls are still
+    running cannot hand it to the current stream's next tensor."""
+    ad, ids, x, base, dy = make(700, 1024, 1536, (16, 8))
+    grads, s = grads_of(ad), torch.cuda.Stream()
+    handle = tc.LoraAdapters(ad, grads)
+    wy, wdx, wda, wdb = formula(ad, ids, x, base, dy)
+    torch.cuda.synchronize()
+    for _ in range(3):
+        h = tc.lora_h(handle, x, stream=s)
+        y = tc.lora(handle, x, ids, base=base, h=h, stream=s)
+        dx = tc.lora_back(handle, x, ids, dy, h, stream=s)
+        at, size = h.data_ptr(), h.shape
+        del h
+        taken = [torch.full(size, float("nan"), device="cuda") for _ in range(8)]  # the current stream's, at once
+        assert at not in [t.data_ptr() for t in taken]
+        torch.cuda.synchronize()
+        near(y, wy)
+        near(dx, wdx)
+        for i in range(2):
+            near(grads[i][0], wda[i])
+            near(grads[i][1], wdb[i])
+
+
 def test_calls_follow_what_wrote_their_inputs(tc):
     """Kernels are set up while the one before drains: they must not read what it still writes. Inputs change
     between calls on one stream without a wait, and every result is that of its own inputs."""

@@ -210,3 +210,14 @@ def test_handles_check_their_tensors():
     with pytest.raises(err, match="share memory"):
         trc_cuda._no_overlap([f(8), *f(16).split(8), (q := f(16))[:9], q[8:]], "x")
     trc_cuda._no_overlap([(q := f(16))[:8], q[8:], q[3:3]], "x")
+
+
+def test_h_belongs_to_the_stream_of_the_calls_that_use_it(monkeypatch):
+    """lora_h allocates as every other buffer of a call is allocated: on the stream that it is given."""
+    asked = []
+    monkeypatch.setattr(trc_cuda, "_scratch", lambda shape, dtype, device, stream: asked.append((shape, dtype, stream)) or torch.empty(shape))
+    handle = type("Handle", (), {"ld": 32})()
+    for x, rows in ((torch.zeros(5, 8), 5), (torch.zeros(2, 3, 8), 6), (torch.zeros(8), 1), (torch.zeros(0, 8), 0)):
+        for stream in (None, object()):
+            assert trc_cuda.lora_h(handle, x, stream=stream).shape == (rows, 32)
+            assert asked.pop() == ((rows, 32), torch.float32, stream) and not asked

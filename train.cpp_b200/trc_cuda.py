@@ -854,10 +854,11 @@ def _check_h(h: torch.Tensor, ad: LoraAdapters, device: int, rows: int, what: st
     return h.data_ptr()
 
 
-def lora_h(adapters: LoraAdapters, x: torch.Tensor) -> torch.Tensor:
-    """An empty buffer for the rows' scale * A x, which lora fills and lora_back takes."""
+def lora_h(adapters: LoraAdapters, x: torch.Tensor, stream=None) -> torch.Tensor:
+    """An empty buffer for the rows' scale * A x, which lora fills and lora_back takes. stream: that of these
+    calls (None: the current one), to which its memory belongs."""
     rows = x.numel() // x.shape[-1] if x.shape[-1] else 0
-    return torch.empty((rows, adapters.ld), dtype=torch.float32, device=x.device)
+    return _scratch((rows, adapters.ld), torch.float32, x.device, stream)
 
 
 def lora(adapters: LoraAdapters, x: torch.Tensor, ids: torch.Tensor | None = None, base: torch.Tensor | None = None,
