@@ -153,6 +153,23 @@ def test_small_batches_with_all_rows_on_one_adapter(tc, rows, kind):
     assert bool((h[ids == 6][:, 16:] == 0).all()) and bool((h[ids == -1] == 0).all())
 
 
+@pytest.mark.parametrize("kind", ["f16", "bf16"])
+@pytest.mark.parametrize("k", [8, 36, 264, 2560])
+@pytest.mark.parametrize("ranks", [(16, 16, 16, 16), (24, 32, 8, 4), (64, 40, 33, 64)], ids=lambda r: f"r{max(r)}")
+def test_decode_batches_of_half_factors_again_and_again(tc, kind, k, ranks):
+    """The two products of a decode batch share a warp's ring in two layouts, between which a lane's places change with
+    half-precision factors: few columns of x (warps without a step), several groups of 16 rows, one call after another."""
+    for rows, n in ((1, 2052), (13, 640), (61, 5000)):
+        ad, ids, x, base, dy = make(rows, k, n, ranks, kind, order="mixed", none=rows // 9)
+        if rows > 16:
+            ids[ids >= 0] = 2  # all of them the same adapter's: one group after another
+        handle = tc.LoraAdapters(ad)
+        assert not tc.lib().trc_cuda_lora_needs_h(handle._arr, len(handle), rows)
+        got = [tc.lora(handle, x, ids, base=base) for _ in range(25)]
+        near(got[0], formula(ad, ids, x, base)[0])
+        assert all(torch.equal(y, got[0]) for y in got)
+
+
 @pytest.mark.parametrize("layout", ["offset", "transposed", "batched", "padded"])
 @pytest.mark.parametrize("rows", [60, 192])
 def test_strides_and_unaligned_rows(tc, layout, rows):

@@ -61,7 +61,8 @@ __device__ __forceinline__ void split_b(float x, uint32_t& head, uint32_t& tail)
 }
 
 // What a warp works on streams through a ring in shared memory: a lane asynchronously copies the 4 - 16 bytes
-// that it will need itself into its own place (so the ring needs no barrier, only the lane's own wait), and takes
+// that it will need itself into its own place (so the ring needs no barrier, only the lane's own wait, as long as its
+// layout stays: where another one follows, few_kernel, the warp meets in between), and takes
 // them into registers some steps later. In flight are thus `stages - 1` steps of every warp, without a register.
 // Loads into registers a step ahead took 15 - 30 % more time than this: the registers for it left 8 warps on
 // an SM.
@@ -710,6 +711,7 @@ __global__ void __launch_bounds__(kThreads, 2) few_kernel(const __grid_constant_
                     for (int e = 0; e < 4; ++e) acc[n][e] += dsum[n][e];
             }
             ring_wait<0>();
+            __syncwarp();  // a lane's places of the next layout were other lanes' in this one (half-precision factors)
         }
         // the first groups of columns set out
         const char* in[2] = {add ? base.row<VEC>(t[0]) : nullptr, add ? base.row<VEC>(t[1]) : nullptr};
