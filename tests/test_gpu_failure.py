@@ -57,3 +57,33 @@ def test_stream_probe_writes_what_it_reads(tc, bulk):
         want[:, :, 0] += j + 1
         assert np.array_equal(o[:, j], want)
     assert bool((out[n16 * 4 * ratio:] == -7).all())
+
+
+@pytest.mark.parametrize("k,n", [(512, 640), (515, 640)], ids=["tma", "copies"])
+def test_adapter_kernels_end_after_an_error(tc, k, n):
+    """With an error recorded, a wait that is not over at once gives up: the adapters' kernels end all the same, the error
+    is still there to be read, and after it has been cleared the next call is right."""
+    g = torch.Generator(device="cuda")
+    g.manual_seed(4)
+    rand = lambda *s: torch.randn(*s, generator=g, device="cuda")  # noqa: E731
+    rows, rank = 700, 24
+    a, b, x, dy = rand(rank, k) * k ** -0.5, rand(n, rank) * rank ** -0.5, rand(rows, k), rand(rows, n)
+    grads = [(torch.zeros_like(a), torch.zeros_like(b))]
+    handle = tc.LoraAdapters([(a, b, 1.0)], grads)
+
+    def step():
+        h = tc.lora_h(handle, x)
+        y = tc.lora(handle, x, h=h)
+        return y, tc.lora_back(handle, x, None, dy, h)
+
+    want = [t.clone() for t in (*step(), *grads[0])]
+    assert tc.device_error() == 0
+    assert tc.selftest_wait_timeout(1_000_000)
+    t0 = time.perf_counter()
+    for _ in range(3):
+        step()
+    torch.cuda.synchronize()
+    assert time.perf_counter() - t0 < 30.0
+    assert tc.device_error() == 8  # the first error, read and cleared
+    assert all(torch.equal(t, u) for t, u in zip((*step(), *grads[0]), want))
+    assert tc.device_error() == 0

@@ -480,6 +480,9 @@ __global__ void __launch_bounds__(kGradThreads, 2) grad_tc_kernel(const __grid_c
         return rank + at * ranks;
     };
     bool ok = true;
+    // A warp's lanes go the same way after a wait, also when it has run out for only some of them: what they do next, votes
+    // and moves to and from TMEM, takes the whole warp.
+    auto wait = [&](uint64_t* bar, uint32_t parity, int code) { return __all_sync(0xFFFFFFFFu, mbar_wait(bar, parity, code)) != 0; };
     float (*sum)[kTile + 4] = reinterpret_cast<float (*)[kTile + 4]>(smem);  // in the place of all that
     constexpr int kStages = S::kStages;
     uint32_t ahead[kStages] = {};  // the rows of the steps in a warp's ring, the oldest step first
@@ -499,7 +502,7 @@ __global__ void __launch_bounds__(kGradThreads, 2) grad_tc_kernel(const __grid_c
         auto put = [&](int s, const float* x, auto pitch, uint32_t mine, bool last) {
             constexpr int kPitch = decltype(pitch)::value;
             const int buf = s & 1;
-            if (s >= 2) ok = ok && mbar_wait(&bars.ab_free[buf], ((s >> 1) - 1) & 1, TRC_DEVERR_WAIT_EMPTY);
+            if (s >= 2) ok = ok && wait(&bars.ab_free[buf], ((s >> 1) - 1) & 1, TRC_DEVERR_WAIT_EMPTY);
             tc_fence_after();
             const uint32_t heads = lane_base + buf * 2 * kGradRows;
 #pragma unroll
@@ -525,7 +528,7 @@ __global__ void __launch_bounds__(kGradThreads, 2) grad_tc_kernel(const __grid_c
         if constexpr (VEC) {
             bool last = false;
             for (int s = 0, stage = 0; !last && ok; ++s) {
-                ok = mbar_wait(&bars.x_full[stage], (s / kStages) & 1, TRC_DEVERR_WAIT_FULL);
+                ok = wait(&bars.x_full[stage], (s / kStages) & 1, TRC_DEVERR_WAIT_FULL);
                 const uint32_t mine = stage_rows[stage];
                 last = stage_last[stage] != 0;
                 if (!ok || mine == 0) break;  // no step at all
@@ -581,7 +584,7 @@ __global__ void __launch_bounds__(kGradThreads, 2) grad_tc_kernel(const __grid_c
         };
         auto add = [&](int q) {  // the sums of steps kGradPromote * q ..
             const int buf = q & 1;
-            ok = ok && mbar_wait(&bars.d_full[buf], (q >> 1) & 1, TRC_DEVERR_WAIT_ACCUM);
+            ok = ok && wait(&bars.d_full[buf], (q >> 1) & 1, TRC_DEVERR_WAIT_ACCUM);
             tc_fence_after();
             __syncwarp();
 #pragma unroll
@@ -602,7 +605,7 @@ __global__ void __launch_bounds__(kGradThreads, 2) grad_tc_kernel(const __grid_c
             turn(fetch, stage == 0 ? kStages - 1 : stage - 1);
             if (ahead[0] == 0) break;
             const int buf = s & 1;
-            if (s >= 2) ok = mbar_wait(&bars.ab_free[buf], ((s >> 1) - 1) & 1, TRC_DEVERR_WAIT_EMPTY);
+            if (s >= 2) ok = wait(&bars.ab_free[buf], ((s >> 1) - 1) & 1, TRC_DEVERR_WAIT_EMPTY);
             copy_wait<kStages - 1>();
             uint8_t* heads = smem + buf * S::kBuf;
 #pragma unroll
@@ -693,6 +696,7 @@ __global__ void __launch_bounds__(kGradThreads, 2) grad_tc_kernel(const __grid_c
                 }
             }
             ok = __shfl_sync(0xFFFFFFFFu, ok ? 1 : 0, 0) != 0;
+            if (!ok) break;  // nothing was asked for in this turn
             go = following != 0;
             mine = following;
             step = after;
