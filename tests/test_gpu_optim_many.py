@@ -248,6 +248,56 @@ def test_state8_edge_blocks(tc, which):
     assert np.isnan(back[7]).all() if which == "v" else (back[7] == 0).all()
 
 
+def encode_v_above_zero(x):
+    """encode(x, "v") with a block's codes of values over 0 raised to the first one that reads back as more than 0."""
+    code, scale = encode(x, "v")
+    every = np.arange(256).astype(F)
+    for row, v, s in zip(code, per_block(x), scale):
+        if np.isfinite(s[0]) and s[0] > 0:
+            u = every * every * s[0]
+            row[v > 0] = np.maximum(row[v > 0], int(np.flatnonzero(u * u > 0)[0]))
+    return code, scale
+
+
+def test_a_second_moment_over_zero_never_vanishes(tc):
+    """Blocks whose roots reach down to where the square of a small code's value is 0 in fp32: from the smallest float
+    on, every v > 0 reads back as more than 0, codes are the restatement's, and zeros stay zeros."""
+    rng = np.random.default_rng(8)
+    blocks = []
+    for e in range(-149, -110, 3):  # the largest v of a block: 2^e
+        v = np.ldexp(1.0, e - rng.integers(0, 40, 256)) * rng.uniform(1, 2, 256)
+        v[0], v[1], v[2] = np.ldexp(1.0, e), 2.0 ** -149, 0.0
+        blocks.append(v.astype(F))
+    x = np.concatenate(blocks + [np.full(3, 2.0 ** -149, dtype=F)])
+    assert (encode(x, "v")[0] != encode_v_above_zero(x)[0]).any()  # the blocks reach that far
+    codes, scales = tc.state8_empty(x.size, "v")
+    tc.state8_from_f32(dev(x), codes, scales)
+    back = host(tc.state8_to_f32(codes, scales))
+    assert ((back > 0) == (x > 0)).all()
+    wc, ws = encode_v_above_zero(x)
+    assert np.array_equal(host(codes), wc.reshape(-1)[:x.size]) and bits(host(scales), ws.reshape(-1))
+    assert bits(back, decode(wc, ws, "v", x.size))
+    # a step from these states, its own new ones among them, without eps: no quotient by zero
+    p6 = [1e-3, 1.0, 1.0, 0.9, 0.999, 0.0]
+    some = x > 0
+    p, g, m = np.zeros(x.size, dtype=F), np.zeros(x.size, dtype=F), np.where(some, F(2.0 ** -60), F(0))
+    P, G, (MC, MS) = dev(p), dev(g), tc.state8_empty(x.size, "m")
+    tc.state8_from_f32(dev(m), MC, MS)
+    step = tc.AdamwMany([P], [G], [MC], [codes], [MS], [scales])
+    m0, v0 = host(tc.state8_to_f32(MC, MS)), back
+    for _ in range(2):
+        before = host(P)
+        step(p6)
+        with np.errstate(all="ignore"):
+            want, m1, v1 = adamw(before, g, m0, v0, p6)
+        assert np.isfinite(host(P)[some]).all() and step_close(host(P)[some], want[some], before[some], F(1))
+        wc, ws = encode_v_above_zero(v1)
+        assert np.array_equal(host(codes), wc.reshape(-1)[:x.size]) and bits(host(scales), ws.reshape(-1))
+        m0, v0 = host(tc.state8_to_f32(MC, MS)), host(tc.state8_to_f32(codes, scales))
+        assert ((v0 > 0) == (v1 > 0)).all()
+        P[~dev(some)] = 0.0  # 0 / 0 where nothing ever was
+
+
 # ------------------------------------------------------------------ the norm
 
 @pytest.mark.parametrize("sizes", SIZES + [[0], [], [16384, 16385], [3] * 2500], ids=lambda s: "x".join(map(str, s[:3])) or "none")

@@ -197,10 +197,11 @@ __device__ __forceinline__ float encode_m(const float (&m)[8], uint32_t (&w)[2])
 }
 
 // root: the approximate roots of v, exact ones below 2^-126. The largest root is the root of the largest value:
-// rounding keeps the order. A v > 0 takes the code 1 at least.
+// rounding keeps the order. A v > 0 takes the code 1 at least, or, where that would read back as 0 (the block's largest root
+// is below 2^-59, so the square of its scale rounds to 0), the first code that does not; 255 never does.
 __device__ __forceinline__ float encode_v(const float (&v)[8], const float (&root)[8], uint32_t (&w)[2]) {
     const float top = __fsqrt_rn(block_max(v));
-    const float per = top > 0.0f ? __fdiv_rn(65025.0f, top) : 0.0f;
+    const float per = top > 0.0f ? __fdiv_rn(65025.0f, top) : 0.0f, scale = __fmul_rn(top, kUnitV);
     w[0] = w[1] = 0;
     if (per > 0.0f) {
         uint32_t c[8];
@@ -212,10 +213,17 @@ __device__ __forceinline__ float encode_v(const float (&v)[8], const float (&roo
 #pragma unroll
             for (int e = 0; e < 8; ++e)
                 c[e] = code_of(fmaxf(__fsqrt_rn(__fmul_rn(__fsqrt_rn(v[e]), per)), v[e] > 0.0f ? 1.0f : 0.0f), off);
+        if (__fmul_rn(scale, scale) == 0.0f) {  // the same for the whole warp
+            uint32_t least = 2;
+            while (least < 255 && decode_v(least, 0, scale) == 0.0f) ++least;
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if (v[e] > 0.0f) c[e] = max(c[e], __float_as_uint(12582912.0f) + least);
+        }
         w[0] = pack4(c[0], c[1], c[2], c[3]);
         w[1] = pack4(c[4], c[5], c[6], c[7]);
     }
-    return __fmul_rn(top, kUnitV);
+    return scale;
 }
 
 __device__ __forceinline__ float root_of(float v) {
