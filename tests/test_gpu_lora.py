@@ -568,6 +568,35 @@ def test_refusals(tc):
         tc.lora(tc.LoraAdapters([]), x, ids)
 
 
+@pytest.mark.parametrize("rows", [8, 200])
+def test_outputs_apart_from_what_is_read(tc, rows):
+    """Square projections invite it: the output in x's place, dx in dy's. Refused, because kernels still read these
+    after the first rows are written. Halves of one buffer, and the base's place, are fine."""
+    ad, ids, x, base, dy = make(rows, 64, 64, (8, 4))
+    grads, err = grads_of(ad), tc.TrcCudaError
+    handle = tc.LoraAdapters(ad, grads)
+    h = tc.lora_h(handle, x)
+    with pytest.raises(err, match="out shares memory"):
+        tc.lora(handle, x, ids, base=base, out=x)
+    with pytest.raises(err, match="out shares memory"):
+        tc.lora(handle, x[:-1], ids[:-1], base=base[:-1], out=base[1:])
+    with pytest.raises(err, match="out shares memory"):
+        tc.lora(handle, x[:2], ids[:2], out=h.view(-1)[:128].view(2, 64), h=h[:2])
+    for other in (x, dy, dy[:1].expand(rows, -1)):
+        with pytest.raises(err, match="dx shares memory"):
+            tc.lora_back(handle, x, ids, dy, h, dx=other)
+    two = torch.empty(rows, 128, device="cuda")
+    xs, out = two[:, :64], two[:, 64:]
+    xs.copy_(x)
+    wy, wdx, wda, wdb = formula(ad, ids, x, base, dy, base)
+    near(tc.lora(handle, xs, ids, base=base, out=out, h=h), wy)
+    out.copy_(base)
+    near(tc.lora_back(handle, xs, ids, dy, h, base=out, dx=out), wdx)
+    for i in range(2):
+        near(grads[i][0], wda[i])
+        near(grads[i][1], wdb[i])
+
+
 def test_beside_a_packed_projection_through_a_training_step(tc):
     """The use they are for: y = W x + adapter from a packed weight, its gradients, the clipped AdamW step of all
     factors, and the next forward pass with them."""

@@ -221,3 +221,31 @@ def test_h_belongs_to_the_stream_of_the_calls_that_use_it(monkeypatch):
         for stream in (None, object()):
             assert trc_cuda.lora_h(handle, x, stream=stream).shape == (rows, 32)
             assert asked.pop() == ((rows, 32), torch.float32, stream) and not asked
+
+
+def test_shared_memory_of_strided_tensors():
+    """Exactly the tensors with an element in common: against the sets of their elements' places."""
+    buf = torch.zeros(600)
+    views = [buf[:60], buf[59:90], buf[60:120], buf[:240].view(10, 24)[:, :12], buf[:240].view(10, 24)[:, 12:], buf[:240].view(10, 24)[:, 11:13],
+             buf[:240].view(10, 24).t()[5:7], buf[:240].view(2, 5, 24)[:, :4, 2:9], buf[4:300:3], buf[5:300:3], buf[7:301:6], buf[3:3],
+             buf[:24].expand(10, 24), buf[12:24].expand(4, 3, 12), buf[500], buf[:512].view(2, 4, 8, 8).permute(3, 0, 2, 1)[::2]]
+    places = [set((torch.arange(600).as_strided(v.shape, v.stride(), v.storage_offset())).reshape(-1).tolist()) for v in views]
+    for v, at in zip(views, places):
+        for u, there in zip(views, places):
+            assert trc_cuda._shares_memory(v, u) == bool(at & there)
+
+
+def test_an_output_may_be_its_base_and_nothing_else():
+    err, apart = trc_cuda.TrcCudaError, trc_cuda._apart
+    out, x, h = torch.zeros(8, 16), torch.zeros(8, 16), torch.zeros(8, 16)
+    apart(out, (x, None, h), None, "out")
+    apart(out, (x, h), out, "out")
+    apart(out, (x, h), out.view(1, 8, 16), "out")  # the same places
+    both = torch.zeros(8, 32)
+    apart(both[:, :16], (both[:, 16:],), None, "out")  # side by side
+    apart(out[:0], (out,), None, "out")
+    for read, base in (((out,), None), ((x, out[7:]), None), ((out.t(),), out), ((x,), out[:1].expand(8, 16))):
+        with pytest.raises(err, match="out shares memory"):
+            apart(out, read, base, "out")
+    with pytest.raises(err, match="out shares memory"):
+        apart(both[1:, :16], (x,), both[:7, :16], "out")  # a row behind

@@ -30,6 +30,7 @@ import struct
 from pathlib import Path
 from typing import Sequence
 
+import numpy as np
 import torch
 
 PKG = Path(__file__).resolve().parent
@@ -747,6 +748,47 @@ def _no_overlap(tensors: Sequence[torch.Tensor], what: str) -> None:
             raise TrcCudaError(f"{what}: two of the written tensors share memory")
 
 
+class _Place:
+    """Where a tensor's elements lie, as numpy takes it to compare places; nothing is read there."""
+
+    def __init__(self, t: torch.Tensor):
+        size = t.element_size()
+        self.__array_interface__ = {"version": 3, "typestr": f"|V{size}", "shape": tuple(t.shape), "data": (t.data_ptr(), True),
+                                    "strides": tuple(size * s for s in t.stride())}
+
+
+def _range(t: torch.Tensor) -> tuple[int, int]:
+    """The addresses between which a tensor's elements lie."""
+    at, n = t.data_ptr(), t.numel()
+    if n and not t.is_contiguous():
+        n = 1
+        for d, s in zip(t.shape, t.stride()):
+            n += (d - 1) * s
+    return at, at + n * t.element_size()
+
+
+def _shares_memory(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether two tensors of any strides have an element's memory in common (rows side by side in one buffer have not)."""
+    (first_a, end_a), (first_b, end_b) = _range(a), _range(b)
+    if end_a <= first_b or end_b <= first_a or not a.numel() or not b.numel():
+        return False
+    try:
+        return bool(np.shares_memory(np.asarray(_Place(a)), np.asarray(_Place(b)), max_work=100_000))
+    except np.exceptions.TooHardError:
+        return True
+
+
+def _apart(out: torch.Tensor, read: Sequence[torch.Tensor | None], base: torch.Tensor | None, what: str) -> None:
+    """Raises if a call's output shares memory with what the call reads; base may be the output itself."""
+    if base is not None and base is not out:
+        where = lambda t: (t.data_ptr(), [d for d in zip(t.shape, t.stride()) if d[0] != 1])  # noqa: E731
+        if where(base) != where(out):
+            read = (*read, base)
+    for t in read:
+        if t is not None and _shares_memory(out, t):
+            raise TrcCudaError(f"{what} shares memory with a tensor that the call reads")
+
+
 # ------------------------------------------------------------------ low-rank adapters
 
 TYPE_F16, TYPE_BF16 = 1, 30
@@ -865,7 +907,7 @@ def lora(adapters: LoraAdapters, x: torch.Tensor, ids: torch.Tensor | None = Non
          out: torch.Tensor | None = None, h: torch.Tensor | None = None, stream=None) -> torch.Tensor:
     """out[t] = base[t] + scale * B (A x[t]) with the adapter ids[t] of each row t of x (..., K); a row
     whose id is no adapter's (-1) keeps its base. base (..., N) is the shared projection's output (None: 0)
-    and may be `out` itself. ids: int32, one for each row; None: the single adapter everywhere.
+    and may be `out` itself, which shares memory with nothing else that is read. ids: int32, one for each row; None: the single adapter everywhere.
     h: a buffer of lora_h to keep for lora_back."""
     n = adapters.n if base is None and out is None else (base if base is not None else out).shape[-1]
     if n is None:
@@ -876,6 +918,8 @@ def lora(adapters: LoraAdapters, x: torch.Tensor, ids: torch.Tensor | None = Non
     vb = None if base is None else _rows_view(base, device, lead, n, "lora: base")
     if out is None:
         out = _scratch(lead + (n,), torch.float32, x.device, stream)
+    else:
+        _apart(out, (x, h), base, "lora: out")
     vd = _rows_view(out, device, lead, n, "lora: out")
     if h is None and L.trc_cuda_lora_needs_h(adapters._arr, adapters._n, rows):
         h = _scratch((rows, adapters.ld), torch.float32, x.device, stream)
@@ -892,7 +936,8 @@ def lora_back(adapters: LoraAdapters, x: torch.Tensor, ids: torch.Tensor | None,
               accumulate: bool = False, stream=None) -> torch.Tensor | None:
     """The gradients of lora for the upstream gradient dy (..., N): writes (accumulate: adds to) the adapters'
     dA and dB and returns dx = base + A^T (scale * B^T dy), base being the gradient that the shared
-    projection's backward gives (None: 0; it may be `dx` itself). need_dx=False: no dx, returns None.
+    projection's backward gives (None: 0; it may be `dx` itself, which shares memory with nothing else that is
+    read). need_dx=False: no dx, returns None.
     x, ids and h are those of the forward call."""
     k, n = x.shape[-1], dy.shape[-1]
     device, rows = _lora_args(adapters, x, ids, n, "lora_back")
@@ -902,7 +947,9 @@ def lora_back(adapters: LoraAdapters, x: torch.Tensor, ids: torch.Tensor | None,
     ptr = _check_h(h, adapters, device, rows, "lora_back")
     if not need_dx and (dx is not None or base is not None):
         raise TrcCudaError("lora_back: dx and base go with need_dx")
-    if need_dx and dx is None:
+    if dx is not None:
+        _apart(dx, (x, dy, h), base, "lora_back: dx")
+    elif need_dx:
         dx = _scratch(x.shape, torch.float32, x.device, stream)
     vd = None if dx is None else _rows_view(dx, device, lead, k, "lora_back: dx")
     vb = None if base is None else _rows_view(base, device, lead, k, "lora_back: base")
