@@ -391,3 +391,19 @@ def test_refusals(tc):
     with pytest.raises(err, match="scales"):
         tc.state8_to_f32(tc.state8_empty(300, "m")[0], f(1))
     tc.AdamwMany([], [], [], [])(P6)
+
+
+def test_gradients_share_memory_with_one_another_only(tc):
+    """One gradient for two tensors is right; a gradient in the place of what the step writes is refused."""
+    err, x = tc.TrcCudaError, tensors([900] * 7, 3, 0.1)
+    P, G, M, V = [dev(x[0]), dev(x[1])], dev(x[2]), [dev(x[3]), dev(x[4])], [dev(x[5] ** 2), dev(x[6] ** 2)]
+    tc.AdamwMany(P, [G, G], M, V)(P6)
+    for i in range(2):
+        p, m, v = adamw(x[i], x[2], x[3 + i], x[5 + i] ** 2, P6)
+        assert bits(host(P[i]), p) and bits(host(M[i]), m) and bits(host(V[i]), v)
+    for other in (P[0], P[1], M[1], V[0]):
+        with pytest.raises(err, match="one that is read"):
+            tc.AdamwMany(P, [G, other], M, V)
+    whole = torch.zeros(2000, device="cuda")
+    with pytest.raises(err, match="one that is read"):
+        tc.AdamwMany([whole[:900], P[1]], [whole[800:1700], G], M, V)

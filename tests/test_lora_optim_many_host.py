@@ -249,3 +249,15 @@ def test_an_output_may_be_its_base_and_nothing_else():
             apart(out, read, base, "out")
     with pytest.raises(err, match="out shares memory"):
         apart(both[1:, :16], (x,), both[:7, :16], "out")  # a row behind
+
+
+def test_what_is_written_and_what_is_read():
+    """Read tensors may share memory with one another, and none with a written one, in whatever order they lie."""
+    q, err, apart = torch.zeros(64), trc_cuda.TrcCudaError, trc_cuda._no_overlap
+    apart([q[:8], q[24:32]], "x", read=[q[8:24], q[8:24], q[10:20], q[32:], q[3:3]])
+    for written, read in (([q[8:16]], [q[:9]]), ([q[8:16]], [q[15:20]]), ([q[8:16]], [q]), ([q], [q[8:16]]), ([q[8:16]], [q[8:16]]),
+                          ([q[:4], q[40:44]], [q[8:50], q[10:12]]), ([q[8:16]], [q[9:10], q[30:]])):
+        with pytest.raises(err, match="one that is read"):
+            apart(written, "x", read=read)
+    with pytest.raises(err, match="written tensors share"):
+        apart([q[:8], q[:20], q[7:9]], "x", read=[q[30:]])

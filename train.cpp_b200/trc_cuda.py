@@ -740,12 +740,20 @@ def _on_current_device(t: torch.Tensor, what: str) -> None:
         raise TrcCudaError(f"{what}: the tensor is on {t.device}, the current device is cuda:{torch.cuda.current_device()}")
 
 
-def _no_overlap(tensors: Sequence[torch.Tensor], what: str) -> None:
-    """Raises if two of these contiguous tensors, all of them written by one launch, share memory."""
-    spans = sorted((t.data_ptr(), t.data_ptr() + t.numel() * t.element_size()) for t in tensors if t.numel())
-    for (_, end), (start, _) in zip(spans, spans[1:]):
-        if start < end:
+def _no_overlap(tensors: Sequence[torch.Tensor], what: str, read: Sequence[torch.Tensor] = ()) -> None:
+    """Raises if two of these contiguous tensors, all of them written by one launch, share memory, or one of them
+    and one that the launch only reads."""
+    spans = sorted([(*_range(t), True) for t in tensors if t.numel()] + [(*_range(t), False) for t in read if t.numel()])
+    write_end = read_end = 0  # of the spans so far
+    for start, end, written in spans:
+        if written and start < write_end:
             raise TrcCudaError(f"{what}: two of the written tensors share memory")
+        if start < (read_end if written else write_end):
+            raise TrcCudaError(f"{what}: a written tensor shares memory with one that is read")
+        if written:
+            write_end = max(write_end, end)
+        else:
+            read_end = max(read_end, end)
 
 
 class _Place:
@@ -977,7 +985,8 @@ def _check_part(t: torch.Tensor, dtype: torch.dtype, numel: int, what: str) -> i
 class AdamwMany:
     """AdamW over many tensors at once: params and grads are lists of float32 tensors; m and v their states,
     either float32, or int8 (m) and uint8 (v) codes with m_scale and v_scale, float32 tensors of one scale
-    for each STATE8_BLOCK elements (state8_empty gives a new tensor's). All are updated in place.
+    for each STATE8_BLOCK elements (state8_empty gives a new tensor's). All are updated in place; only gradients
+    may share memory, with one another.
     The table is built and checked once; a call is one step: params6 as in opt_step_adamw_; norm (a
     float32 CUDA tensor of one element, SumSqrMany's) clips the gradients to max_norm on the way in."""
 
@@ -1003,7 +1012,7 @@ class AdamwMany:
                 e.m_scale = _check_part(m_scale[i], torch.float32, blocks, f"AdamwMany: m_scale[{i}]")
                 e.v_scale = _check_part(v_scale[i], torch.float32, blocks, f"AdamwMany: v_scale[{i}]")
         written = [*params, *m, *v, *(m_scale or ()), *(v_scale or ())]
-        _no_overlap(written, "AdamwMany")
+        _no_overlap(written, "AdamwMany", read=grads)
         self._device = params[0].get_device() if self._n else None
 
     def __len__(self) -> int:
