@@ -363,7 +363,9 @@ typedef struct trc_cuda_lora_adapter {
 int64_t trc_cuda_lora_h_ld(const trc_cuda_lora_adapter* adapters, int n_adapters);
 
 /* 1 if trc_cuda_lora has to be given h for so many rows, 0 if h may be null (a decode batch, whose two
- * products are one launch); a negative status if an adapter is not valid. */
+ * products are one launch); a negative status if an adapter is not valid. The rows' ids are on the device, so the
+ * rule knows only how many rows and adapters there are: a decode batch of up to 16 rows for each adapter. If nearly all
+ * of its rows have one and the same adapter, a call with that adapter alone is faster. */
 int trc_cuda_lora_needs_h(const trc_cuda_lora_adapter* adapters, int n_adapters, int64_t rows);
 
 /* d[:, t] = base[:, t] + scale * B (A x[:, t]) with the adapter ids[t] of row t.
@@ -403,7 +405,7 @@ int trc_cuda_lora_back(int type, const trc_cuda_lora_adapter* adapters, int n_ad
                        void* stream);
 
 /* ------------------------------------------------------------------ the optimizer over many tensors
- * One launch (per 256 tensors) for a step that trc_cuda_opt_step_adamw takes tensor by tensor, with
+ * One launch (per 480 tensors) for a step that trc_cuda_opt_step_adamw takes tensor by tensor, with
  * the states in 32 bits, or in 8 bits with one float scale for each TRC_CUDA_STATE8_BLOCK
  * elements of a tensor (its last block may be shorter). The 8-bit forms:
  *     first moment   m = c |c| scale,        c an int8 in -127 .. 127   (scale = max|m| / 127^2)

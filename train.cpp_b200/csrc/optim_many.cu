@@ -4,7 +4,8 @@
 // A low-rank adapter gives two small tensors for every projection, hundreds for a model, so one launch
 // per tensor costs more than its work. Here the tensors of a call are a table in the kernel's parameters,
 // cut into runs of 1024 elements; one CTA of four warps takes one run. Many short CTAs overlap one another's
-// loads, roots and stores best. 202 M elements, clipped 32-bit step / 8-bit step with the states read back, in us:
+// loads, roots and stores best. 202 M elements, clipped 32-bit step / 8-bit step with the states read back, in us, as
+// the forms compared when they were tried (the kept one, the first, since took 937 - 951 / 888 - 1004 on several machines):
 //   four warps, one block of 256 for each         937 /  886
 //   eight warps, one, two or four blocks in turn   935 /  928, 946 / 1103, 977 / 1065
 //   eight warps, one block, 24 warps on an SM (80 registers instead of 64)  934 / 1027
@@ -18,8 +19,10 @@
 // root (5 * 2^-23 of the step at most). A code is round(sqrt(x * per)): the approximate square root (2^-23)
 // decides it except next to a border, where the rounded one does. Codes become numbers and numbers codes through
 // the low bits of 2^23 + c, because the conversion unit is the one that the roots need. 83 instructions for each element were
-// left of 126 (conversions, four rounded roots, two rounded quotients: 1144 us for 202 M elements; now about 585 us, 5.5 TB/s: what
-// bounds it is their latency at 32 warps on an SM, no longer one unit).
+// left of 126 (conversions, four rounded roots, two rounded quotients): 202 M elements take 585 - 700 us, 4.7 - 5.6 TB/s.
+// What bounds it is their latency at 32 warps on an SM, no longer one unit. With a rounded root and rounded quotients in the
+// parameter's own step, measured in turn and with the states read back: 1140 us against 967. 64 registers leave 32 - 36
+// bytes of a thread in local memory.
 #include <cuda_runtime.h>
 
 #include <algorithm>

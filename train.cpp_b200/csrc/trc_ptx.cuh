@@ -179,8 +179,9 @@ __device__ __forceinline__ bool mbar_wait_drain(uint64_t* bar, uint32_t parity) 
 
 // A kernel launched with programmatic stream serialization may be set up while the kernel before it on the stream
 // drains; grid_wait() returns once that one has ended and its writes are visible. Until then it touches nothing that
-// another kernel reads or writes. (The adapters' second product, which always follows their first, reads its ids, base
-// and factors before: the first lets it start, grid_dependents(), only after its own wait.)
+// another kernel reads or writes. (The adapters' second product, which always follows their first, reads its ids before,
+// and on tcgen05 its base: the first lets it start, grid_dependents(), only after its own wait, so what wrote these has
+// ended. Factors and h it reads after.)
 __device__ __forceinline__ void grid_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ __forceinline__ void grid_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 

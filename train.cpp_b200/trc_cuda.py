@@ -987,7 +987,8 @@ class AdamwMany:
     either float32, or int8 (m) and uint8 (v) codes with m_scale and v_scale, float32 tensors of one scale
     for each STATE8_BLOCK elements (state8_empty gives a new tensor's). All are updated in place; only gradients
     may share memory, with one another.
-    The table is built and checked once; a call is one step: params6 as in opt_step_adamw_; norm (a
+    The table is built and checked once, 2.5 ms for 448 tensors, and holds their addresses, so keep the gradients'
+    memory from step to step: gradients that are freed and made anew need a new handle. A call is one step: params6 as in opt_step_adamw_; norm (a
     float32 CUDA tensor of one element, SumSqrMany's) clips the gradients to max_norm on the way in."""
 
     def __init__(self, params, grads, m, v, m_scale=None, v_scale=None):
