@@ -413,10 +413,11 @@ int trc_cuda_lora_back(int type, const trc_cuda_lora_adapter* adapters, int n_ad
  * The square law spends the codes on small values: neighbouring codes at the top are 1.6 % (m) and
  * 0.8 % (sqrt(v)) apart, and the smallest nonzero value is 1/16129 (m) and 1/65025 (sqrt(v)) of the block's
  * largest. Codes are rounded to nearest in the code; a v > 0 never takes a code that reads back as 0, so no step
- * is divided by a vanished second moment: where the code 1 would (its v, the square of the block's scale, is at most
- * 2^-150, which is 0 in fp32: the block's largest sqrt(v) is below 2^-59), the first code that does not. A block whose largest |m| is below 2^-100 is stored as zero. A
- * block that holds an infinity or a NaN gets the scale NaN: all of it reads back as NaN. Zero codes with
- * zero scales are the initial state. */
+ * is divided by a vanished second moment: where the code 1 would (its v, the square of the block's
+ * scale, is at most 2^-150, which is 0 in fp32: the block's largest sqrt(v) is below 2^-59), the first
+ * code that does not. A block whose largest |m| is below 2^-100 is stored as zero. A block that holds
+ * an infinity or a NaN gets the scale NaN: all of it reads back as NaN. Zero codes with zero scales
+ * are the initial state. */
 #define TRC_CUDA_STATE8_BLOCK 256
 
 typedef struct trc_cuda_adamw_job {
